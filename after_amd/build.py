@@ -17,8 +17,11 @@ ARCH = "gfx950"
 # AGPRs inside the MFMA block and copies every accumulator VGPR<->AGPR around it, once per K
 # slab (3064 v_accvgpr moves in gemm.hip alone; measured +25 % loop time in the 9-accumulator
 # split-K GEMM).  gfx950 has a unified 512-register file, so nothing is gained by AGPRs here.
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32.  hipcc -O3 forms them by itself from ordinary float code, and some of their
+# forms have given wrong results on this hardware now and then; the scalar forms round the same.  (hipcc's host pass warns
+# that it does not know the feature.)
 FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
-         "-mllvm", "-amdgpu-mfma-vgpr-form"]
+         "-mllvm", "-amdgpu-mfma-vgpr-form", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 # The kernels were tuned and validated with this hipcc: register budgets (scripts/kernel_regs.py: the persistent samplers sit
