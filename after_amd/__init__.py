@@ -7,6 +7,7 @@ from .diffusion import DenoiserV2, RectifiedFlow, Encoder1D, ECAPATDNN, UNET1D  
 from .autoencoder import AutoEncoder  # noqa: F401
 
 from .streaming import Streamer, MidiStreamer  # noqa: F401
+from .attention import attend_packed, KVCache4  # noqa: F401
 
 __all__ = ["configs", "DenoiserV2", "RectifiedFlow", "AutoEncoder", "Encoder1D", "ECAPATDNN",
-           "Streamer", "MidiStreamer", "UNET1D"]
+           "Streamer", "MidiStreamer", "UNET1D", "attend_packed", "KVCache4"]

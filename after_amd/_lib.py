@@ -48,6 +48,11 @@ class EcapaCfg(ctypes.Structure):
                 ("use_tanh", c_int)]
 
 
+class KV4(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("keys", "key_scales", "values", "value_scales", "weights", "lengths", "failed")] + \
+               [(n, c_int) for n in ("rows", "kv_heads", "head_dim", "capacity")]
+
+
 class AFTERHipError(RuntimeError):
     pass
 
@@ -149,6 +154,15 @@ SIGNATURES = {
     "after_gemm_x6_offset": (ctypes.c_longlong, [c_int, c_int, c_int, c_int]),
     "after_gemm_x6": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int,
                               c_int, c_int, c_int, c_int, c_void_p]),
+    "after_attend_packed": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_void_p, c_void_p,
+                                    c_int, c_int, c_int, c_int] + [c_longlong] * 8 + [c_float, c_int, c_int, c_int, c_int, c_void_p]),
+    "after_kv4_append": (c_int, [POINTER(KV4), c_void_p, c_void_p, c_int, c_void_p, c_int] + [c_longlong] * 5 + [c_void_p]),
+    "after_kv4_truncate": (c_int, [POINTER(KV4), c_void_p, c_void_p]),
+    "after_kv4_read": (c_int, [POINTER(KV4), c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p]),
+    "after_kv4_attend_workspace": (c_int, [POINTER(KV4), c_int, c_int, c_int, POINTER(c_longlong)]),
+    "after_kv4_attend": (c_int, [POINTER(KV4), c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong, c_float,
+                                 c_int, c_float, c_void_p, c_longlong, c_void_p]),
+    "after_kv4_evict": (c_int, [POINTER(KV4), POINTER(KV4), c_int, c_int, c_void_p, c_void_p]),
 }
 
 

@@ -1,0 +1,257 @@
+"""Attention over sequences of different lengths: of whole prompts (`attend_packed`), and over a key / value cache that is held
+in four bits (`KVCache4`), next to the attention and the streaming K/V caches inside `DenoiserV2`
+(after/diffusion/networks/transformerv2.py:62-235).  fp32, bf16 and fp16 tensors; inference only, like the rest of the package;
+hand-written HIP kernels behind the C ABI of include/after_hip.h, no fallback.
+
+    cache = KVCache4(rows=4, kv_heads=8, head_dim=128, capacity=16384)
+    y = attend_packed(q, k, v, starts)                       # the prompts, one behind the other
+    cache.append(k, v, starts)
+    cache.attend(q_last, accumulate=True)                    # which slots do the last tokens look at?
+    small = KVCache4(4, 8, 128, capacity=4096)
+    cache.evict(small, keep=2048, recent=64)                 # keep those, and the newest
+    while ...:                                               # one token per row and step
+        small.append(k1, v1)                                 # [rows, 1, kv_heads, head_dim]
+        y = small.attend(q1)                                 # [rows, 1, heads, head_dim]
+"""
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _operand(t, name, dims, device=None, dtype=None):
+    """A tensor the kernels can address: fp32 / bf16 / fp16 on the GPU, channels contiguous, strides and base multiples of 16
+    bytes -- a view of a fused projection is taken as it is, anything else is copied."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise _lib.AFTERHipError(f"{name} is on {t.device}: after_amd runs on MI355X only (HIP kernels)")
+    if t.dtype not in _TYPES:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if t.dim() != dims:
+        raise ValueError(f"{name} must have {dims} dimensions, got {tuple(t.shape)}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(f"{name} requires a gradient: after_amd is inference only (use torch.no_grad())")
+    size = t.element_size()
+    if t.numel() and (t.stride(-1) != 1 or t.data_ptr() % 16 or any(s * size % 16 for s in t.stride()[:-1])):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _starts(t, name, n, device):
+    """int32 [n + 1] on the device (n None: any)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype != torch.int32 or t.dim() != 1 or t.device != device:
+        raise ValueError(f"{name} must be a one-dimensional int32 tensor on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.numel() != n + 1 if n is not None else t.numel() < 1:
+        raise ValueError(f"{name} has {t.numel()} entries, expected {'one more than sequences' if n is None else n + 1}")
+    return t.contiguous()
+
+
+def _scale(scale, dim):
+    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, got {scale}")
+    return scale
+
+
+def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=True, window=None, chunk=1, scale=None, out=None):
+    """Attention of packed sequences (include/after_hip.h: after_attend_packed).
+
+    q [tokens, heads, D], k / v [keys, kv_heads, D], D = 64 or 128, heads a multiple of kv_heads; sequence b's queries are the
+    rows q_starts[b] .. q_starts[b + 1] - 1 and its keys the rows k_starts[b] ... (int32 device tensors from 0, ascending;
+    k_starts defaults to q_starts).  A sequence's queries are the newest of its keys: with more keys than queries it continues
+    what is cached, with one query it is a decoding step.
+
+    causal: a query sees the keys up to its own position; with `chunk` > 1 also the rest of its chunk, and with `window` only the
+    newest `window` keys outside its chunk: the mask of DenoiserV2's local attention (transformerv2.py:62-96).  A query that
+    sees nothing gets zeros.  Rows behind the last sequence are zeros in a new tensor and left alone in `out`, which must be
+    contiguous and must not overlap k or v (it may be q)."""
+    q = _operand(q, "q", 3)
+    k = _operand(k, "k", 3, q.device, q.dtype)
+    v = _operand(v, "v", 3, q.device, q.dtype)
+    n, heads, dim = q.shape
+    if k.shape != v.shape or k.shape[2] != dim or k.shape[1] == 0 or heads == 0 or heads % k.shape[1]:
+        raise ValueError(f"bad shapes q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)}: k and v alike, heads a multiple of kv_heads, one head_dim")
+    if dim not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, got {dim}")
+    chunk, window = int(chunk), None if window is None else int(window)
+    if chunk < 1 or (window is not None and window < 1):
+        raise ValueError(f"chunk and window must be at least 1, got {chunk} and {window}")
+    if not causal and (chunk != 1 or window is not None):
+        raise ValueError("chunk and window belong to causal attention")
+    q_starts = _starts(q_starts, "q_starts", None, q.device)
+    k_starts = q_starts if k_starts is None else _starts(k_starts, "k_starts", q_starts.numel() - 1, q.device)
+    scale = _scale(scale, dim)
+    fresh = out is None
+    if fresh:
+        out = torch.empty(n, heads, dim, device=q.device, dtype=q.dtype)
+    elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device \
+            or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f"out must be a contiguous, 16-byte aligned {q.dtype} tensor {tuple(q.shape)} on {q.device}")
+    with torch.cuda.device(q.device):
+        _lib.check(
+            _lib.lib().after_attend_packed(_lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(out), _TYPES[q.dtype], n, k.shape[0],
+                                           _lib.ptr(q_starts), _lib.ptr(k_starts), q_starts.numel() - 1, heads, k.shape[1], dim,
+                                           q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                                           out.stride(0), out.stride(1), scale, int(bool(causal)), window or 0, chunk, int(fresh),
+                                           _lib.current_stream(q.device)), "after_attend_packed")
+    return out
+
+
+class KVCache4:
+    """Keys and values of `rows` sequences, `kv_heads` heads each, in four bits: 17 bytes per 32 channels, with the attention
+    that reads them and the eviction of slots by the attention they received (include/after_hip.h: after_kv4, which states the
+    format).  `capacity` slots per row (rounded up to a multiple of 32).
+
+    The state is six tensors of the object -- `keys`, `key_scales`, `values`, `value_scales` (uint8), `weights` (fp32
+    [rows, kv_heads, capacity]: attention received, summed up by `attend(accumulate=True)`), `lengths` (int32 [rows]: slots in
+    use) -- which `buffers()` returns and `KVCache4(..., buffers=...)` takes over as they are.
+
+    Every call enqueues on the current stream, never synchronises and can be captured into a graph; the lengths live on the
+    device.  One call at a time works on a cache: order calls on different streams with events, as for any tensor."""
+
+    def __init__(self, rows, kv_heads, head_dim, capacity, device="cuda", buffers=None):
+        rows, kv_heads, head_dim, capacity = int(rows), int(kv_heads), int(head_dim), int(capacity)
+        if rows < 1 or kv_heads < 1 or rows * kv_heads > 1 << 20:
+            raise ValueError(f"rows and kv_heads must be at least 1, and rows x kv_heads at most 2^20, got {rows} and {kv_heads}")
+        if head_dim not in (64, 128):
+            raise ValueError(f"head_dim must be 64 or 128, got {head_dim}")
+        if not 1 <= capacity <= 1 << 24:
+            raise ValueError(f"capacity must be 1 .. 2^24, got {capacity}")
+        self.rows, self.kv_heads, self.head_dim = rows, kv_heads, head_dim
+        self.capacity = C = (capacity + 31) // 32 * 32
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise _lib.AFTERHipError(f"KVCache4 on {device}: after_amd runs on MI355X only (HIP kernels)")
+        self.device = torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)
+        layout = dict(keys=((rows, kv_heads, C, head_dim // 2), torch.uint8), key_scales=((rows, kv_heads, C, head_dim // 32), torch.uint8),
+                      values=((rows, kv_heads, C // 8, head_dim, 4), torch.uint8), value_scales=((rows, kv_heads, C, head_dim // 32), torch.uint8),
+                      weights=((rows, kv_heads, C), torch.float32), lengths=((rows, ), torch.int32))
+        if buffers is not None and set(buffers) != set(layout):
+            raise ValueError(f"buffers must hold {sorted(layout)}, got {sorted(buffers)}")
+        for name, (shape, dtype) in layout.items():
+            if buffers is None:
+                t = torch.zeros(shape, dtype=dtype, device=self.device)
+            else:
+                t = buffers[name]
+                if not isinstance(t, torch.Tensor) or tuple(t.shape) != shape or t.dtype != dtype or t.device != self.device \
+                        or not t.is_contiguous() or t.data_ptr() % 16:
+                    raise ValueError(f"buffers[{name!r}] must be a contiguous, 16-byte aligned {dtype} tensor {shape} on {self.device}")
+            setattr(self, name, t)
+        self._failed = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._c = _lib.KV4(*(t.data_ptr() for t in self.buffers().values()), self._failed.data_ptr(), rows, kv_heads, head_dim, C)
+        self._ref = ctypes.byref(self._c)
+
+    def buffers(self):
+        """The six tensors of the state, by name."""
+        return dict(keys=self.keys, key_scales=self.key_scales, values=self.values, value_scales=self.value_scales,
+                    weights=self.weights, lengths=self.lengths)
+
+    def _call(self, name, *args):
+        with torch.cuda.device(self.device):
+            _lib.check(getattr(_lib.lib(), name)(self._ref, *args, _lib.current_stream(self.device)), name)
+
+    def _row_values(self, t, name):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != (self.rows, ) or t.device != self.device:
+            raise ValueError(f"{name} must be an int32 tensor ({self.rows},) on {self.device}")
+        return t.contiguous()
+
+    def append(self, k, v, starts=None):
+        """Rounds new keys and values to four bits and puts them behind each row's slots: [rows, tokens, kv_heads, head_dim], or
+        [total, kv_heads, head_dim] with `starts` (int32 [rows + 1]): those of row r are starts[r] .. starts[r + 1] - 1.  Tokens
+        for which a row has no room are dropped; `check()` reports that."""
+        dims = 4 if starts is None else 3
+        k = _operand(k, "k", dims, self.device)
+        v = _operand(v, "v", dims, self.device, k.dtype)
+        if k.shape != v.shape or tuple(k.shape[-2:]) != (self.kv_heads, self.head_dim) or (starts is None and k.shape[0] != self.rows):
+            raise ValueError(f"bad shapes k{tuple(k.shape)} v{tuple(v.shape)} for {self.rows} rows of {self.kv_heads} heads of {self.head_dim}")
+        tokens = 0
+        if starts is None:
+            tokens = k.shape[1]
+            if tokens > self.capacity:
+                raise ValueError(f"{tokens} new tokens, the cache has {self.capacity} slots per row")
+            k, v = k.flatten(0, 1), v.flatten(0, 1)
+        else:
+            starts = _starts(starts, "starts", self.rows, self.device)
+        self._call("after_kv4_append", _lib.ptr(k), _lib.ptr(v), _TYPES[k.dtype], _lib.ptr(starts), tokens, k.shape[0],
+                   k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+
+    def truncate(self, lengths=None):
+        """Takes back the newest slots: row r keeps the first lengths[r] (int32 [rows] on the device); None empties the cache."""
+        self._call("after_kv4_truncate", _lib.ptr(None if lengths is None else self._row_values(lengths, "lengths")))
+
+    def read(self, start=None, count=None, dtype=torch.bfloat16):
+        """(k, v) [rows, kv_heads, count, head_dim]: the values that the slots start[r] .. start[r] + count - 1 stand for (int32
+        [rows]; default: from slot 0, the whole capacity), zeros past a row's length.  bf16 holds them exactly."""
+        count = self.capacity if count is None else int(count)
+        if not 0 <= count <= self.capacity:
+            raise ValueError(f"count must be 0 .. {self.capacity}, got {count}")
+        if dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError(f"values are read as bfloat16 or float32, got {dtype}")
+        start = None if start is None else self._row_values(start, "start")
+        k, v = (torch.empty(self.rows, self.kv_heads, count, self.head_dim, dtype=dtype, device=self.device) for _ in range(2))
+        self._call("after_kv4_read", _lib.ptr(k), _lib.ptr(v), _TYPES[dtype], _lib.ptr(start), count)
+        return k, v
+
+    def attend(self, q, scale=None, accumulate=False, decay=1.0):
+        """Attention of the newest tokens of every row, q [rows, tokens, heads, head_dim], over the cached keys and values (their
+        own have been appended): token t of T sees the slots below lengths - T + t + 1; one that sees none gets zeros.  A row
+        with fewer new tokens than T has its own at the end.  Returns [rows, tokens, heads, head_dim].
+
+        accumulate: `weights` = decay * weights + the probability that each slot received, summed over the tokens and the heads
+        of its group (decay = 0 replaces them)."""
+        q = _operand(q, "q", 4, self.device)
+        rows, tokens, heads, dim = q.shape
+        if rows != self.rows or dim != self.head_dim or heads == 0 or heads % self.kv_heads:
+            raise ValueError(f"bad shape q{tuple(q.shape)} for {self.rows} rows of {self.kv_heads} key heads of {self.head_dim}")
+        scale, decay = _scale(scale, dim), float(decay)
+        if not math.isfinite(decay):
+            raise ValueError(f"decay must be finite, got {decay}")
+        out = torch.empty(rows, tokens, heads, dim, dtype=q.dtype, device=self.device)
+        if tokens == 0:
+            if accumulate and decay != 1.0:
+                raise ValueError("accumulate with a decay needs at least one token")
+            return out
+        size = ctypes.c_longlong()
+        _lib.check(_lib.lib().after_kv4_attend_workspace(self._ref, heads, tokens, int(bool(accumulate)), ctypes.byref(size)),
+                   "after_kv4_attend_workspace")
+        # (scratch of this call: the allocator gives it to later calls of this stream only, and to a captured graph its own)
+        work = torch.empty(size.value, dtype=torch.uint8, device=self.device)
+        self._call("after_kv4_attend", _lib.ptr(q), _lib.ptr(out), _TYPES[q.dtype], heads, tokens, q.stride(0), q.stride(1), q.stride(2),
+                   scale, int(bool(accumulate)), decay, _lib.ptr(work), size.value)
+        return out
+
+    def evict(self, into, keep, recent=0):
+        """Moves min(length, keep) slots per row and head into another cache of the same rows, heads and head_dim, in their order,
+        replacing its content: the `recent` newest, and of the others those that received most attention (`weights`; ties go to
+        the lower slot, NaN counts as the least).  Heads choose for themselves.  This cache stays as it is.  Returns int32
+        [rows, kv_heads, keep]: the slot each came from, -1 past a row's new length."""
+        keep, recent = int(keep), int(recent)
+        if not isinstance(into, KVCache4) or into is self:
+            raise ValueError("evict moves into another KVCache4")
+        if (into.rows, into.kv_heads, into.head_dim, into.device) != (self.rows, self.kv_heads, self.head_dim, self.device):
+            raise ValueError("both caches need the same rows, kv_heads, head_dim and device")
+        mine = {t.data_ptr() for t in self.buffers().values()}
+        if any(t.data_ptr() in mine for t in into.buffers().values()):
+            raise ValueError("the two caches share buffers")
+        if not 1 <= keep <= into.capacity or not 0 <= recent <= keep:
+            raise ValueError(f"1 <= keep <= {into.capacity} and 0 <= recent <= keep, got {keep} and {recent}")
+        slots = torch.empty(self.rows, self.kv_heads, keep, dtype=torch.int32, device=self.device)
+        self._call("after_kv4_evict", into._ref, keep, recent, _lib.ptr(slots))
+        return slots
+
+    def check(self):
+        """Waits for the work on this cache and raises AFTERHipError if an append has dropped tokens since the last look."""
+        if int(self._failed.item()):
+            self._failed.zero_()
+            raise _lib.AFTERHipError(f"KVCache4.append: a row had no room for all of its new tokens ({self.capacity} slots)")

@@ -1,0 +1,385 @@
+// Attention of packed sequences (include/after_hip.h: after_attend_packed; Python: after_amd.attend_packed).
+//
+// Mathematics.  One pass over the keys with the running maximum m and sum l of the softmax: a tile's scores s raise m to m',
+// what is summed so far shrinks by 2^(m - m'), p = 2^(s - m') (scores carry log2 e).  Scores and output are formed transposed,
+// S^T = K Q^T and O^T = V^T P^T, so that a query is a lane: its maximum and sum are a chain over the lane's registers and one
+// exchange with the other half of the wave, and a rescale is one factor per lane.  Row i of a 32 x 32 result stands at
+// 8 (i / 4) + 4 (lane / 32) + i % 4; with the contraction of the second product taken in that same order, the probabilities
+// are its operand as they lie, and only V is read accordingly (two transposing LDS reads per 16 tokens).
+//
+// Rows.  The `group` heads that share a key head are rows of one tile, row = token * group + head: short sequences fill tiles,
+// and a key tile is read once for all of them.  A workgroup holds 128 rows, 32 to a wave; its tile number alone says which
+// sequence it serves (sequence b owns the numbers from floor(start_b * group / 128) + b on), so the grid needs no lengths.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+
+#include "common.h"
+
+namespace after {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int BM = 128, BN = 64;
+
+template <int TYPE>
+struct Elem;
+template <>
+struct Elem<AFTER_T_F32> {
+    using T = float;
+};
+template <>
+struct Elem<AFTER_T_BF16> {
+    using T = __bf16;
+    using V8 = bf16x8;
+    static __device__ __forceinline__ f32x16 mfma(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Elem<AFTER_T_F16> {
+    using T = _Float16;
+    using V8 = f16x8;
+    static __device__ __forceinline__ f32x16 mfma(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+
+struct PackedArgs {
+    const void *q, *k, *v;
+    void* out;
+    const int *qs, *ks;
+    long long qts, qhs, kts, khs, vts, vhs, ots, ohs;
+    int q_rows, k_rows, n_seqs, heads, kv_heads, group, tiles;
+    float scale2;
+    int causal, window, chunk, zero_rest;
+};
+
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
+
+// Sequence b of the queries begins at row ...; one more "sequence" without keys stands for the rows behind the last
+__device__ __forceinline__ int q_start(const PackedArgs& a, int b) {
+    return b <= 0 ? 0 : b > a.n_seqs ? a.q_rows : clampi(a.qs[b], 0, a.q_rows);
+}
+
+// [first, last) of the keys that the query at position p of its sequence sees
+__device__ __forceinline__ void seen(const PackedArgs& a, int p, int keys, int& first, int& last) {
+    first = 0;
+    last = keys;
+    if (a.causal) {
+        // (floor: a query older than the keys has a negative position)
+        const int q = p >= 0 ? p / a.chunk : -((a.chunk - 1 - p) / a.chunk);
+        const int begin = q * a.chunk;
+        last = clampi(begin + a.chunk, 0, keys);
+        if (a.window > 0) first = max(0, min(begin, p - a.window + 1));
+    }
+}
+
+// 16-byte pieces of a 64-row tile in LDS.  Keys: a wave reads the same piece of 32 rows, so a row's pieces are permuted by its
+// number; values (16-bit types): a transposing read takes 32 bytes each of four neighbouring rows, so pairs of pieces are.
+template <int PIECES>
+__device__ __forceinline__ int k_piece(int row, int c) {
+    return row * PIECES + (c ^ (row & (PIECES < 16 ? PIECES - 1 : 15)));
+}
+template <int PIECES>
+__device__ __forceinline__ int v_piece(int row, int c) {
+    return row * PIECES + (c ^ ((row & (PIECES < 16 ? 3 : 7)) << 1));
+}
+
+// whether one of the words' elements is an infinity or NaN
+template <int TYPE>
+__device__ __forceinline__ bool odd_value(u32x4 w) {
+    constexpr unsigned e = TYPE == AFTER_T_F16 ? 0x7C00u : 0x7F80u;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (TYPE == AFTER_T_F32)
+            bad |= (w[i] & 0x7F800000u) == 0x7F800000u;
+        else
+            bad |= (w[i] & e) == e || (w[i] >> 16 & e) == e;
+    }
+    return bad;
+}
+
+template <int TYPE, int D>
+__global__ __launch_bounds__(256) void attend_packed_kernel(PackedArgs a) {
+    using E = Elem<TYPE>;
+    using T = typename E::T;
+    constexpr int PIECES = D * (int)sizeof(T) / 16;  // 16-byte pieces of a row
+    constexpr int LOADS = BN * PIECES / 256;         // pieces per thread of a tile
+    constexpr int DT = D / 32;
+    extern __shared__ __align__(16) char lds[];
+    u32x4* lk = reinterpret_cast<u32x4*>(lds);
+    u32x4* lv = lk + BN * PIECES;
+    __shared__ unsigned long long odd_rows;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, half = lane >> 5;
+    // neighbouring workgroups are dispatched to different XCDs: a key head's workgroups stay on one L2 where there are eight.
+    // Tiles from the last to the first: with a causal mask the longest first.
+    const int h = blockIdx.x % a.kv_heads, tile = a.tiles - 1 - blockIdx.x / a.kv_heads;
+    int lo = 0, hi = a.n_seqs;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if ((int)((long long)q_start(a, mid) * a.group / BM) + mid <= tile)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    const int b = lo, q0 = q_start(a, b), nq = q_start(a, b + 1) - q0;
+    const int row0 = (tile - ((int)((long long)q0 * a.group / BM) + b)) * BM;
+    const int rows = nq * a.group;  // (< 2^31: checked on the host)
+    if (row0 < 0 || row0 >= rows) return;
+    int k0 = 0, nk = 0;
+    if (b < a.n_seqs) {
+        k0 = b == 0 ? 0 : clampi(a.ks[b], 0, a.k_rows);
+        nk = max(clampi(a.ks[b + 1], 0, a.k_rows) - k0, 0);
+    } else if (!a.zero_rest)
+        return;
+
+    // this lane's query, and the keys that it and its workgroup see
+    const int row = row0 + wave * 32 + l31, t = min(row, rows - 1) / a.group, g = min(row, rows - 1) - t * a.group;
+    int first, last, t_first, t_last, dummy;
+    seen(a, t + nk - nq, nk, first, last);
+    seen(a, row0 / a.group + nk - nq, nk, t_first, dummy);
+    seen(a, (min(row0 + BM, rows) - 1) / a.group + nk - nq, nk, dummy, t_last);
+    // every query of the workgroup sees [all_first, all_last)
+    int all_first, all_last;
+    seen(a, row0 / a.group + nk - nq, nk, dummy, all_last);
+    seen(a, (min(row0 + BM, rows) - 1) / a.group + nk - nq, nk, all_first, dummy);
+
+    const T* qp = (const T*)a.q + (long long)(q0 + t) * a.qts + (long long)(h * a.group + g) * a.qhs;
+    const T* kp = (const T*)a.k + (long long)k0 * a.kts + (long long)h * a.khs;
+    const T* vp = (const T*)a.v + (long long)k0 * a.vts + (long long)h * a.vhs;
+
+    // Q: 16-bit types: step s contracts channels 16 s + 8 half + 0 .. 7; fp32: step s, e channels 8 s + 4 half + e
+    constexpr int QN = sizeof(T) == 4 ? D / 8 : D / 16;
+    u32x4 qf[QN];
+#pragma unroll
+    for (int s = 0; s < QN; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qp + (2 * s + half) * (16 / (int)sizeof(T)));
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+    float mx = -INFINITY, l = 0.f;
+
+    const int n_first = t_first / BN, n_last = (t_last + BN - 1) / BN;  // key tiles
+    u32x4 rk[LOADS], rv[LOADS];
+    auto fetch = [&](int n) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int id = i * 256 + tid, r = id / PIECES, c = id % PIECES, j = n * BN + r;
+            rk[i] = rv[i] = u32x4{0, 0, 0, 0};  // (rows behind the sequence are zeros, whatever stands there)
+            if (j < nk) {
+                rk[i] = *reinterpret_cast<const u32x4*>(kp + (long long)j * a.kts + c * (16 / (int)sizeof(T)));
+                rv[i] = *reinterpret_cast<const u32x4*>(vp + (long long)j * a.vts + c * (16 / (int)sizeof(T)));
+            }
+        }
+    };
+    if (n_first < n_last) fetch(n_first);
+    for (int n = n_first; n < n_last; ++n) {
+        const bool masked = n * BN < all_first || (n + 1) * BN > all_last;
+        __syncthreads();
+        if (masked && tid == 0) odd_rows = 0;
+        if (masked) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int id = i * 256 + tid, r = id / PIECES, c = id % PIECES;
+            lk[k_piece<PIECES>(r, c)] = rk[i];
+            lv[sizeof(T) == 4 ? id : v_piece<PIECES>(r, c)] = rv[i];
+            // what a query does not see must not reach it: 0 x NaN would
+            if (masked && odd_value<TYPE>(rv[i])) atomicOr(&odd_rows, 1ull << r);
+        }
+        __syncthreads();
+        unsigned long long odd = 0;
+        if (masked) {
+            odd = odd_rows;
+            if (odd) {  // (rare) such rows are taken out of the product and added one by one below
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) {
+                    const int id = i * 256 + tid, r = id / PIECES, c = id % PIECES;
+                    if (odd >> r & 1) lv[sizeof(T) == 4 ? id : v_piece<PIECES>(r, c)] = u32x4{0, 0, 0, 0};
+                }
+                __syncthreads();
+            }
+        }
+        if (n + 1 < n_last) fetch(n + 1);
+
+        f32x16 sc[2];
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[f][e] = 0.f;
+#pragma unroll
+            for (int s = 0; s < QN; ++s) {
+                const u32x4 kf = lk[k_piece<PIECES>(32 * f + l31, 2 * s + half)];
+                if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        sc[f] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]), __uint_as_float(qf[s][e]), sc[f], 0, 0, 0);
+                } else
+                    sc[f] = E::mfma(__builtin_bit_cast(typename E::V8, kf), __builtin_bit_cast(typename E::V8, qf[s]), sc[f]);
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                float x = sc[f][e] * a.scale2;
+                if (masked) {
+                    const int j = n * BN + 32 * f + 8 * (e >> 2) + 4 * half + (e & 3);
+                    x = j >= first && j < last ? x : -INFINITY;
+                }
+                sc[f][e] = x;
+                top = fmaxf(top, x);
+            }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        if (__any(top > mx)) {
+            const float now = fmaxf(mx, top), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - now);
+            mx = now;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < DT; ++i) o[i] = o[i] * f;
+        }
+        const float off = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                sc[f][e] = __builtin_amdgcn_exp2f(sc[f][e] - off);
+                l += sc[f][e];
+            }
+        // O^T += V^T P^T
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+            if constexpr (sizeof(T) == 4) {
+                const float* vv = reinterpret_cast<const float*>(lv);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int j = 32 * f + 8 * (e >> 2) + 4 * half + (e & 3);
+#pragma unroll
+                    for (int i = 0; i < DT; ++i) o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(vv[j * D + 32 * i + l31], sc[f][e], o[i], 0, 0, 0);
+                }
+            } else {
+                const char* vv = reinterpret_cast<const char*>(lv);
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    typename E::V8 pf;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) pf[e] = (T)sc[f][8 * s + e];  // (the products' own type: half a step of 2^-9 / 2^-12 each)
+#pragma unroll
+                    for (int i = 0; i < DT; ++i) {
+                        // lane l of 16 reads 8 bytes of row l / 4: it gets column l of the four rows
+                        union {
+                            typename E::V8 v;
+                            s16x4 p[2];
+                        } vf;
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) {
+                            const int r = 32 * f + 16 * s + 8 * w + 4 * half + ((lane & 15) >> 2);
+                            const int byte = 64 * i + (lane & 16) * 2 + (lane & 3) * 8;
+                            vf.p[w] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (__attribute__((address_space(3))) s16x4*)(vv + 16 * v_piece<PIECES>(r, byte >> 4) + (byte & 15)));
+                        }
+                        o[i] = E::mfma(vf.v, pf, o[i]);
+                    }
+                }
+            }
+        }
+        while (odd) {  // (uniform) rows of V with infinities or NaN in a masked tile: only for the queries that see them
+            const int j = __ffsll((unsigned long long)odd) - 1, at = n * BN + j;
+            odd &= odd - 1;
+            const int e_at = (j >> 3 & 3) * 4 + (j & 3), holder = (j >> 2 & 1) * 32 + l31;
+            float p = 0.f;
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if ((j >> 5) == f && e == e_at) p = sc[f][e];
+            p = __shfl(p, holder);
+            if (at >= first && at < last) {
+#pragma unroll
+                for (int i = 0; i < DT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        o[i][e] = fmaf(p, (float)vp[(long long)at * a.vts + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3)], o[i][e]);
+            }
+        }
+    }
+
+    l += __shfl_xor(l, 32);
+    if (row >= rows) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* op = (T*)a.out + (long long)(q0 + t) * a.ots + (long long)(h * a.group + g) * a.ohs;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            typedef T T4 __attribute__((ext_vector_type(4)));
+            T4 y;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) y[w] = (T)(o[i][e + w] * inv);
+            *reinterpret_cast<T4*>(op + 32 * i + 2 * e + 4 * half) = y;
+        }
+}
+
+template <int TYPE, int D>
+int run_packed(const PackedArgs& a, hipStream_t s) {
+    constexpr size_t lds = 2 * BN * D * sizeof(typename Elem<TYPE>::T);
+    static LdsAttr attr;
+    AFTER_TRY(ensure_lds_attr(attr, (const void*)attend_packed_kernel<TYPE, D>, lds));
+    hipLaunchKernelGGL((attend_packed_kernel<TYPE, D>), dim3((unsigned)a.tiles * a.kv_heads), dim3(256), lds, s, a);
+    AFTER_HIP_CHECK(hipGetLastError());
+    return AFTER_OK;
+}
+
+}  // namespace
+}  // namespace after
+
+using namespace after;
+
+extern "C" int after_attend_packed(const void* q, const void* k, const void* v, void* out, int type, long long q_rows, long long k_rows,
+                                   const int* q_starts, const int* k_starts, int n_seqs, int heads, int kv_heads, int head_dim,
+                                   long long q_token_stride, long long q_head_stride, long long k_token_stride, long long k_head_stride,
+                                   long long v_token_stride, long long v_head_stride, long long out_token_stride, long long out_head_stride,
+                                   float scale, int causal, int window, int chunk, int zero_rest, void* stream) {
+    AFTER_REQUIRE(type == AFTER_T_F32 || type == AFTER_T_BF16 || type == AFTER_T_F16, AFTER_E_INVALID, "attend_packed: unknown element type %d", type);
+    AFTER_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, AFTER_E_INVALID, "attend_packed: heads must be a multiple of kv_heads (got %d, %d)", heads,
+                  kv_heads);
+    AFTER_REQUIRE(head_dim == 64 || head_dim == 128, AFTER_E_INVALID, "attend_packed: head_dim 64 or 128 (got %d)", head_dim);
+    AFTER_REQUIRE(n_seqs >= 0 && n_seqs <= (1 << 24) && q_rows >= 0 && k_rows >= 0 && k_rows < (1ll << 30), AFTER_E_INVALID,
+                  "attend_packed: 0 <= n_seqs <= 2^24, 0 <= rows < 2^30");
+    const int group = heads / kv_heads;
+    AFTER_REQUIRE(q_rows * group < (1ll << 30), AFTER_E_INVALID, "attend_packed: q_rows x heads / kv_heads must stay below 2^30");
+    AFTER_REQUIRE(std::isfinite(scale), AFTER_E_INVALID, "attend_packed: scale must be finite");
+    AFTER_REQUIRE(window >= 0 && chunk >= 1 && chunk <= (1 << 24) && (causal || (window == 0 && chunk == 1)), AFTER_E_INVALID,
+                  "attend_packed: window >= 0 (0: none) and chunk >= 1, both for causal attention only");
+    if (q_rows == 0) return AFTER_OK;
+    const int per16 = 16 / (type == AFTER_T_F32 ? 4 : 2);
+    const long long strides = q_token_stride | q_head_stride | k_token_stride | k_head_stride | v_token_stride | v_head_stride | out_token_stride | out_head_stride;
+    AFTER_REQUIRE(q && out && q_starts && k_starts && (k_rows == 0 || (k && v)), AFTER_E_INVALID, "attend_packed: a pointer is NULL");
+    AFTER_REQUIRE((((size_t)q | (size_t)k | (size_t)v | (size_t)out) & 15) == 0 && (strides & (per16 - 1)) == 0, AFTER_E_INVALID,
+                  "attend_packed: q, k, v, out and their token and head strides must be multiples of 16 bytes");
+    PackedArgs a;
+    a.q = q, a.k = k, a.v = v, a.out = out, a.qs = q_starts, a.ks = k_starts;
+    a.qts = q_token_stride, a.qhs = q_head_stride, a.kts = k_token_stride, a.khs = k_head_stride;
+    a.vts = v_token_stride, a.vhs = v_head_stride, a.ots = out_token_stride, a.ohs = out_head_stride;
+    a.q_rows = (int)q_rows, a.k_rows = (int)k_rows, a.n_seqs = n_seqs, a.heads = heads, a.kv_heads = kv_heads, a.group = group;
+    a.tiles = (int)(q_rows * group / BM) + n_seqs + 1;
+    a.scale2 = scale * 1.44269504088896340736f;
+    a.causal = causal != 0, a.window = window < (1 << 30) ? window : 1 << 30, a.chunk = chunk, a.zero_rest = zero_rest;
+    AFTER_REQUIRE((long long)a.tiles * kv_heads < (1ll << 31), AFTER_E_INVALID, "attend_packed: too many tokens x heads for one call");
+    hipStream_t s = (hipStream_t)stream;
+    if (head_dim == 64) {
+        if (type == AFTER_T_F32) return run_packed<AFTER_T_F32, 64>(a, s);
+        if (type == AFTER_T_BF16) return run_packed<AFTER_T_BF16, 64>(a, s);
+        return run_packed<AFTER_T_F16, 64>(a, s);
+    }
+    if (type == AFTER_T_F32) return run_packed<AFTER_T_F32, 128>(a, s);
+    if (type == AFTER_T_BF16) return run_packed<AFTER_T_BF16, 128>(a, s);
+    return run_packed<AFTER_T_F16, 128>(a, s);
+}

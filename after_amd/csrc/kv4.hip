@@ -1,0 +1,910 @@
+// A key / value cache held in four bits, the attention that reads it, and the eviction of slots by the attention they received
+// (include/after_hip.h: after_kv4_*; Python: after_amd.KVCache4).
+//
+// Format.  32 neighbouring channels of one token form a group: one byte b, the power of two 2^(b - 127), and 32 four-bit floats
+// (sign, two bits of exponent, one of fraction: 0, .5, 1, 1.5, 2, 3, 4, 6).  17 bytes per 32 channels, against 64 of a 16-bit
+// cache.  The power is the smallest with which the group's largest magnitude is <= 6, so nothing saturates (but beyond
+// 6 * 2^125); gfx950 converts both ways in hardware (v_cvt_scalef32_pk_*_fp4, to nearest even).  Bytes run from 16 to 252:
+// every value but 0 is a normal bf16 number, so that bf16 carries all of them exactly.  Byte 255 marks a group that held an
+// infinity or NaN: it reads as NaN.
+//
+// Layout.  keys [rows][H][C][D / 2]: a token's channels side by side, two to a byte.  values [rows][H][C / 8][D][4]: eight
+// tokens of a channel in a dword, since the product P V contracts over tokens: a lane's eight tokens of one channel are then one
+// load and four conversions, and nothing is transposed on the way to the matrix pipe.  The channels of such a block stand in the
+// order [d / 2 % 16][d / 32][d % 2]: what lane d / 2 % 16 of the product needs is one piece of D / 4 bytes.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+
+#include "common.h"
+
+namespace after {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kMinByte = 16, kMaxByte = 252, kBadByte = 255;
+
+template <int TYPE>
+struct Elem;
+template <>
+struct Elem<AFTER_T_F32> {
+    using T = float;
+};
+template <>
+struct Elem<AFTER_T_BF16> {
+    using T = __bf16;
+};
+template <>
+struct Elem<AFTER_T_F16> {
+    using T = _Float16;
+};
+
+// N consecutive elements (N * sizeof(T) aligned) as floats
+template <int N, typename T>
+__device__ __forceinline__ void load_n(const T* p, float (&x)[N]) {
+    typedef T vec __attribute__((ext_vector_type(N)));
+    const vec v = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = (float)v[i];
+}
+template <int N, typename T>
+__device__ __forceinline__ void store_n(T* p, const float (&x)[N]) {
+    typedef T vec __attribute__((ext_vector_type(N)));
+    vec v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (T)x[i];
+    *reinterpret_cast<vec*>(p) = v;
+}
+
+__device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+// the scale byte of a group whose largest magnitude has these bits: the smallest e with top <= 1.5 * 2^(e + 2)
+__device__ __forceinline__ int scale_byte(unsigned top) {
+    if (top >= 0x7F800000u) return kBadByte;
+    const int b = (int)(top >> 23) - 2 + ((top & 0x7FFFFFu) > 0x400000u ? 1 : 0);
+    return min(max(b, kMinByte), kMaxByte);
+}
+__device__ __forceinline__ float byte_scale(int b) { return __uint_as_float((unsigned)b << 23); }
+
+// two floats -> the low byte: two codes
+__device__ __forceinline__ unsigned round4(float a, float b, float scale) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, a, b, scale, 0) & 255u;
+}
+// the four bytes of a dword -> eight bf16 values (code * scale)
+__device__ __forceinline__ bf16x8 widen8(unsigned w, float scale) {
+    union {
+        bf16x8 v;
+        bf16x2 p[4];
+    } u;
+    u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0);
+    u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1);
+    u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2);
+    u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
+    return u.v;
+}
+
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
+__device__ __forceinline__ int row_length(const after_kv4& c, int r) { return clampi(c.lengths[r], 0, c.capacity); }
+
+// ---------------------------------------------------------------------------------------------------------------- append
+struct NewTokens {
+    const int* starts;  // [rows + 1], or nullptr: `each` tokens of every row
+    int each;
+    int total;
+    __device__ __forceinline__ int start(int r) const { return starts ? clampi(starts[r], 0, total) : r * each; }
+};
+
+// One wave rounds the new tokens of one (row, head) that fall into one block of eight slots.  Row r owns the block numbers from
+// start(r) / 8 + 2 r on: at least as many as its tokens touch, wherever in a block they begin, so the grid needs no lengths.
+template <int TYPE, int D>
+__global__ __launch_bounds__(256) void kv4_append_kernel(after_kv4 c, NewTokens nt, const void* kp, const void* vp, long long kts, long long khs,
+                                                         long long vts, long long vhs, int items) {
+    using T = typename Elem<TYPE>::T;
+    constexpr int G = D / 32;
+    const int lane = threadIdx.x & 63;
+    const int item = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item >= items) return;
+    const int h = item % c.kv_heads, fb = item / c.kv_heads;
+    int lo = 0, hi = c.rows - 1;  // the last row that begins at or before fb
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (nt.start(mid) / 8 + 2 * mid <= fb)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    const int r = lo, t0 = nt.start(r), n = nt.start(r + 1) - t0;
+    const int len = row_length(c, r);
+    const int sb = len / 8 + fb - (t0 / 8 + 2 * r);
+    const int end = min(len + max(n, 0), c.capacity);  // tokens that do not fit are dropped (kv4_advance_kernel reports them)
+    if (sb < 0 || 8 * sb >= end) return;
+    const size_t rh = (size_t)r * c.kv_heads + h;
+    const T* k = (const T*)kp + (size_t)h * khs;
+    const T* v = (const T*)vp + (size_t)h * vhs;
+
+    if (lane < 8) {
+        const int s = 8 * sb + lane;
+        if (s >= len && s < end) c.weights[rh * c.capacity + s] = 0.f;
+    }
+    // keys: eight channels per lane
+#pragma unroll
+    for (int it = 0; it < D / 64; ++it) {
+        const int id = it * 64 + lane, tt = id / (D / 8), ch = id % (D / 8), s = 8 * sb + tt;
+        const bool in = s >= len && s < end;
+        float x[8] = {};
+        if (in) load_n<8, T>(k + (long long)(t0 + s - len) * kts + 8 * ch, x);
+        unsigned top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, abs_bits(x[i]));
+        top = max(top, (unsigned)__shfl_xor((int)top, 1));
+        top = max(top, (unsigned)__shfl_xor((int)top, 2));
+        const int b = scale_byte(top);
+        const float sc = byte_scale(b);
+        unsigned w = round4(x[0], x[1], sc) | round4(x[2], x[3], sc) << 8 | round4(x[4], x[5], sc) << 16 | round4(x[6], x[7], sc) << 24;
+        if (b == kBadByte) w = 0;
+        if (in) {
+            *reinterpret_cast<unsigned*>(c.keys + (rh * c.capacity + s) * (D / 2) + 4 * ch) = w;
+            if ((ch & 3) == 0) c.key_scales[(rh * c.capacity + s) * G + ch / 4] = (unsigned char)b;
+        }
+    }
+    // values: two channels of the eight tokens per lane
+    if (2 * lane < D) {
+        unsigned w0 = 0, w1 = 0, mask = 0;
+#pragma unroll
+        for (int tt = 0; tt < 8; ++tt) {
+            const int s = 8 * sb + tt;
+            const bool in = s >= len && s < end;
+            if (!in) continue;  // (uniform)
+            float x[2];
+            load_n<2, T>(v + (long long)(t0 + s - len) * vts + 2 * lane, x);
+            unsigned top = max(abs_bits(x[0]), abs_bits(x[1]));
+#pragma unroll
+            for (int o = 1; o < 16; o *= 2) top = max(top, (unsigned)__shfl_xor((int)top, o));
+            const int b = scale_byte(top);
+            const unsigned u = b == kBadByte ? 0u : round4(x[0], x[1], byte_scale(b));
+            w0 |= (u & 15u) << 4 * tt;
+            w1 |= (u >> 4) << 4 * tt;
+            mask |= 15u << 4 * tt;
+            if ((lane & 15) == 0) c.value_scales[(rh * c.capacity + s) * G + lane / 16] = (unsigned char)b;
+        }
+        u32x2* at = reinterpret_cast<u32x2*>(c.values + ((rh * (c.capacity / 8) + sb) * D + (lane & 15) * (D / 16) + (lane >> 4) * 2) * 4);
+        u32x2 w = {w0, w1};
+        if (mask != 0xFFFFFFFFu) {  // the other slots of the block keep what they hold
+            const u32x2 old = *at;
+            w = w | (old & ~mask);
+        }
+        *at = w;
+    }
+}
+
+__global__ void kv4_advance_kernel(after_kv4 c, NewTokens nt) {
+    const int r = blockIdx.x * blockDim.x + threadIdx.x;
+    if (r >= c.rows) return;
+    const int len = row_length(c, r), n = max(nt.start(r + 1) - nt.start(r), 0);
+    if (n > c.capacity - len) *c.failed = 1;
+    c.lengths[r] = min(n, c.capacity - len) + len;
+}
+
+__global__ void kv4_truncate_kernel(after_kv4 c, const int* lengths) {
+    const int r = blockIdx.x * blockDim.x + threadIdx.x;
+    if (r < c.rows) c.lengths[r] = lengths ? clampi(lengths[r], 0, row_length(c, r)) : 0;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- read
+// One wave per (row, head, block of eight slots): the slots [start, start + count) as values; past the row's length zeros.
+template <int TYPE, int D>
+__global__ __launch_bounds__(256) void kv4_read_kernel(after_kv4 c, void* ko, void* vo, const int* start, int count, int nb, long long items) {
+    using T = typename Elem<TYPE>::T;
+    constexpr int G = D / 32;
+    const int lane = threadIdx.x & 63;
+    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item >= items) return;
+    const size_t rh = item / nb;
+    const int r = (int)(rh / c.kv_heads);
+    const int st = start ? clampi(start[r], 0, c.capacity) : 0;
+    const int sb = st / 8 + (int)(item % nb);
+    if (8 * sb >= st + count) return;
+    const int len = row_length(c, r);
+    T* k = (T*)ko + rh * count * D;
+    T* v = (T*)vo + rh * count * D;
+#pragma unroll
+    for (int it = 0; it < D / 64; ++it) {
+        const int id = it * 64 + lane, tt = id / (D / 8), ch = id % (D / 8), s = 8 * sb + tt, o = s - st;
+        if (o < 0 || o >= count) continue;
+        float x[8] = {};
+        if (s < len) {
+            const unsigned w = *reinterpret_cast<const unsigned*>(c.keys + (rh * c.capacity + s) * (D / 2) + 4 * ch);
+            const bf16x8 y = widen8(w, byte_scale(c.key_scales[(rh * c.capacity + s) * G + ch / 4]));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = (float)y[i];
+        }
+        store_n<8, T>(k + (size_t)o * D + 8 * ch, x);
+    }
+    if (2 * lane < D) {
+        u32x2 w = {0, 0};
+        if (8 * sb < len) w = *reinterpret_cast<const u32x2*>(c.values + ((rh * (c.capacity / 8) + sb) * D + (lane & 15) * (D / 16) + (lane >> 4) * 2) * 4);
+#pragma unroll
+        for (int tt = 0; tt < 8; ++tt) {
+            const int s = 8 * sb + tt, o = s - st;
+            if (o < 0 || o >= count) continue;
+            float x[2] = {};
+            if (s < len) {
+                const bf16x2 y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((w[0] >> 4 * tt & 15u) | (w[1] >> 4 * tt & 15u) << 4,
+                                                                           byte_scale(c.value_scales[(rh * c.capacity + s) * G + lane / 16]), 0);
+                x[0] = (float)y[0];
+                x[1] = (float)y[1];
+            }
+            store_n<2, T>(v + (size_t)o * D + 2 * lane, x);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- attend
+// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16: the 16 columns are (token, head of the group) pairs that share
+// the cached head, the rows cached tokens / channels.  Everything stays in registers: which token a row of S^T stands for and
+// which channel a step of its product contracts are chosen so that a lane's S values are the P operand that it needs next.
+// A cached value is exact in bf16; queries and probabilities travel as NP bf16 pieces (1 for bf16 queries, 2 for fp16: exact,
+// 3 for fp32: exact), so that what is rounded is never coarser than the output's own type.
+struct AttendArgs {
+    after_kv4 c;
+    const void* q;
+    void* out;  // [rows][tokens][heads][D]
+    long long qrs, qts, qhs;
+    int heads, tokens, group, m_rows;  // m_rows = tokens * group
+    int splits, mgroups;
+    float scale2;  // scale * log2(e)
+    float* part_o;  // [rows * H][splits][m_rows][D]
+    f32x2* part_ml; // [rows * H][splits][m_rows]
+    float* scores;  // [rows * H][m_rows][C] or nullptr
+};
+
+// tokens per split of a row: whole tiles of 32
+__device__ __forceinline__ int split_chunk(int len, int splits) { return ((len + splits - 1) / splits + 31) & ~31; }
+
+template <int N>
+__device__ __forceinline__ void pieces8(const float (&x)[8], bf16x8 (&p)[N]) {
+    float rest[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rest[i] = x[i];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[n][i] = (__bf16)rest[i];
+        if (n + 1 < N) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) rest[i] -= (float)p[n][i];
+        }
+    }
+}
+
+template <int TYPE, int D, int NM, bool COUNT>
+__global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
+    using T = typename Elem<TYPE>::T;
+    constexpr int NP = TYPE == AFTER_T_BF16 ? 1 : TYPE == AFTER_T_F16 ? 2 : 3;
+    constexpr int G = D / 32, S = D / 32, KW = D / 32, VW = D / 16;  // groups, steps of a score, dwords of keys / values per lane
+    __shared__ float so[4][16][D + 4];
+    __shared__ float sm[4][NM * 16], sl[4][NM * 16];
+    const after_kv4& c = a.c;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, kq = lane >> 4;
+    // neighbours in x are dispatched to different XCDs: the query groups of one piece of the cache stand 8 apart, on one L2
+    const int x = blockIdx.x, mg = (x >> 3) % a.mgroups, unit = (x >> 3) / a.mgroups * 8 + (x & 7);
+    const int n_rh = c.rows * c.kv_heads;
+    if (unit >= n_rh * a.splits) return;
+    const int rh = unit % n_rh, split = unit / n_rh, r = rh / c.kv_heads, h = rh % c.kv_heads;
+    const int len = row_length(c, r);
+    const int chunk = split_chunk(len, a.splits);
+    const int begin = split * chunk, end = min(begin + chunk, len);
+    if (begin >= end && (split > 0 || a.splits > 1)) return;  // (an empty row of an unsplit call still writes its zeros)
+
+    bf16x8 qf[NM][S][NP];
+    int vis[NM];
+#pragma unroll
+    for (int nm = 0; nm < NM; ++nm) {
+        const int m = (mg * NM + nm) * 16 + l15, t = m / a.group, g = m - t * a.group;
+        const bool in = m < a.m_rows;
+        vis[nm] = in ? max(len - a.tokens + t + 1, 0) : 0;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            float y[8] = {};
+            if (in) load_n<8, T>((const T*)a.q + r * a.qrs + t * a.qts + (long long)(h * a.group + g) * a.qhs + D / 4 * kq + 8 * s, y);
+            pieces8<NP>(y, qf[nm][s]);
+        }
+    }
+    const int all_see = len - a.tokens + mg * NM * 16 / a.group + 1;  // slots below this are seen by every query here
+
+    f32x4 o[NM][2 * G];
+    float mx[NM], l[NM];
+#pragma unroll
+    for (int nm = 0; nm < NM; ++nm) {
+        mx[nm] = -INFINITY;
+        l[nm] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2 * G; ++i) o[nm][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const size_t base = (size_t)rh * c.capacity;
+    for (int t0 = begin + 32 * wave; t0 < end; t0 += 128) {
+        // tile rows (2 x 16): row m of half f is token t0 + 8 (m / 4) + 4 f + m % 4
+        unsigned kw[2][KW], vw[VW];
+        float ks[2];
+        unsigned vs[2 * G];  // the scale bytes of the lane's eight tokens: [token][group]
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+            const size_t tok = base + t0 + 8 * (l15 >> 2) + (l15 & 3) + 4 * f;
+            const unsigned* p = reinterpret_cast<const unsigned*>(c.keys + tok * (D / 2) + kq * (D / 8));
+#pragma unroll
+            for (int i = 0; i < KW; ++i) kw[f][i] = p[i];
+            ks[f] = byte_scale(c.key_scales[tok * G + kq * G / 4]);
+        }
+        {
+            const unsigned* p = reinterpret_cast<const unsigned*>(c.values + ((base + t0) / 8 + kq) * (size_t)(4 * D)) + l15 * VW;
+#pragma unroll
+            for (int i = 0; i < VW; ++i) vw[i] = p[i];
+            const unsigned* ps = reinterpret_cast<const unsigned*>(c.value_scales + (base + t0 + 8 * kq) * G);
+#pragma unroll
+            for (int i = 0; i < 2 * G; ++i) vs[i] = ps[i];
+        }
+        f32x4 sc[NM][2];
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+#pragma unroll
+            for (int nm = 0; nm < NM; ++nm) sc[nm][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                const bf16x8 kf = widen8(kw[f][s], ks[f]);
+#pragma unroll
+                for (int nm = 0; nm < NM; ++nm)
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; --p) sc[nm][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[nm][s][p], sc[nm][f], 0, 0, 0);
+            }
+        }
+        const bool masked = t0 + 32 > all_see;
+        float p[NM][8];
+#pragma unroll
+        for (int nm = 0; nm < NM; ++nm) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                p[nm][j] = sc[nm][j >> 2][j & 3] * a.scale2;
+                if (masked && t0 + 8 * kq + j >= vis[nm]) p[nm][j] = -INFINITY;
+                top = fmaxf(top, p[nm][j]);
+            }
+            if constexpr (COUNT) {
+                const int m = (mg * NM + nm) * 16 + l15;
+                if (m < a.m_rows) {
+                    float* w = a.scores + ((size_t)rh * a.m_rows + m) * c.capacity + t0 + 8 * kq;
+                    *reinterpret_cast<f32x4*>(w) = f32x4{p[nm][0], p[nm][1], p[nm][2], p[nm][3]};
+                    *reinterpret_cast<f32x4*>(w + 4) = f32x4{p[nm][4], p[nm][5], p[nm][6], p[nm][7]};
+                }
+            }
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            if (__any(top > mx[nm])) {
+                const float now = fmaxf(mx[nm], top), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[nm] - now);
+                mx[nm] = now;
+                l[nm] *= f;
+#pragma unroll
+                for (int i = 0; i < 2 * G; ++i) o[nm][i] = o[nm][i] * f;
+            }
+            const float off = mx[nm] == -INFINITY ? 0.f : mx[nm];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                p[nm][j] = __builtin_amdgcn_exp2f(p[nm][j] - off);
+                l[nm] += p[nm][j];
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            bf16x8 pf[NM][NP];
+#pragma unroll
+            for (int nm = 0; nm < NM; ++nm) {
+                float y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int byte = j * G + g;
+                    y[j] = p[nm][j] * byte_scale(vs[byte >> 2] >> 8 * (byte & 3) & 255u);
+                    // (a masked slot may hold anything, a NaN group included: 0 x NaN must not reach the sum)
+                    if (masked && t0 + 8 * kq + j >= vis[nm]) y[j] = 0.f;
+                }
+                pieces8<NP>(y, pf[nm]);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const bf16x8 vf = widen8(vw[2 * g + i], 1.f);
+#pragma unroll
+                for (int nm = 0; nm < NM; ++nm)
+#pragma unroll
+                    for (int q = NP - 1; q >= 0; --q) o[nm][2 * g + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[nm][q], o[nm][2 * g + i], 0, 0, 0);
+            }
+        }
+    }
+
+    // the four waves' shares -> one
+#pragma unroll
+    for (int nm = 0; nm < NM; ++nm) {
+        l[nm] += __shfl_xor(l[nm], 16);
+        l[nm] += __shfl_xor(l[nm], 32);
+        if (kq == 0) {
+            sm[wave][nm * 16 + l15] = mx[nm];
+            sl[wave][nm * 16 + l15] = l[nm];
+        }
+    }
+#pragma unroll
+    for (int nm = 0; nm < NM; ++nm) {
+        __syncthreads();
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) so[wave][l15][32 * g + 8 * kq + e] = o[nm][2 * g + (e & 1)][e >> 1];
+        __syncthreads();
+        constexpr int W = D / 16;
+        const int row = threadIdx.x >> 4, d = (threadIdx.x & 15) * W, m = (mg * NM + nm) * 16 + row;
+        if (m < a.m_rows) {
+            float top = -INFINITY, sum = 0.f, acc[W] = {};
+            for (int w = 0; w < 4; ++w) top = fmaxf(top, sm[w][nm * 16 + row]);
+            for (int w = 0; w < 4; ++w) {
+                const float mw = sm[w][nm * 16 + row];
+                const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - top);
+                // (a wave without a visible slot has sum 0; one whose scores were all NaN keeps its NaN: NaN x 0)
+                sum += sl[w][nm * 16 + row] * f;
+#pragma unroll
+                for (int i = 0; i < W; ++i) acc[i] += so[w][row][d + i] * f;
+            }
+            if (a.splits == 1) {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+                for (int i = 0; i < W; ++i) acc[i] *= inv;
+                const int t = m / a.group, g = m - t * a.group;
+                store_n<W, T>((T*)a.out + (((size_t)r * a.tokens + t) * a.heads + h * a.group + g) * D + d, acc);
+            } else {
+                float* po = a.part_o + (((size_t)rh * a.splits + split) * a.m_rows + m) * D + d;
+                store_n<W, float>(po, acc);
+            }
+            if ((a.splits > 1 || COUNT) && (threadIdx.x & 15) == 0) a.part_ml[((size_t)rh * a.splits + split) * a.m_rows + m] = f32x2{top, sum};
+        }
+    }
+}
+
+// (largest score, sum of exponentials to it) of a query over all splits of its row
+__device__ __forceinline__ f32x2 join_ml(const AttendArgs& a, int rh, int m, int used) {
+    const f32x2* p = a.part_ml + (size_t)rh * a.splits * a.m_rows + m;
+    float top = -INFINITY, sum = 0.f;
+    for (int s = 0; s < used; ++s) top = fmaxf(top, p[(size_t)s * a.m_rows][0]);
+    for (int s = 0; s < used; ++s) {
+        const f32x2 ml = p[(size_t)s * a.m_rows];
+        sum += ml[1] * (ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - top));
+    }
+    return f32x2{top, sum};
+}
+
+// The splits of a row -> the output (blocks below `merge_blocks`), and the probabilities that each slot received, from the
+// stored scores (the others: 1024 slots of one row and head each).
+template <int TYPE, int D>
+__global__ __launch_bounds__(256) void kv4_join_kernel(AttendArgs a, int merge_blocks, int slot_blocks, float decay) {
+    using T = typename Elem<TYPE>::T;
+    const after_kv4& c = a.c;
+    if ((int)blockIdx.x < merge_blocks) {
+        constexpr int W = D / 16;
+        const long long item = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);  // (row, head, query)
+        const int d = (threadIdx.x & 15) * W;
+        if (item >= (long long)c.rows * c.kv_heads * a.m_rows) return;
+        const int rh = (int)(item / a.m_rows), m = (int)(item % a.m_rows), r = rh / c.kv_heads, h = rh % c.kv_heads;
+        const int len = row_length(c, r), chunk = split_chunk(len, a.splits), used = len ? (len + chunk - 1) / chunk : 0;
+        const f32x2 all = join_ml(a, rh, m, used);
+        const float inv = all[1] == 0.f ? 0.f : 1.f / all[1];
+        float acc[W] = {};
+        for (int s = 0; s < used; ++s) {
+            const size_t at = ((size_t)rh * a.splits + s) * a.m_rows + m;
+            const float ms = a.part_ml[at][0], f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - all[0]);
+            float x[W];
+            load_n<W, float>(a.part_o + at * D + d, x);
+#pragma unroll
+            for (int i = 0; i < W; ++i) acc[i] += x[i] * f;
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i) acc[i] *= inv;
+        const int t = m / a.group, g = m - t * a.group;
+        store_n<W, T>((T*)a.out + (((size_t)r * a.tokens + t) * a.heads + h * a.group + g) * D + d, acc);
+        return;
+    }
+    const int b = blockIdx.x - merge_blocks, rh = b / slot_blocks, r = rh / c.kv_heads;
+    const int len = row_length(c, r), s0 = (b % slot_blocks) * 1024;
+    if (s0 >= len) return;
+    const int chunk = split_chunk(len, a.splits), used = (len + chunk - 1) / chunk;
+    const int s = s0 + 4 * threadIdx.x;
+    __shared__ f32x2 ml[256];
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int m0 = 0; m0 < a.m_rows; m0 += 256) {
+        const int n = min(256, a.m_rows - m0);
+        __syncthreads();
+        if ((int)threadIdx.x < n) {
+            const f32x2 all = join_ml(a, rh, m0 + threadIdx.x, used);
+            ml[threadIdx.x] = f32x2{all[0] == -INFINITY ? 0.f : all[0], all[1] == 0.f ? 0.f : 1.f / all[1]};
+        }
+        __syncthreads();
+        if (s < len) {
+            const float* p = a.scores + ((size_t)rh * a.m_rows + m0) * c.capacity + s;
+            for (int m = 0; m < n; ++m) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(p + (size_t)m * c.capacity);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] += x[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[i] - ml[m][0]) * ml[m][1];
+            }
+        }
+    }
+    float* w = c.weights + (size_t)rh * c.capacity + s;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (s + i < len) w[i] = decay == 0.f ? sum[i] : fmaf(decay, w[i], sum[i]);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- evict
+// A key that orders floats as unsigned numbers, NaN below everything
+__device__ __forceinline__ unsigned order_key(float x) {
+    const unsigned u = __float_as_uint(x);
+    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 0u;
+    return u == 0x80000000u ? 0x80000000u : (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+constexpr int kSelThreads = 1024;
+
+// inclusive sum over the workgroup's threads; *total = the last one's.  `tmp`: one word per wave
+__device__ __forceinline__ int block_scan(int x, int* tmp, int* total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const int y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) tmp[wave] = x;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < kSelThreads / 64; ++w) {
+        if (w < wave) before += tmp[w];
+        all += tmp[w];
+    }
+    *total = all;
+    return x + before;
+}
+
+// One workgroup per (row, head): which slots stay, in order.  The `recent` newest stay; of the others the `want` with the
+// largest weights: the value of the smallest of those is found eleven bits at a time (a histogram of the next digit of the
+// candidates), then one ordered pass writes the slots above it, and the first of those equal to it.
+__global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(after_kv4 c, int keep, int recent, int* slots) {
+    __shared__ int hist[2048];
+    __shared__ int tmp[kSelThreads / 64];
+    __shared__ int found[2];
+    const int rh = blockIdx.x, r = rh / c.kv_heads, tid = threadIdx.x;
+    const int len = row_length(c, r);
+    int* out = slots + (size_t)rh * keep;
+    const float* w = c.weights + (size_t)rh * c.capacity;
+    for (int i = min(len, keep) + tid; i < keep; i += kSelThreads) out[i] = -1;
+    if (len <= keep) {
+        for (int i = tid; i < len; i += kSelThreads) out[i] = i;
+        return;
+    }
+    const int old = len - recent;  // (recent <= keep < len)
+    int want = keep - recent;
+    unsigned prefix = 0;
+    int total;
+    if (want > 0) {
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, bins = 1 << bits;
+            for (int i = tid; i < bins; i += kSelThreads) hist[i] = 0;
+            __syncthreads();
+            for (int i = tid; i < old; i += kSelThreads) {
+                const unsigned k = order_key(w[i]);
+                if (pass == 0 || (k >> (shift + bits)) == (prefix >> (shift + bits))) atomicAdd(&hist[k >> shift & (bins - 1)], 1);
+            }
+            __syncthreads();
+            // the digit in which the want-th largest lies: thread t looks at bins from the top, two each
+            const int per = bins / kSelThreads;
+            int mine = 0;
+            for (int i = 0; i < per; ++i) mine += hist[bins - 1 - (tid * per + i)];
+            const int upto = block_scan(mine, tmp, &total);
+            if (upto >= want && upto - mine < want) {
+                int above = upto - mine;
+                for (int i = 0; i < per; ++i) {
+                    const int bin = bins - 1 - (tid * per + i);
+                    if (above + hist[bin] >= want) {
+                        found[0] = bin;
+                        found[1] = want - above;
+                        break;
+                    }
+                    above += hist[bin];
+                }
+            }
+            __syncthreads();
+            prefix |= (unsigned)found[0] << shift;
+            want = found[1];  // of those equal to the prefix so far
+            __syncthreads();
+        }
+    }
+    // slots above the value, the first `want` equal to it, and the newest, in order
+    int done = 0, equal_done = 0;
+    const bool any = keep > recent;
+    for (int i0 = 0; i0 < len; i0 += kSelThreads) {
+        const int i = i0 + tid;
+        int above = 0, equal = 0;
+        if (i < len) {
+            if (i >= old)
+                above = 1;
+            else if (any) {
+                const unsigned k = order_key(w[i]);
+                above = k > prefix;
+                equal = k == prefix;
+            }
+        }
+        int n_equal, n_stay;
+        const int eq = block_scan(equal, tmp, &n_equal);
+        const int stay = above | (equal && equal_done + eq <= want);
+        const int at = block_scan(stay, tmp, &n_stay);
+        if (stay) out[done + at - 1] = i;
+        done += n_stay;
+        equal_done += n_equal;
+    }
+}
+
+// One wave per (row, head, block of eight kept slots): codes, scales and weights of the chosen slots, to their new places
+template <int D>
+__global__ __launch_bounds__(256) void kv4_move_kernel(after_kv4 c, after_kv4 to, int keep, const int* slots, int nb, long long items) {
+    constexpr int G = D / 32;
+    const int lane = threadIdx.x & 63;
+    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item >= items) return;
+    const size_t rh = item / nb;
+    const int sb = (int)(item % nb), r = (int)(rh / c.kv_heads);
+    const int n = min(row_length(c, r), keep);
+    if (sb == 0 && lane == 0 && rh % c.kv_heads == 0) to.lengths[r] = n;
+    if (8 * sb >= n) return;
+    const int* pick = slots + rh * keep + 8 * sb;
+    const size_t src = rh * c.capacity, dst = rh * to.capacity + 8 * sb;
+    if (lane < 8 && 8 * sb + lane < n) to.weights[dst + lane] = c.weights[src + pick[lane]];
+#pragma unroll
+    for (int it = 0; it < D / 64; ++it) {  // a dword (eight channels) per lane
+        const int id = it * 64 + lane, tt = id / (D / 8), ch = id % (D / 8);
+        if (8 * sb + tt < n)
+            reinterpret_cast<unsigned*>(to.keys + (dst + tt) * (D / 2))[ch] = reinterpret_cast<const unsigned*>(c.keys + (src + pick[tt]) * (D / 2))[ch];
+    }
+    if (lane < 8 * G) {
+        const int tt = lane / G, g = lane % G;
+        if (8 * sb + tt < n) {
+            to.key_scales[(dst + tt) * G + g] = c.key_scales[(src + pick[tt]) * G + g];
+            to.value_scales[(dst + tt) * G + g] = c.value_scales[(src + pick[tt]) * G + g];
+        }
+    }
+    if (2 * lane < D) {
+        u32x2 w = {0, 0};
+#pragma unroll
+        for (int tt = 0; tt < 8; ++tt) {
+            if (8 * sb + tt >= n) continue;
+            const int s = pick[tt];
+            const u32x2 x = reinterpret_cast<const u32x2*>(c.values + (src / 8 + s / 8) * (size_t)(4 * D))[lane];
+            w = w | (x >> 4 * (s & 7) & 15u) << 4 * tt;
+        }
+        reinterpret_cast<u32x2*>(to.values + (dst / 8) * (size_t)(4 * D))[lane] = w;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+int check_cache(const after_kv4* c, const char* what) {
+    AFTER_REQUIRE(c, AFTER_E_INVALID, "%s: no cache", what);
+    AFTER_REQUIRE(c->keys && c->key_scales && c->values && c->value_scales && c->weights && c->lengths && c->failed, AFTER_E_INVALID,
+                  "%s: a buffer of the cache is missing", what);
+    AFTER_REQUIRE(c->rows > 0 && c->kv_heads > 0 && (c->head_dim == 64 || c->head_dim == 128), AFTER_E_INVALID,
+                  "%s: rows and kv_heads > 0, head_dim 64 or 128 (got %d, %d, %d)", what, c->rows, c->kv_heads, c->head_dim);
+    AFTER_REQUIRE(c->capacity > 0 && c->capacity % 32 == 0 && c->capacity <= (1 << 24), AFTER_E_INVALID,
+                  "%s: capacity a multiple of 32, at most 2^24 (got %d)", what, c->capacity);
+    AFTER_REQUIRE((long long)c->rows * c->kv_heads <= (1 << 20), AFTER_E_INVALID, "%s: rows x kv_heads is at most 2^20", what);
+    return AFTER_OK;
+}
+bool known_type(int t) { return t == AFTER_T_F32 || t == AFTER_T_BF16 || t == AFTER_T_F16; }
+int type_bytes(int t) { return t == AFTER_T_F32 ? 4 : 2; }
+bool aligned16(const void* p) { return ((size_t)p & 15) == 0; }
+
+// Splits of a row: enough workgroups for the chip, none shorter than 256 slots at full length
+int attend_splits(const after_kv4& c, int mgroups) {
+    const long long units = (long long)c.rows * c.kv_heads * mgroups;
+    const long long wanted = (2048 + units - 1) / units, most = (c.capacity + 255) / 256;
+    return (int)(wanted < most ? wanted : most);
+}
+int attend_nm(int m_rows) { return m_rows > 16 ? 2 : 1; }
+
+struct Plan {
+    int m_rows, nm, mgroups, splits;
+    long long o_bytes, ml_bytes, s_bytes;
+};
+Plan attend_plan(const after_kv4& c, int heads, int tokens, bool count) {
+    Plan p;
+    p.m_rows = tokens * (heads / c.kv_heads);
+    p.nm = attend_nm(p.m_rows);
+    p.mgroups = cdiv(p.m_rows, 16 * p.nm);
+    p.splits = attend_splits(c, p.mgroups);
+    const long long n = (long long)c.rows * c.kv_heads * p.m_rows;
+    p.o_bytes = p.splits > 1 ? n * p.splits * c.head_dim * 4 : 0;
+    p.ml_bytes = p.splits > 1 || count ? (n * p.splits * 8 + 255) / 256 * 256 : 0;
+    p.s_bytes = count ? n * c.capacity * 4 : 0;
+    return p;
+}
+
+template <int TYPE, int D>
+int run_attend(const AttendArgs& a, const Plan& p, bool count, float decay, hipStream_t s) {
+    const long long units = cdivll((long long)a.c.rows * a.c.kv_heads * a.splits, 8) * 8 * a.mgroups;
+    const dim3 grid((unsigned)units), block(256);
+    if (p.nm == 1) {
+        if (count)
+            hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, 1, true>), grid, block, 0, s, a);
+        else
+            hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, 1, false>), grid, block, 0, s, a);
+    } else {
+        if (count)
+            hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, 2, true>), grid, block, 0, s, a);
+        else
+            hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, 2, false>), grid, block, 0, s, a);
+    }
+    if (a.splits > 1 || count) {
+        const int merge = a.splits > 1 ? (int)cdivll((long long)a.c.rows * a.c.kv_heads * a.m_rows, 16) : 0;
+        const int slots = cdiv(a.c.capacity, 1024), more = count ? a.c.rows * a.c.kv_heads * slots : 0;
+        hipLaunchKernelGGL((kv4_join_kernel<TYPE, D>), dim3(merge + more), block, 0, s, a, merge, slots, decay);
+    }
+    AFTER_HIP_CHECK(hipGetLastError());
+    return AFTER_OK;
+}
+
+#define KV4_BY_TYPE(type, dim, CALL)                                       \
+    do {                                                                   \
+        if ((dim) == 64) {                                                 \
+            if ((type) == AFTER_T_F32) CALL(AFTER_T_F32, 64);              \
+            else if ((type) == AFTER_T_BF16) CALL(AFTER_T_BF16, 64);       \
+            else CALL(AFTER_T_F16, 64);                                    \
+        } else {                                                           \
+            if ((type) == AFTER_T_F32) CALL(AFTER_T_F32, 128);             \
+            else if ((type) == AFTER_T_BF16) CALL(AFTER_T_BF16, 128);      \
+            else CALL(AFTER_T_F16, 128);                                   \
+        }                                                                  \
+    } while (0)
+
+}  // namespace
+}  // namespace after
+
+using namespace after;
+
+extern "C" int after_kv4_append(const after_kv4* c, const void* k, const void* v, int type, const int* starts, int tokens, long long total,
+                                long long k_token_stride, long long k_head_stride, long long v_token_stride, long long v_head_stride, void* stream) {
+    AFTER_TRY(check_cache(c, "kv4_append"));
+    AFTER_REQUIRE(known_type(type), AFTER_E_INVALID, "kv4_append: unknown element type %d", type);
+    AFTER_REQUIRE(total >= 0 && total < (1ll << 30) && tokens >= 0, AFTER_E_INVALID, "kv4_append: 0 <= total < 2^30 new tokens (got %lld)", total);
+    AFTER_REQUIRE(starts || (long long)tokens * c->rows == total, AFTER_E_INVALID, "kv4_append: total = rows x tokens without starts");
+    if (total == 0) return AFTER_OK;
+    const int per16 = 16 / type_bytes(type);
+    AFTER_REQUIRE(k && v && aligned16(k) && aligned16(v) && k_token_stride % per16 == 0 && k_head_stride % per16 == 0 && v_token_stride % per16 == 0 &&
+                      v_head_stride % per16 == 0,
+                  AFTER_E_INVALID, "kv4_append: k and v, their token and head strides must be 16-byte aligned");
+    hipStream_t s = (hipStream_t)stream;
+    const NewTokens nt{starts, tokens, (int)total};
+    const long long items = (total / 8 + 2ll * c->rows) * c->kv_heads;
+    AFTER_REQUIRE(items < (1ll << 31), AFTER_E_INVALID, "kv4_append: too many new tokens x heads for one call");
+#define CALL(T, D)                                                                                                                            \
+    hipLaunchKernelGGL((kv4_append_kernel<T, D>), dim3((unsigned)cdivll(items, 4)), dim3(256), 0, s, *c, nt, k, v, k_token_stride, k_head_stride, \
+                       v_token_stride, v_head_stride, (int)items)
+    KV4_BY_TYPE(type, c->head_dim, CALL);
+#undef CALL
+    hipLaunchKernelGGL(kv4_advance_kernel, dim3(cdiv(c->rows, 256)), dim3(256), 0, s, *c, nt);
+    AFTER_HIP_CHECK(hipGetLastError());
+    return AFTER_OK;
+}
+
+extern "C" int after_kv4_truncate(const after_kv4* c, const int* lengths, void* stream) {
+    AFTER_TRY(check_cache(c, "kv4_truncate"));
+    hipLaunchKernelGGL(kv4_truncate_kernel, dim3(cdiv(c->rows, 256)), dim3(256), 0, (hipStream_t)stream, *c, lengths);
+    AFTER_HIP_CHECK(hipGetLastError());
+    return AFTER_OK;
+}
+
+extern "C" int after_kv4_read(const after_kv4* c, void* k, void* v, int type, const int* start, int count, void* stream) {
+    AFTER_TRY(check_cache(c, "kv4_read"));
+    AFTER_REQUIRE(type == AFTER_T_F32 || type == AFTER_T_BF16, AFTER_E_INVALID, "kv4_read: values are written as fp32 or bf16 (both hold them exactly)");
+    AFTER_REQUIRE(count >= 0 && count <= c->capacity, AFTER_E_INVALID, "kv4_read: 0 <= count <= capacity (got %d)", count);
+    if (count == 0) return AFTER_OK;
+    AFTER_REQUIRE(k && v && aligned16(k) && aligned16(v), AFTER_E_INVALID, "kv4_read: k and v must be 16-byte aligned");
+    const int nb = count / 8 + 2;
+    const long long items = (long long)c->rows * c->kv_heads * nb;
+    AFTER_REQUIRE(items < (1ll << 32), AFTER_E_INVALID, "kv4_read: too many slots x heads for one call");
+#define CALL(T, D) \
+    hipLaunchKernelGGL((kv4_read_kernel<T, D>), dim3((unsigned)cdivll(items, 4)), dim3(256), 0, (hipStream_t)stream, *c, k, v, start, count, nb, items)
+    if (c->head_dim == 64) {
+        if (type == AFTER_T_F32) CALL(AFTER_T_F32, 64);
+        else CALL(AFTER_T_BF16, 64);
+    } else {
+        if (type == AFTER_T_F32) CALL(AFTER_T_F32, 128);
+        else CALL(AFTER_T_BF16, 128);
+    }
+#undef CALL
+    AFTER_HIP_CHECK(hipGetLastError());
+    return AFTER_OK;
+}
+
+static int check_attend(const after_kv4* c, int heads, int tokens, const char* what) {
+    AFTER_TRY(check_cache(c, what));
+    AFTER_REQUIRE(heads > 0 && heads % c->kv_heads == 0, AFTER_E_INVALID, "%s: heads must be a multiple of the cache's %d", what, c->kv_heads);
+    AFTER_REQUIRE(tokens > 0 && (long long)tokens * (heads / c->kv_heads) <= 65536, AFTER_E_INVALID, "%s: 1 .. 65536 / (heads / kv_heads) tokens (got %d)",
+                  what, tokens);
+    const Plan p = attend_plan(*c, heads, tokens, false);
+    AFTER_REQUIRE((long long)c->rows * c->kv_heads * p.splits * p.mgroups < (1ll << 30), AFTER_E_INVALID, "%s: too many rows x heads x tokens for one call", what);
+    return AFTER_OK;
+}
+
+extern "C" int after_kv4_attend_workspace(const after_kv4* c, int heads, int tokens, int accumulate, long long* bytes) {
+    AFTER_TRY(check_attend(c, heads, tokens, "kv4_attend_workspace"));
+    AFTER_REQUIRE(bytes, AFTER_E_INVALID, "kv4_attend_workspace: bytes is NULL");
+    const Plan p = attend_plan(*c, heads, tokens, accumulate != 0);
+    *bytes = p.o_bytes + p.ml_bytes + p.s_bytes;
+    return AFTER_OK;
+}
+
+extern "C" int after_kv4_attend(const after_kv4* c, const void* q, void* out, int type, int heads, int tokens, long long q_row_stride,
+                                long long q_token_stride, long long q_head_stride, float scale, int accumulate, float decay, void* workspace,
+                                long long workspace_bytes, void* stream) {
+    AFTER_TRY(check_attend(c, heads, tokens, "kv4_attend"));
+    AFTER_REQUIRE(known_type(type), AFTER_E_INVALID, "kv4_attend: unknown element type %d", type);
+    const int per16 = 16 / type_bytes(type);
+    AFTER_REQUIRE(q && out && aligned16(q) && aligned16(out) && q_row_stride % per16 == 0 && q_token_stride % per16 == 0 && q_head_stride % per16 == 0,
+                  AFTER_E_INVALID, "kv4_attend: q, its strides and out must be 16-byte aligned");
+    AFTER_REQUIRE(std::isfinite(scale) && std::isfinite(decay), AFTER_E_INVALID, "kv4_attend: scale and decay must be finite");
+    const bool count = accumulate != 0;
+    const Plan p = attend_plan(*c, heads, tokens, count);
+    const long long need = p.o_bytes + p.ml_bytes + p.s_bytes;
+    AFTER_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need), AFTER_E_CAPACITY,
+                  "kv4_attend: needs a 16-byte aligned workspace of %lld bytes (got %lld)", need, workspace_bytes);
+    AttendArgs a;
+    a.c = *c;
+    a.q = q;
+    a.out = out;
+    a.qrs = q_row_stride;
+    a.qts = q_token_stride;
+    a.qhs = q_head_stride;
+    a.heads = heads;
+    a.tokens = tokens;
+    a.group = heads / c->kv_heads;
+    a.m_rows = p.m_rows;
+    a.splits = p.splits;
+    a.mgroups = p.mgroups;
+    a.scale2 = scale * 1.44269504088896340736f;
+    char* w = (char*)workspace;
+    a.scores = count ? (float*)w : nullptr;
+    a.part_ml = (f32x2*)(w + p.s_bytes);
+    a.part_o = (float*)(w + p.s_bytes + p.ml_bytes);
+#define CALL(T, D) return run_attend<T, D>(a, p, count, decay, (hipStream_t)stream)
+    KV4_BY_TYPE(type, c->head_dim, CALL);
+#undef CALL
+    return AFTER_OK;
+}
+
+extern "C" int after_kv4_evict(const after_kv4* c, const after_kv4* to, int keep, int recent, int* slots, void* stream) {
+    AFTER_TRY(check_cache(c, "kv4_evict"));
+    AFTER_TRY(check_cache(to, "kv4_evict"));
+    AFTER_REQUIRE(to->rows == c->rows && to->kv_heads == c->kv_heads && to->head_dim == c->head_dim, AFTER_E_INVALID,
+                  "kv4_evict: both caches need the same rows, kv_heads and head_dim");
+    AFTER_REQUIRE(to->keys != c->keys && to->lengths != c->lengths, AFTER_E_INVALID, "kv4_evict: the slots move into another cache");
+    AFTER_REQUIRE(keep > 0 && keep <= to->capacity, AFTER_E_CAPACITY, "kv4_evict: keep %d slots, the other cache holds %d", keep, to->capacity);
+    AFTER_REQUIRE(recent >= 0 && recent <= keep, AFTER_E_INVALID, "kv4_evict: 0 <= recent <= keep (got %d of %d)", recent, keep);
+    AFTER_REQUIRE(slots, AFTER_E_INVALID, "kv4_evict: slots is NULL");
+    hipStream_t s = (hipStream_t)stream;
+    const int n_rh = c->rows * c->kv_heads, nb = cdiv(keep, 8);
+    const long long items = (long long)n_rh * nb;
+    AFTER_REQUIRE(items < (1ll << 32), AFTER_E_INVALID, "kv4_evict: too many slots x heads for one call");
+    hipLaunchKernelGGL(kv4_select_kernel, dim3(n_rh), dim3(kSelThreads), 0, s, *c, keep, recent, slots);
+    if (c->head_dim == 64)
+        hipLaunchKernelGGL((kv4_move_kernel<64>), dim3((unsigned)cdivll(items, 4)), dim3(256), 0, s, *c, *to, keep, slots, nb, items);
+    else
+        hipLaunchKernelGGL((kv4_move_kernel<128>), dim3((unsigned)cdivll(items, 4)), dim3(256), 0, s, *c, *to, keep, slots, nb, items);
+    AFTER_HIP_CHECK(hipGetLastError());
+    return AFTER_OK;
+}

@@ -562,6 +562,82 @@ long long after_conv_h3_launches(void);
    AFTER_AE_FUSE_K1=0 keeps them on the two launches (A/B switch) */
 long long after_conv1_act_launches(void);
 
+/* ------------------------------------------------------------------ attention over sequences
+ * Operators for sequences of different lengths whose keys and values are shared by groups of query heads, next to the
+ * attention inside DenoiserV2 (transformerv2.py:107-235) and its streaming K/V caches: of whole prompts, and over a cache
+ * that is held in four bits.  Elements are one of three types; strides count elements, the channels of a head are contiguous,
+ * and every pointer and stride of q, k and v is a multiple of 16 bytes.  Inference only, as everywhere here.  None of these
+ * calls synchronises, allocates or reads device memory on the host: all of them can be captured into a graph. */
+#define AFTER_T_F32 0
+#define AFTER_T_BF16 1
+#define AFTER_T_F16 2
+
+/* out[t, h, :] = sum_j softmax_j(scale * q[t, h, :] . k[j, h / (heads / kv_heads), :]) v[j, ...] for n_seqs sequences that
+ * stand one behind the other: queries of sequence b are the rows [q_starts[b], q_starts[b + 1]) of q / out [q_rows, heads, D],
+ * its keys the rows [k_starts[b], k_starts[b + 1]) of k / v [k_rows, kv_heads, D] (int32 device arrays of n_seqs + 1, from 0,
+ * ascending; entries outside [0, rows] are taken as the nearest of them).  The queries are the newest of their sequence's
+ * keys: query i of n stands at p = i + (keys - n).  causal: it sees the keys of its own chunk of `chunk` tokens and all chunks
+ * before (chunk = 1: the keys up to its own), and with window > 0 of the earlier chunks only keys > p - window, as DenoiserV2's
+ * mask does (transformerv2.py:62-96).  causal = 0: all keys.  A query that sees no key gets zeros; what a query does not see
+ * has no effect on it, NaN and infinities included.  Rows of out behind the last sequence stay as they are, or are set to
+ * zero with zero_rest.  D = 64 or 128.  fp32: fp32 products; bf16 / fp16: products of that type, sums and softmax in fp32. */
+int after_attend_packed(const void* q, const void* k, const void* v, void* out, int type, long long q_rows, long long k_rows,
+                        const int* q_starts, const int* k_starts, int n_seqs, int heads, int kv_heads, int head_dim,
+                        long long q_token_stride, long long q_head_stride, long long k_token_stride, long long k_head_stride,
+                        long long v_token_stride, long long v_head_stride, long long out_token_stride, long long out_head_stride,
+                        float scale, int causal, int window, int chunk, int zero_rest, void* stream);
+
+/* A cache of keys and values in four bits.  The caller owns the (device) buffers; the struct itself is passed from the host.
+ * 32 neighbouring channels of a token share one scale byte b, 2^(b - 127): the smallest power of two (16 <= b <= 252) with
+ * which none of them is beyond 6; a code is sign, two bits of exponent, one of fraction: +-{0, .5, 1, 1.5, 2, 3, 4, 6}, to
+ * nearest, ties to even.  b = 255: the group held an infinity or NaN and reads as NaN.
+ * Channel d of slot s in row r, head h:
+ *   keys   [rows][kv_heads][capacity][D / 2]: byte d / 2, low nibble for even d
+ *   values [rows][kv_heads][capacity / 8][D][4]: block s / 8, place (d / 2 % 16) * (D / 16) + d / 32 * 2 + d % 2, byte s % 8 / 2,
+ *          low nibble for even s
+ *   key_scales, value_scales [rows][kv_heads][capacity][D / 32]
+ *   weights [rows][kv_heads][capacity]: the attention each slot has received (after_kv4_attend)
+ *   lengths [rows]: slots in use (values outside [0, capacity] are taken as the nearest of them)
+ *   failed  [1]: set to 1 by an append that found no room for some of its tokens; nothing here clears it
+ * One call at a time works on a cache: calls on several streams are the caller's to order. */
+typedef struct after_kv4 {
+    unsigned char* keys;
+    unsigned char* key_scales;
+    unsigned char* values;
+    unsigned char* value_scales;
+    float* weights;
+    int* lengths;
+    int* failed;
+    int rows;
+    int kv_heads;
+    int head_dim; /* 64 or 128 */
+    int capacity; /* slots per row and head: a multiple of 32, at most 2^24 */
+} after_kv4;
+
+/* Puts new tokens behind each row's slots and adds them to lengths: k, v [total, kv_heads, D], those of row r at
+ * [starts[r], starts[r + 1]) (int32 [rows + 1]), or starts = NULL and `tokens` for each row.  Their weights become 0.
+ * Tokens for which a row has no room are dropped, and `failed` is set. */
+int after_kv4_append(const after_kv4* c, const void* k, const void* v, int type, const int* starts, int tokens, long long total,
+                     long long k_token_stride, long long k_head_stride, long long v_token_stride, long long v_head_stride, void* stream);
+/* lengths[r] = min(lengths[r], the given length); NULL: 0 for every row */
+int after_kv4_truncate(const after_kv4* c, const int* lengths, void* stream);
+/* The values of the slots [start[r], start[r] + count) (start = NULL: from 0) as k, v [rows, kv_heads, count, D], fp32 or bf16;
+ * zeros past a row's length. */
+int after_kv4_read(const after_kv4* c, void* k, void* v, int type, const int* start, int count, void* stream);
+/* out [rows, tokens, heads, D] (contiguous, of q's type): attention of the newest `tokens` tokens of each row, whose keys are
+ * in the cache already: query t sees the slots below lengths[r] - tokens + t + 1, none of them: zeros.  (A row with fewer new
+ * tokens than others has its queries at the end.)  accumulate: weights = decay * weights + the probabilities that each slot
+ * in use received, summed over tokens and the group's heads (decay = 0: they are replaced).  The workspace is scratch: its
+ * size depends on the arguments alone, and two calls that may run at the same time need two. */
+int after_kv4_attend_workspace(const after_kv4* c, int heads, int tokens, int accumulate, long long* bytes);
+int after_kv4_attend(const after_kv4* c, const void* q, void* out, int type, int heads, int tokens, long long q_row_stride,
+                     long long q_token_stride, long long q_head_stride, float scale, int accumulate, float decay, void* workspace,
+                     long long workspace_bytes, void* stream);
+/* Moves, per row and head, min(length, keep) slots into the cache `to` (same rows, kv_heads, head_dim; its former content is
+ * replaced), in their order: the `recent` newest, and of the others those with the largest weights (NaN counts as the
+ * smallest; ties go to the lower slot).  slots [rows, kv_heads, keep]: where each came from, -1 past the new length.  `c` stays as it is. */
+int after_kv4_evict(const after_kv4* c, const after_kv4* to, int keep, int recent, int* slots, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
