@@ -291,6 +291,8 @@ def _cache(s, capacity):
     c = s["case"]
     if "handle" not in s:
         s["handle"] = KVCache4(c["rows"], c["kv_heads"], c["dim"], c["capacity"], device="cuda", buffers=s.get("cache"))
+        if c["op"] == "append":
+            s["handle"].lengths.copy_(s["held"])  # its rows hold that many slots already
         if c["op"] == "evict":
             s["smaller"] = KVCache4(c["rows"], c["kv_heads"], c["dim"], capacity, device="cuda")
     return s["handle"]
