@@ -15,11 +15,11 @@
 #include <cmath>
 
 #include "common.h"
+#include "gemm_pipe.h"
 
 namespace after {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -53,7 +53,8 @@ struct PackedArgs {
     const int *qs, *ks;
     long long qts, qhs, kts, khs, vts, vhs, ots, ohs;
     int q_rows, k_rows, n_seqs, heads, kv_heads, group, tiles;
-    float scale2;
+    float scale2;     // |scale| log2 e, > 0 (a masked score, -inf, stays -inf)
+    unsigned q_sign;  // the sign bits of a word of q, if scale is negative
     int causal, window, chunk, zero_rest;
 };
 
@@ -80,12 +81,12 @@ __device__ __forceinline__ void seen(const PackedArgs& a, int p, int keys, int& 
 // 16-byte pieces of a 64-row tile in LDS.  Keys: a wave reads the same piece of 32 rows, so a row's pieces are permuted by its
 // number; values (16-bit types): a transposing read takes 32 bytes each of four neighbouring rows, so pairs of pieces are.
 template <int PIECES>
-__device__ __forceinline__ int k_piece(int row, int c) {
-    return row * PIECES + (c ^ (row & (PIECES < 16 ? PIECES - 1 : 15)));
+__device__ __forceinline__ int k_flip(int row) {
+    return row & (PIECES == 16 ? 15 : 7);
 }
 template <int PIECES>
-__device__ __forceinline__ int v_piece(int row, int c) {
-    return row * PIECES + (c ^ ((row & (PIECES < 16 ? 3 : 7)) << 1));
+__device__ __forceinline__ int v_flip(int row) {
+    return (row & (PIECES < 16 ? 3 : 7)) << 1;
 }
 
 // whether one of the words' elements is an infinity or NaN
@@ -104,15 +105,14 @@ __device__ __forceinline__ bool odd_value(u32x4 w) {
 }
 
 template <int TYPE, int D>
-__global__ __launch_bounds__(256) void attend_packed_kernel(PackedArgs a) {
+__global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 : 2) void attend_packed_kernel(PackedArgs a) {
     using E = Elem<TYPE>;
     using T = typename E::T;
     constexpr int PIECES = D * (int)sizeof(T) / 16;  // 16-byte pieces of a row
     constexpr int LOADS = BN * PIECES / 256;         // pieces per thread of a tile
     constexpr int DT = D / 32;
+    constexpr unsigned STAGE = 2 * BN * PIECES * 16;
     extern __shared__ __align__(16) char lds[];
-    u32x4* lk = reinterpret_cast<u32x4*>(lds);
-    u32x4* lv = lk + BN * PIECES;
     __shared__ unsigned long long odd_rows;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, half = lane >> 5;
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(256) void attend_packed_kernel(PackedArgs a) {
     constexpr int QN = sizeof(T) == 4 ? D / 8 : D / 16;
     u32x4 qf[QN];
 #pragma unroll
-    for (int s = 0; s < QN; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qp + (2 * s + half) * (16 / (int)sizeof(T)));
+    for (int s = 0; s < QN; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qp + (2 * s + half) * (16 / (int)sizeof(T))) ^ a.q_sign;
 
     f32x16 o[DT];
 #pragma unroll
@@ -166,47 +166,60 @@ __global__ __launch_bounds__(256) void attend_packed_kernel(PackedArgs a) {
         for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
     float mx = -INFINITY, l = 0.f;
 
+    // K and V tiles go from memory to LDS without passing registers, two stages: while a tile is computed the next is on its way.
+    // A lane's place in LDS is its number, so the pieces are permuted by the address it reads from.  Rows behind the sequence
+    // repeat its last one: they are masked, and taken out below where that one holds an infinity or NaN.
     const int n_first = t_first / BN, n_last = (t_last + BN - 1) / BN;  // key tiles
-    u32x4 rk[LOADS], rv[LOADS];
-    auto fetch = [&](int n) {
+    const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) char*)lds;
+    constexpr int ROWS = 256 / PIECES;  // rows that one piece per thread covers: the permutations repeat after them
+    const int fr = tid / PIECES, fc = tid % PIECES;
+    const unsigned kc = (fc ^ k_flip<PIECES>(fr)) * 16, vc = (sizeof(T) == 4 ? fc : fc ^ v_flip<PIECES>(fr)) * 16;
+    const unsigned kb = (unsigned)a.kts * (unsigned)sizeof(T), vb = (unsigned)a.vts * (unsigned)sizeof(T);  // (< 2^24: checked on the host)
+    const unsigned k_at = fr * kb + kc, v_at = fr * vb + vc;
+    auto fetch = [&](int n, int stage) {
+        const unsigned to = lds0 + stage * STAGE + wave * 1024;
+        const unsigned long long kt = reinterpret_cast<unsigned long long>(kp) + (unsigned long long)n * BN * kb;
+        const unsigned long long vt = reinterpret_cast<unsigned long long>(vp) + (unsigned long long)n * BN * vb;
+        if ((n + 1) * BN <= nk) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int id = i * 256 + tid, r = id / PIECES, c = id % PIECES, j = n * BN + r;
-            rk[i] = rv[i] = u32x4{0, 0, 0, 0};  // (rows behind the sequence are zeros, whatever stands there)
-            if (j < nk) {
-                rk[i] = *reinterpret_cast<const u32x4*>(kp + (long long)j * a.kts + c * (16 / (int)sizeof(T)));
-                rv[i] = *reinterpret_cast<const u32x4*>(vp + (long long)j * a.vts + c * (16 / (int)sizeof(T)));
+            for (int i = 0; i < LOADS; ++i) {
+                lds_dma16(to + i * 4096, k_at, kt + i * ROWS * kb);
+                lds_dma16(to + i * 4096 + STAGE / 2, v_at, vt + i * ROWS * vb);
+            }
+        } else {
+            const int left = nk - 1 - n * BN;
+            for (int i = 0; i < LOADS; ++i) {
+                const unsigned j = min(i * ROWS + fr, left);
+                lds_dma16(to + i * 4096, j * kb + kc, kt);
+                lds_dma16(to + i * 4096 + STAGE / 2, j * vb + vc, vt);
             }
         }
     };
-    if (n_first < n_last) fetch(n_first);
+    if (n_first < n_last) fetch(n_first, 0);
     for (int n = n_first; n < n_last; ++n) {
         const bool masked = n * BN < all_first || (n + 1) * BN > all_last;
-        __syncthreads();
-        if (masked && tid == 0) odd_rows = 0;
-        if (masked) __syncthreads();
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int id = i * 256 + tid, r = id / PIECES, c = id % PIECES;
-            lk[k_piece<PIECES>(r, c)] = rk[i];
-            lv[sizeof(T) == 4 ? id : v_piece<PIECES>(r, c)] = rv[i];
-            // what a query does not see must not reach it: 0 x NaN would
-            if (masked && odd_value<TYPE>(rv[i])) atomicOr(&odd_rows, 1ull << r);
-        }
-        __syncthreads();
+        const int stage = (n - n_first) & 1;
+        u32x4* lk = reinterpret_cast<u32x4*>(lds + stage * STAGE);
+        u32x4* lv = lk + BN * PIECES;
+        wait_vmcnt_imm<0>();
+        __syncthreads();  // the tile is there, and nobody reads the other stage any more
+        if (n + 1 < n_last) fetch(n + 1, stage ^ 1);
         unsigned long long odd = 0;
-        if (masked) {
+        if (masked) {  // what a query does not see must not reach it, but 0 x NaN would
+            if (tid == 0) odd_rows = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i)
+                if (odd_value<TYPE>(lv[i * 256 + tid])) atomicOr(&odd_rows, 1ull << (i * 256 + tid) / PIECES);
+            __syncthreads();
             odd = odd_rows;
             if (odd) {  // (rare) such rows are taken out of the product and added one by one below
 #pragma unroll
-                for (int i = 0; i < LOADS; ++i) {
-                    const int id = i * 256 + tid, r = id / PIECES, c = id % PIECES;
-                    if (odd >> r & 1) lv[sizeof(T) == 4 ? id : v_piece<PIECES>(r, c)] = u32x4{0, 0, 0, 0};
-                }
+                for (int i = 0; i < LOADS; ++i)
+                    if (odd >> (i * 256 + tid) / PIECES & 1) lv[i * 256 + tid] = u32x4{0, 0, 0, 0};
                 __syncthreads();
             }
         }
-        if (n + 1 < n_last) fetch(n + 1);
 
         f32x16 sc[2];
 #pragma unroll
@@ -215,7 +228,7 @@ __global__ __launch_bounds__(256) void attend_packed_kernel(PackedArgs a) {
             for (int e = 0; e < 16; ++e) sc[f][e] = 0.f;
 #pragma unroll
             for (int s = 0; s < QN; ++s) {
-                const u32x4 kf = lk[k_piece<PIECES>(32 * f + l31, 2 * s + half)];
+                const u32x4 kf = lk[(32 * f + l31) * PIECES + ((2 * s + half) ^ k_flip<PIECES>(l31))];
                 if constexpr (sizeof(T) == 4) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
@@ -224,21 +237,24 @@ __global__ __launch_bounds__(256) void attend_packed_kernel(PackedArgs a) {
                     sc[f] = E::mfma(__builtin_bit_cast(typename E::V8, kf), __builtin_bit_cast(typename E::V8, qf[s]), sc[f]);
             }
         }
+        if (masked) {
+            const int j0 = n * BN + 4 * half;
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int j = j0 + 32 * f + 8 * (e >> 2) + (e & 3);
+                    sc[f][e] = j >= first && j < last ? sc[f][e] : -INFINITY;
+                }
+        }
         float top = -INFINITY;
 #pragma unroll
         for (int f = 0; f < 2; ++f)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                float x = sc[f][e] * a.scale2;
-                if (masked) {
-                    const int j = n * BN + 32 * f + 8 * (e >> 2) + 4 * half + (e & 3);
-                    x = j >= first && j < last ? x : -INFINITY;
-                }
-                sc[f][e] = x;
-                top = fmaxf(top, x);
-            }
-        top = fmaxf(top, __shfl_xor(top, 32));
-        if (__any(top > mx)) {
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[f][e]);
+        top = fmaxf(top, __shfl_xor(top, 32)) * a.scale2;
+        // the maximum moves only when scores outgrow it by 2^8: probabilities up to 256 are as exact, and a rescale is rare
+        if (__any(top > mx + 8.f)) {
             const float now = fmaxf(mx, top), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - now);
             mx = now;
             l *= f;
@@ -250,7 +266,7 @@ __global__ __launch_bounds__(256) void attend_packed_kernel(PackedArgs a) {
         for (int f = 0; f < 2; ++f)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                sc[f][e] = __builtin_amdgcn_exp2f(sc[f][e] - off);
+                sc[f][e] = __builtin_amdgcn_exp2f(fmaf(sc[f][e], a.scale2, -off));
                 l += sc[f][e];
             }
         // O^T += V^T P^T
@@ -283,7 +299,7 @@ __global__ __launch_bounds__(256) void attend_packed_kernel(PackedArgs a) {
                             const int r = 32 * f + 16 * s + 8 * w + 4 * half + ((lane & 15) >> 2);
                             const int byte = 64 * i + (lane & 16) * 2 + (lane & 3) * 8;
                             vf.p[w] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                (__attribute__((address_space(3))) s16x4*)(vv + 16 * v_piece<PIECES>(r, byte >> 4) + (byte & 15)));
+                                (__attribute__((address_space(3))) s16x4*)(vv + 16 * (r * PIECES + ((byte >> 4) ^ v_flip<PIECES>(r))) + (byte & 15)));
                         }
                         o[i] = E::mfma(vf.v, pf, o[i]);
                     }
@@ -329,7 +345,7 @@ __global__ __launch_bounds__(256) void attend_packed_kernel(PackedArgs a) {
 
 template <int TYPE, int D>
 int run_packed(const PackedArgs& a, hipStream_t s) {
-    constexpr size_t lds = 2 * BN * D * sizeof(typename Elem<TYPE>::T);
+    constexpr size_t lds = 4 * BN * D * sizeof(typename Elem<TYPE>::T);
     static LdsAttr attr;
     AFTER_TRY(ensure_lds_attr(attr, (const void*)attend_packed_kernel<TYPE, D>, lds));
     hipLaunchKernelGGL((attend_packed_kernel<TYPE, D>), dim3((unsigned)a.tiles * a.kv_heads), dim3(256), lds, s, a);
@@ -364,13 +380,16 @@ extern "C" int after_attend_packed(const void* q, const void* k, const void* v, 
     AFTER_REQUIRE(q && out && q_starts && k_starts && (k_rows == 0 || (k && v)), AFTER_E_INVALID, "attend_packed: a pointer is NULL");
     AFTER_REQUIRE((((size_t)q | (size_t)k | (size_t)v | (size_t)out) & 15) == 0 && (strides & (per16 - 1)) == 0, AFTER_E_INVALID,
                   "attend_packed: q, k, v, out and their token and head strides must be multiples of 16 bytes");
+    AFTER_REQUIRE(k_token_stride >= 0 && v_token_stride >= 0 && k_token_stride < (1 << 22) && v_token_stride < (1 << 22), AFTER_E_INVALID,
+                  "attend_packed: the token strides of k and v must be below 2^22 elements");
     PackedArgs a;
     a.q = q, a.k = k, a.v = v, a.out = out, a.qs = q_starts, a.ks = k_starts;
     a.qts = q_token_stride, a.qhs = q_head_stride, a.kts = k_token_stride, a.khs = k_head_stride;
     a.vts = v_token_stride, a.vhs = v_head_stride, a.ots = out_token_stride, a.ohs = out_head_stride;
     a.q_rows = (int)q_rows, a.k_rows = (int)k_rows, a.n_seqs = n_seqs, a.heads = heads, a.kv_heads = kv_heads, a.group = group;
     a.tiles = (int)(q_rows * group / BM) + n_seqs + 1;
-    a.scale2 = scale * 1.44269504088896340736f;
+    a.scale2 = std::fmax(std::fabs(scale) * 1.44269504088896340736f, 1e-30f);
+    a.q_sign = scale < 0 ? (type == AFTER_T_F32 ? 0x80000000u : 0x80008000u) : 0u;
     a.causal = causal != 0, a.window = window < (1 << 30) ? window : 1 << 30, a.chunk = chunk, a.zero_rest = zero_rest;
     AFTER_REQUIRE((long long)a.tiles * kv_heads < (1ll << 31), AFTER_E_INVALID, "attend_packed: too many tokens x heads for one call");
     hipStream_t s = (hipStream_t)stream;
