@@ -40,10 +40,30 @@ def _operand(t, name, dims, device=None, dtype=None):
         raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
     if t.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError(f"{name} requires a gradient: after_amd is inference only (use torch.no_grad())")
-    size = t.element_size()
-    if t.numel() and (t.stride(-1) != 1 or t.data_ptr() % 16 or any(s * size % 16 for s in t.stride()[:-1])):
+    if not t.numel():
+        return t
+    *outer, last = t.stride()
+    each = 3 if t.dtype == torch.float32 else 7  # (elements in 16 bytes, less one)
+    odd = 0
+    for s in outer:
+        odd |= s
+    # (a token's place in a tile is addressed with 32 bits)
+    if last != 1 or odd & each or t.data_ptr() & 15 or outer[-2] >= 1 << 22:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
+
+
+def _enqueue(name, device, *args):
+    """One call of the C ABI on the device's current stream."""
+    index, fn = device.index, getattr(_lib.lib(), name)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc, name)
 
 
 def _starts(t, name, n, device):
@@ -98,13 +118,9 @@ def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=True, window=None,
     elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device \
             or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f"out must be a contiguous, 16-byte aligned {q.dtype} tensor {tuple(q.shape)} on {q.device}")
-    with torch.cuda.device(q.device):
-        _lib.check(
-            _lib.lib().after_attend_packed(_lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(out), _TYPES[q.dtype], n, k.shape[0],
-                                           _lib.ptr(q_starts), _lib.ptr(k_starts), q_starts.numel() - 1, heads, k.shape[1], dim,
-                                           q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                                           out.stride(0), out.stride(1), scale, int(bool(causal)), window or 0, chunk, int(fresh),
-                                           _lib.current_stream(q.device)), "after_attend_packed")
+    _enqueue("after_attend_packed", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _TYPES[q.dtype], n, k.shape[0],
+             q_starts.data_ptr(), k_starts.data_ptr(), q_starts.numel() - 1, heads, k.shape[1], dim, *q.stride()[:2], *k.stride()[:2],
+             *v.stride()[:2], *out.stride()[:2], scale, int(bool(causal)), window or 0, chunk, int(fresh))
     return out
 
 
@@ -151,15 +167,12 @@ class KVCache4:
         self._failed = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._c = _lib.KV4(*(t.data_ptr() for t in self.buffers().values()), self._failed.data_ptr(), rows, kv_heads, head_dim, C)
         self._ref = ctypes.byref(self._c)
+        self._work = {}  # (heads, tokens, accumulate) -> bytes of an attend call's scratch
 
     def buffers(self):
         """The six tensors of the state, by name."""
         return dict(keys=self.keys, key_scales=self.key_scales, values=self.values, value_scales=self.value_scales,
                     weights=self.weights, lengths=self.lengths)
-
-    def _call(self, name, *args):
-        with torch.cuda.device(self.device):
-            _lib.check(getattr(_lib.lib(), name)(self._ref, *args, _lib.current_stream(self.device)), name)
 
     def _row_values(self, t, name):
         if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != (self.rows, ) or t.device != self.device:
@@ -183,12 +196,13 @@ class KVCache4:
             k, v = k.flatten(0, 1), v.flatten(0, 1)
         else:
             starts = _starts(starts, "starts", self.rows, self.device)
-        self._call("after_kv4_append", _lib.ptr(k), _lib.ptr(v), _TYPES[k.dtype], _lib.ptr(starts), tokens, k.shape[0],
-                   k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+        _enqueue("after_kv4_append", self.device, self._ref, k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], None if starts is None else starts.data_ptr(),
+                 tokens, k.shape[0], *k.stride()[:2], *v.stride()[:2])
 
     def truncate(self, lengths=None):
         """Takes back the newest slots: row r keeps the first lengths[r] (int32 [rows] on the device); None empties the cache."""
-        self._call("after_kv4_truncate", _lib.ptr(None if lengths is None else self._row_values(lengths, "lengths")))
+        lengths = None if lengths is None else self._row_values(lengths, "lengths")
+        _enqueue("after_kv4_truncate", self.device, self._ref, None if lengths is None else lengths.data_ptr())
 
     def read(self, start=None, count=None, dtype=torch.bfloat16):
         """(k, v) [rows, kv_heads, count, head_dim]: the values that the slots start[r] .. start[r] + count - 1 stand for (int32
@@ -200,7 +214,7 @@ class KVCache4:
             raise TypeError(f"values are read as bfloat16 or float32, got {dtype}")
         start = None if start is None else self._row_values(start, "start")
         k, v = (torch.empty(self.rows, self.kv_heads, count, self.head_dim, dtype=dtype, device=self.device) for _ in range(2))
-        self._call("after_kv4_read", _lib.ptr(k), _lib.ptr(v), _TYPES[dtype], _lib.ptr(start), count)
+        _enqueue("after_kv4_read", self.device, self._ref, k.data_ptr(), v.data_ptr(), _TYPES[dtype], None if start is None else start.data_ptr(), count)
         return k, v
 
     def attend(self, q, scale=None, accumulate=False, decay=1.0):
@@ -222,13 +236,17 @@ class KVCache4:
             if accumulate and decay != 1.0:
                 raise ValueError("accumulate with a decay needs at least one token")
             return out
-        size = ctypes.c_longlong()
-        _lib.check(_lib.lib().after_kv4_attend_workspace(self._ref, heads, tokens, int(bool(accumulate)), ctypes.byref(size)),
-                   "after_kv4_attend_workspace")
+        accumulate = int(bool(accumulate))
+        key = (heads, tokens, accumulate)
+        if key not in self._work:
+            size = ctypes.c_longlong()
+            _lib.check(_lib.lib().after_kv4_attend_workspace(self._ref, heads, tokens, accumulate, ctypes.byref(size)), "after_kv4_attend_workspace")
+            self._work[key] = size.value
         # (scratch of this call: the allocator gives it to later calls of this stream only, and to a captured graph its own)
-        work = torch.empty(size.value, dtype=torch.uint8, device=self.device)
-        self._call("after_kv4_attend", _lib.ptr(q), _lib.ptr(out), _TYPES[q.dtype], heads, tokens, q.stride(0), q.stride(1), q.stride(2),
-                   scale, int(bool(accumulate)), decay, _lib.ptr(work), size.value)
+        size = self._work[key]
+        work = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
+        _enqueue("after_kv4_attend", self.device, self._ref, q.data_ptr(), out.data_ptr(), _TYPES[q.dtype], heads, tokens, *q.stride()[:3],
+                 scale, accumulate, decay, None if work is None else work.data_ptr(), size)
         return out
 
     def evict(self, into, keep, recent=0):
@@ -247,7 +265,7 @@ class KVCache4:
         if not 1 <= keep <= into.capacity or not 0 <= recent <= keep:
             raise ValueError(f"1 <= keep <= {into.capacity} and 0 <= recent <= keep, got {keep} and {recent}")
         slots = torch.empty(self.rows, self.kv_heads, keep, dtype=torch.int32, device=self.device)
-        self._call("after_kv4_evict", into._ref, keep, recent, _lib.ptr(slots))
+        _enqueue("after_kv4_evict", self.device, self._ref, into._ref, keep, recent, slots.data_ptr())
         return slots
 
     def check(self):
