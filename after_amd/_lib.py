@@ -159,7 +159,7 @@ SIGNATURES = {
     "after_kv4_append": (c_int, [POINTER(KV4), c_void_p, c_void_p, c_int, c_void_p, c_int] + [c_longlong] * 5 + [c_void_p]),
     "after_kv4_truncate": (c_int, [POINTER(KV4), c_void_p, c_void_p]),
     "after_kv4_read": (c_int, [POINTER(KV4), c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p]),
-    "after_kv4_attend_workspace": (c_int, [POINTER(KV4), c_int, c_int, c_int, POINTER(c_longlong)]),
+    "after_kv4_attend_workspace": (c_int, [POINTER(KV4), c_int, c_int, c_int, c_int, POINTER(c_longlong)]),
     "after_kv4_attend": (c_int, [POINTER(KV4), c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong, c_float,
                                  c_int, c_float, c_void_p, c_longlong, c_void_p]),
     "after_kv4_evict": (c_int, [POINTER(KV4), POINTER(KV4), c_int, c_int, c_void_p, c_void_p]),

@@ -167,7 +167,7 @@ class KVCache4:
         self._failed = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._c = _lib.KV4(*(t.data_ptr() for t in self.buffers().values()), self._failed.data_ptr(), rows, kv_heads, head_dim, C)
         self._ref = ctypes.byref(self._c)
-        self._work = {}  # (heads, tokens, accumulate) -> bytes of an attend call's scratch
+        self._work = {}  # (type, heads, tokens, accumulate) -> bytes of an attend call's scratch
 
     def buffers(self):
         """The six tensors of the state, by name."""
@@ -237,10 +237,10 @@ class KVCache4:
                 raise ValueError("accumulate with a decay needs at least one token")
             return out
         accumulate = int(bool(accumulate))
-        key = (heads, tokens, accumulate)
+        key = (q.dtype, heads, tokens, accumulate)
         if key not in self._work:
             size = ctypes.c_longlong()
-            _lib.check(_lib.lib().after_kv4_attend_workspace(self._ref, heads, tokens, accumulate, ctypes.byref(size)), "after_kv4_attend_workspace")
+            _lib.check(_lib.lib().after_kv4_attend_workspace(self._ref, _TYPES[q.dtype], *key[1:], ctypes.byref(size)), "after_kv4_attend_workspace")
             self._work[key] = size.value
         # (scratch of this call: the allocator gives it to later calls of this stream only, and to a captured graph its own)
         size = self._work[key]

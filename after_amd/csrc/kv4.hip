@@ -17,15 +17,17 @@
 #include <cmath>
 
 #include "common.h"
+#include "gemm_pipe.h"
 
 namespace after {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
@@ -258,16 +260,26 @@ struct AttendArgs {
     void* out;  // [rows][tokens][heads][D]
     long long qrs, qts, qhs;
     int heads, tokens, group, m_rows;  // m_rows = tokens * group
-    int splits, mgroups;
-    float scale2;  // scale * log2(e)
-    float* part_o;  // [rows * H][splits][m_rows][D]
-    f32x2* part_ml; // [rows * H][splits][m_rows]
-    float* scores;  // [rows * H][m_rows][C] or nullptr
+    int workers;      // waves that share the work (below); 0: a workgroup for each row and head
+    float scale2;     // |scale| log2(e), > 0 (a masked score, -inf, stays -inf)
+    float q_sign;     // the scale's sign, on the queries
+    float* part_o;    // [pieces][m_rows][D]: a piece is one worker's part of a row and head, number worker + row * H + head
+    f32x2* part_ml;   // [pieces][m_rows]: largest score, sum of exponentials to it
+    int2* ends;       // [rows * H]: the first and the last piece of a row and head, written by the workers that hold its ends
+    float* scores;    // [rows * H][m_rows][C] or nullptr
 };
 
-// tokens per split of a row: whole tiles of 32
-__device__ __forceinline__ int split_chunk(int len, int splits) { return ((len + splits - 1) / splits + 31) & ~31; }
-
+// How the slots in use are shared out: the steps of 32 slots of all rows and heads, one behind the other, are cut into equal
+// shares, one for each wave on the chip, wherever that cuts a row.  So all end together however different the rows are, and
+// there are no more ends than waves, rows and heads; no wave waits for another.  Lengths are on the device: every wave looks at
+// them (64 at a time) before it begins.
+constexpr int kStep = 32;
+__device__ __forceinline__ long long wave_sum(long long x) {
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) x += __shfl_xor(x, o);
+    return x;
+}
+__device__ __forceinline__ int row_steps(const after_kv4& c, int r) { return (row_length(c, r) + kStep - 1) / kStep; }
 template <int N>
 __device__ __forceinline__ void pieces8(const float (&x)[8], bf16x8 (&p)[N]) {
     float rest[8];
@@ -284,24 +296,82 @@ __device__ __forceinline__ void pieces8(const float (&x)[8], bf16x8 (&p)[N]) {
     }
 }
 
-template <int TYPE, int D, int NM, bool COUNT>
+constexpr int kRing = 3;  // tiles of 32 tokens that each wave has in LDS
+template <int D>
+constexpr int kTileBytes = 32 * D + 2 * D;  // keys, values, key scales, value scales
+
+// A lane's share of 32 tokens as they lie in memory
+template <int D>
+struct Tile {
+    unsigned k[2][D / 32];  // keys: D / 4 channels of two tokens
+    unsigned v[D / 16];     // values: eight tokens of D / 16 channels
+    unsigned vs[D / 16];    // the scale bytes of those tokens, [token][group]
+    unsigned look;          // one word of vs for every lane of 16: together all of them
+    unsigned char ks[2];    // the scale bytes of the keys' group
+};
+
+// JOINT: a workgroup's four waves take the tiles of one row and head in turn and add up in LDS (short rows: one launch);
+// otherwise every wave is a worker of its own.
+template <int TYPE, int D, int NM, bool COUNT, bool JOINT>
 __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
     using T = typename Elem<TYPE>::T;
     constexpr int NP = TYPE == AFTER_T_BF16 ? 1 : TYPE == AFTER_T_F16 ? 2 : 3;
     constexpr int G = D / 32, S = D / 32, KW = D / 32, VW = D / 16;  // groups, steps of a score, dwords of keys / values per lane
-    __shared__ float so[4][16][D + 4];
-    __shared__ float sm[4][NM * 16], sl[4][NM * 16];
+    constexpr int RING = kRing, BYTES = kTileBytes<D>, LOADS = D / 32 + 1;
+    constexpr int STRIDE = JOINT ? 128 : 32;  // tokens from one tile of a wave to its next
+    extern __shared__ __align__(16) char lds[];  // [4][RING][BYTES]; JOINT: then [4][16][D + 4] floats
     const after_kv4& c = a.c;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, kq = lane >> 4;
-    // neighbours in x are dispatched to different XCDs: the query groups of one piece of the cache stand 8 apart, on one L2
-    const int x = blockIdx.x, mg = (x >> 3) % a.mgroups, unit = (x >> 3) / a.mgroups * 8 + (x & 7);
-    const int n_rh = c.rows * c.kv_heads;
-    if (unit >= n_rh * a.splits) return;
-    const int rh = unit % n_rh, split = unit / n_rh, r = rh / c.kv_heads, h = rh % c.kv_heads;
-    const int len = row_length(c, r);
-    const int chunk = split_chunk(len, a.splits);
-    const int begin = split * chunk, end = min(begin + chunk, len);
-    if (begin >= end && (split > 0 || a.splits > 1)) return;  // (an empty row of an unsplit call still writes its zeros)
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, kq = lane >> 4;
+    const int mg = blockIdx.y;
+
+    // the first row and head of this worker's share, and where in it the share begins
+    const int worker = blockIdx.x * 4 + wave;
+    int r, h, step = 0;
+    long long left = 1;
+    if constexpr (JOINT) {
+        r = blockIdx.x / c.kv_heads;
+        h = blockIdx.x % c.kv_heads;
+    } else {
+        long long all = 0;
+        for (int i = lane; i < c.rows; i += 64) all += row_steps(c, i);
+        all = wave_sum(all);
+        const long long share = (all * c.kv_heads + a.workers - 1) / a.workers, at = share * worker;
+        const long long mine = min(share, all * c.kv_heads - at);
+        if (mine <= 0) return;
+        left = (long long)__builtin_amdgcn_readfirstlane((int)(mine >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)mine);
+        long long before = 0;
+        int r0 = 0;
+        for (;; r0 += 64) {  // (ends: at < all * H, which the last row's sum reaches)
+            long long sum = r0 + lane < c.rows ? row_steps(c, r0 + lane) : 0;
+#pragma unroll
+            for (int o = 1; o < 64; o *= 2) {
+                const long long y = __shfl_up(sum, o);
+                if (lane >= o) sum += y;
+            }
+            const unsigned long long past = __ballot((before + sum) * c.kv_heads > at);
+            if (past) {
+                const int first = __ffsll(past) - 1;
+                r = r0 + first;
+                before += first ? __shfl(sum, first - 1) : 0;
+                break;
+            }
+            before += __shfl(sum, 63);
+        }
+        const long long in = at - before * c.kv_heads;
+        const int n = row_steps(c, r);
+        h = (int)(in / n);
+        step = (int)(in - (long long)h * n);
+        // (the same in every lane: kept in scalar registers)
+        r = __builtin_amdgcn_readfirstlane(r);
+        h = __builtin_amdgcn_readfirstlane(h);
+        step = __builtin_amdgcn_readfirstlane(step);
+    }
+
+    for (;;) {  // one piece of the share: slots of one row and head
+    const int len = row_length(c, r), steps = (len + kStep - 1) / kStep, rh = r * c.kv_heads + h;
+    const int n_steps = JOINT ? steps : (int)min(left, (long long)(steps - step));
+    const int begin = step * kStep, end = min((step + n_steps) * kStep, len);
+    const bool whole = n_steps == steps;
 
     bf16x8 qf[NM][S][NP];
     int vis[NM];
@@ -314,6 +384,8 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
         for (int s = 0; s < S; ++s) {
             float y[8] = {};
             if (in) load_n<8, T>((const T*)a.q + r * a.qrs + t * a.qts + (long long)(h * a.group + g) * a.qhs + D / 4 * kq + 8 * s, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] *= a.q_sign;
             pieces8<NP>(y, qf[nm][s]);
         }
     }
@@ -330,26 +402,54 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
     }
 
     const size_t base = (size_t)rh * c.capacity;
-    for (int t0 = begin + 32 * wave; t0 < end; t0 += 128) {
-        // tile rows (2 x 16): row m of half f is token t0 + 8 (m / 4) + 4 f + m % 4
-        unsigned kw[2][KW], vw[VW];
-        float ks[2];
-        unsigned vs[2 * G];  // the scale bytes of the lane's eight tokens: [token][group]
+    // 32 tokens at a time go from memory to this wave's own ring in LDS, without passing registers: two tiles are on their way
+    // while one is computed (the memory's latency is longer than a tile's work), and no wave waits for another.
+    const unsigned ring = (unsigned)(unsigned long)(__attribute__((address_space(3))) char*)lds + wave * (RING * BYTES);
+    const unsigned char* sc_at = (lane < 8 * G ? c.key_scales : c.value_scales - 32 * G) + base * G + lane * 4;  // keys' scales, then the values'
+    auto fetch = [&](int t0, int slot) {
+        const unsigned to = ring + slot * BYTES;
+        const unsigned long long k = reinterpret_cast<unsigned long long>(c.keys + (base + t0) * (D / 2));
+        const unsigned long long v = reinterpret_cast<unsigned long long>(c.values + (base + t0) * (D / 2));
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+            lds_dma16(to + i * 1024, lane * 16, k + i * 1024);
+            lds_dma16(to + 16 * D + i * 1024, lane * 16, v + i * 1024);
+        }
+        if (lane < 16 * G)
+            __builtin_amdgcn_global_load_lds((gbl_ptr_t)(sc_at + t0 * G), (lds_ptr_t)(__attribute__((address_space(3))) char*)(unsigned long)(to + 32 * D), 4, 0, 0);
+    };
+    int t0 = begin + (JOINT ? 32 * wave : 0);
+#pragma unroll
+    for (int i = 0; i < RING - 1; ++i)
+        if (t0 + i * STRIDE < end) fetch(t0 + i * STRIDE, i);
+    for (int slot = 0; t0 < end; t0 += STRIDE, slot = slot == RING - 1 ? 0 : slot + 1) {
+        // (the slot that the tile before used is free once its values have been read)
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (t0 + (RING - 1) * STRIDE < end) {
+            fetch(t0 + (RING - 1) * STRIDE, slot == 0 ? RING - 1 : slot - 1);
+            wait_vmcnt_imm<(RING - 1) * LOADS>();
+        } else if (RING == 3 && t0 + STRIDE < end)
+            wait_vmcnt_imm<LOADS>();
+        else
+            wait_vmcnt_imm<0>();
+        Tile<D> w;
+        const char* at = lds + (wave * RING + slot) * BYTES;
+        const int tok = 8 * (l15 >> 2) + (l15 & 3);  // tile rows (2 x 16): row m of half f is token 8 (m / 4) + 4 f + m % 4
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
-            const size_t tok = base + t0 + 8 * (l15 >> 2) + (l15 & 3) + 4 * f;
-            const unsigned* p = reinterpret_cast<const unsigned*>(c.keys + tok * (D / 2) + kq * (D / 8));
+            const unsigned* p = reinterpret_cast<const unsigned*>(at + (tok + 4 * f) * (D / 2) + kq * (D / 8));
 #pragma unroll
-            for (int i = 0; i < KW; ++i) kw[f][i] = p[i];
-            ks[f] = byte_scale(c.key_scales[tok * G + kq * G / 4]);
+            for (int i = 0; i < KW; ++i) w.k[f][i] = p[i];
+            w.ks[f] = at[32 * D + (tok + 4 * f) * G + kq * G / 4];
         }
         {
-            const unsigned* p = reinterpret_cast<const unsigned*>(c.values + ((base + t0) / 8 + kq) * (size_t)(4 * D)) + l15 * VW;
+            const unsigned* p = reinterpret_cast<const unsigned*>(at + 16 * D + kq * (4 * D) + l15 * (D / 4));
 #pragma unroll
-            for (int i = 0; i < VW; ++i) vw[i] = p[i];
-            const unsigned* ps = reinterpret_cast<const unsigned*>(c.value_scales + (base + t0 + 8 * kq) * G);
+            for (int i = 0; i < VW; ++i) w.v[i] = p[i];
+            const unsigned* ps = reinterpret_cast<const unsigned*>(at + 32 * D + 32 * G + kq * (8 * G));
 #pragma unroll
-            for (int i = 0; i < 2 * G; ++i) vs[i] = ps[i];
+            for (int i = 0; i < 2 * G; ++i) w.vs[i] = ps[i];
+            w.look = ps[l15 % (2 * G)];
         }
         f32x4 sc[NM][2];
 #pragma unroll
@@ -358,35 +458,42 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
             for (int nm = 0; nm < NM; ++nm) sc[nm][f] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                const bf16x8 kf = widen8(kw[f][s], ks[f]);
+                const bf16x8 kf = widen8(w.k[f][s], byte_scale(w.ks[f]));
 #pragma unroll
                 for (int nm = 0; nm < NM; ++nm)
 #pragma unroll
                     for (int p = NP - 1; p >= 0; --p) sc[nm][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[nm][s][p], sc[nm][f], 0, 0, 0);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
         const bool masked = t0 + 32 > all_see;
+        if (masked) {
+#pragma unroll
+            for (int nm = 0; nm < NM; ++nm)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (t0 + 8 * kq + j >= vis[nm]) sc[nm][j >> 2][j & 3] = -INFINITY;
+        }
         float p[NM][8];
 #pragma unroll
         for (int nm = 0; nm < NM; ++nm) {
             float top = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                p[nm][j] = sc[nm][j >> 2][j & 3] * a.scale2;
-                if (masked && t0 + 8 * kq + j >= vis[nm]) p[nm][j] = -INFINITY;
-                top = fmaxf(top, p[nm][j]);
-            }
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, sc[nm][j >> 2][j & 3]);
             if constexpr (COUNT) {
                 const int m = (mg * NM + nm) * 16 + l15;
                 if (m < a.m_rows) {
-                    float* w = a.scores + ((size_t)rh * a.m_rows + m) * c.capacity + t0 + 8 * kq;
-                    *reinterpret_cast<f32x4*>(w) = f32x4{p[nm][0], p[nm][1], p[nm][2], p[nm][3]};
-                    *reinterpret_cast<f32x4*>(w + 4) = f32x4{p[nm][4], p[nm][5], p[nm][6], p[nm][7]};
+                    float* to = a.scores + ((size_t)rh * a.m_rows + m) * c.capacity + t0 + 8 * kq;
+                    *reinterpret_cast<f32x4*>(to) = sc[nm][0] * a.scale2;
+                    *reinterpret_cast<f32x4*>(to + 4) = sc[nm][1] * a.scale2;
                 }
             }
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            if (__any(top > mx[nm])) {
+            // The maximum moves only when a score outgrows it by 2^2, so that most tiles need no exchange between lanes: a
+            // probability of up to 4 is as exact (and still has an exponent to spare for every scale byte, below).
+            top *= a.scale2;
+            if (__any(top > mx[nm] + 2.f)) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
                 const float now = fmaxf(mx[nm], top), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[nm] - now);
                 mx[nm] = now;
                 l[nm] *= f;
@@ -396,143 +503,243 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
             const float off = mx[nm] == -INFINITY ? 0.f : mx[nm];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                p[nm][j] = __builtin_amdgcn_exp2f(p[nm][j] - off);
+                p[nm][j] = __builtin_amdgcn_exp2f(fmaf(sc[nm][j >> 2][j & 3], a.scale2, -off));
                 l[nm] += p[nm][j];
             }
         }
+        // P times the scale of its token and group, as bf16 pieces.  The scale is a power of two: its exponent is added to the
+        // probability's as an integer, two tokens at a time -- one v_perm_b32 for both bytes, one v_pk_mad_u16, and a maximum
+        // with 0 for what falls below bf16's exponents (products below 2^-126 vanish; p = 0 counts as 2^-127): a third of the
+        // instructions of extracting eight scales per group and multiplying.  Pieces are cut off, not rounded, so that none is
+        // negative; a single one is rounded.
+        u16x2 bits[NM][NP][4];
+#pragma unroll
+        for (int nm = 0; nm < NM; ++nm)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float x0 = p[nm][2 * i], x1 = p[nm][2 * i + 1];
+#pragma unroll
+                for (int q = 0; q < NP; ++q) {
+                    unsigned u;
+                    if constexpr (NP == 1)
+                        u = __builtin_bit_cast(unsigned, bf16x2{(__bf16)x0, (__bf16)x1});
+                    else
+                        u = __builtin_amdgcn_perm(__float_as_uint(x1), __float_as_uint(x0), 0x07060302u);
+                    x0 -= __uint_as_float(u << 16);
+                    x1 -= __uint_as_float(u & 0xFFFF0000u);
+                    bits[nm][q][i] = __builtin_bit_cast(u16x2, u) - (unsigned short)(127 << 7);
+                }
+            }
+        const bool special = masked || __any((w.look & 0x7F7F7F7Fu) + 0x01010101u & w.look & 0x80808080u);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            bf16x8 pf[NM][NP];
+            u32x4 pf[NM][NP];
+            if (special) {
+                // (a slot that is not seen, or a NaN group: what a masked slot holds must not reach the sum, 0 x NaN would)
 #pragma unroll
-            for (int nm = 0; nm < NM; ++nm) {
-                float y[8];
+                for (int nm = 0; nm < NM; ++nm) {
+                    float y[8];
+                    bf16x8 z[NP];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int byte = j * G + g;
-                    y[j] = p[nm][j] * byte_scale(vs[byte >> 2] >> 8 * (byte & 3) & 255u);
-                    // (a masked slot may hold anything, a NaN group included: 0 x NaN must not reach the sum)
-                    if (masked && t0 + 8 * kq + j >= vis[nm]) y[j] = 0.f;
+                    for (int j = 0; j < 8; ++j) {
+                        const int byte = j * G + g;
+                        y[j] = t0 + 8 * kq + j >= vis[nm] ? 0.f : p[nm][j] * byte_scale(w.vs[byte >> 2] >> 8 * (byte & 3) & 255u);
+                    }
+                    pieces8<NP>(y, z);
+#pragma unroll
+                    for (int q = 0; q < NP; ++q) pf[nm][q] = __builtin_bit_cast(u32x4, z[q]);
                 }
-                pieces8<NP>(y, pf[nm]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const unsigned b = G == 4 ? __builtin_amdgcn_perm(w.vs[2 * i + 1], w.vs[2 * i], 0x0C040C00u + 0x00010001u * g)
+                                              : __builtin_amdgcn_perm(0u, w.vs[i], 0x0C020C00u + 0x00010001u * g);
+#pragma unroll
+                    for (int nm = 0; nm < NM; ++nm)
+#pragma unroll
+                        for (int q = 0; q < NP; ++q) {
+                            s16x2 x;  // (the compiler takes a product by 128 apart into a shift and a sum)
+                            asm("v_pk_mad_u16 %0, %1, %2, %3" : "=v"(x) : "v"(b), "s"(0x00800080u), "v"(bits[nm][q][i]));
+                            pf[nm][q][i] = __builtin_bit_cast(unsigned, __builtin_elementwise_max(x, s16x2{0, 0}));
+                        }
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const bf16x8 vf = widen8(vw[2 * g + i], 1.f);
+                const bf16x8 vf = widen8(w.v[2 * g + i], 1.f);
 #pragma unroll
                 for (int nm = 0; nm < NM; ++nm)
 #pragma unroll
-                    for (int q = NP - 1; q >= 0; --q) o[nm][2 * g + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[nm][q], o[nm][2 * g + i], 0, 0, 0);
+                    for (int q = NP - 1; q >= 0; --q)
+                        o[nm][2 * g + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8, pf[nm][q]), o[nm][2 * g + i], 0, 0, 0);
             }
         }
     }
 
-    // the four waves' shares -> one
 #pragma unroll
     for (int nm = 0; nm < NM; ++nm) {
         l[nm] += __shfl_xor(l[nm], 16);
         l[nm] += __shfl_xor(l[nm], 32);
-        if (kq == 0) {
-            sm[wave][nm * 16 + l15] = mx[nm];
-            sl[wave][nm * 16 + l15] = l[nm];
-        }
     }
+    if constexpr (JOINT) {  // the four waves' shares -> one
+        __shared__ float sm[4][NM * 16], sl[4][NM * 16];
+        float(*so)[16][D + 4] = reinterpret_cast<float(*)[16][D + 4]>(lds);
 #pragma unroll
-    for (int nm = 0; nm < NM; ++nm) {
-        __syncthreads();
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) so[wave][l15][32 * g + 8 * kq + e] = o[nm][2 * g + (e & 1)][e >> 1];
-        __syncthreads();
-        constexpr int W = D / 16;
-        const int row = threadIdx.x >> 4, d = (threadIdx.x & 15) * W, m = (mg * NM + nm) * 16 + row;
-        if (m < a.m_rows) {
-            float top = -INFINITY, sum = 0.f, acc[W] = {};
-            for (int w = 0; w < 4; ++w) top = fmaxf(top, sm[w][nm * 16 + row]);
-            for (int w = 0; w < 4; ++w) {
-                const float mw = sm[w][nm * 16 + row];
-                const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - top);
-                // (a wave without a visible slot has sum 0; one whose scores were all NaN keeps its NaN: NaN x 0)
-                sum += sl[w][nm * 16 + row] * f;
-#pragma unroll
-                for (int i = 0; i < W; ++i) acc[i] += so[w][row][d + i] * f;
+        for (int nm = 0; nm < NM; ++nm)
+            if (kq == 0) {
+                sm[wave][nm * 16 + l15] = mx[nm];
+                sl[wave][nm * 16 + l15] = l[nm];
             }
-            if (a.splits == 1) {
+#pragma unroll
+        for (int nm = 0; nm < NM; ++nm) {
+            __syncthreads();
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) so[wave][l15][32 * g + 8 * kq + e] = o[nm][2 * g + (e & 1)][e >> 1];
+            __syncthreads();
+            constexpr int W = D / 16;
+            const int row = threadIdx.x >> 4, d = (threadIdx.x & 15) * W, m = (mg * NM + nm) * 16 + row;
+            if (m < a.m_rows) {
+                float top = -INFINITY, sum = 0.f, acc[W] = {};
+                for (int w = 0; w < 4; ++w) top = fmaxf(top, sm[w][nm * 16 + row]);
+                for (int w = 0; w < 4; ++w) {
+                    const float mw = sm[w][nm * 16 + row];
+                    const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - top);
+                    // (a wave without a visible slot has sum 0; one whose scores were all NaN keeps its NaN: NaN x 0)
+                    sum += sl[w][nm * 16 + row] * f;
+#pragma unroll
+                    for (int i = 0; i < W; ++i) acc[i] += so[w][row][d + i] * f;
+                }
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
                 for (int i = 0; i < W; ++i) acc[i] *= inv;
                 const int t = m / a.group, g = m - t * a.group;
                 store_n<W, T>((T*)a.out + (((size_t)r * a.tokens + t) * a.heads + h * a.group + g) * D + d, acc);
-            } else {
-                float* po = a.part_o + (((size_t)rh * a.splits + split) * a.m_rows + m) * D + d;
-                store_n<W, float>(po, acc);
+                if (COUNT && (threadIdx.x & 15) == 0) a.part_ml[(size_t)rh * a.m_rows + m] = f32x2{top, sum};
             }
-            if ((a.splits > 1 || COUNT) && (threadIdx.x & 15) == 0) a.part_ml[((size_t)rh * a.splits + split) * a.m_rows + m] = f32x2{top, sum};
+        }
+        return;
+    } else {
+        const size_t piece = (size_t)worker + rh;
+        if (mg == 0 && lane == 0) {
+            if (step == 0) a.ends[rh].x = (int)piece;
+            if (step + n_steps == steps) a.ends[rh].y = (int)piece;
+        }
+#pragma unroll
+        for (int nm = 0; nm < NM; ++nm) {
+            const int m = (mg * NM + nm) * 16 + l15;
+            if (m < a.m_rows) {
+                if ((!whole || COUNT) && kq == 0) a.part_ml[piece * a.m_rows + m] = f32x2{mx[nm], l[nm]};
+                const float inv = l[nm] == 0.f ? 0.f : 1.f / l[nm];
+                const int t = m / a.group, g0 = m - t * a.group;
+                T* out = (T*)a.out + (((size_t)r * a.tokens + t) * a.heads + h * a.group + g0) * D + 8 * kq;
+                float* part = a.part_o + (piece * a.m_rows + m) * D + 8 * kq;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = o[nm][2 * g + (e & 1)][e >> 1] * (whole ? inv : 1.f);
+                    if (whole)
+                        store_n<8, T>(out + 32 * g, y);
+                    else
+                        store_n<8, float>(part + 32 * g, y);
+                }
+            }
+        }
+        left -= n_steps;
+        if (left <= 0) return;
+        step = 0;
+        if (++h == c.kv_heads) {
+            h = 0;
+            do ++r;  // (ends: work is left, so a later row holds it)
+            while (row_length(c, r) == 0);
         }
     }
-}
-
-// (largest score, sum of exponentials to it) of a query over all splits of its row
-__device__ __forceinline__ f32x2 join_ml(const AttendArgs& a, int rh, int m, int used) {
-    const f32x2* p = a.part_ml + (size_t)rh * a.splits * a.m_rows + m;
-    float top = -INFINITY, sum = 0.f;
-    for (int s = 0; s < used; ++s) top = fmaxf(top, p[(size_t)s * a.m_rows][0]);
-    for (int s = 0; s < used; ++s) {
-        const f32x2 ml = p[(size_t)s * a.m_rows];
-        sum += ml[1] * (ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - top));
     }
-    return f32x2{top, sum};
 }
 
-// The splits of a row -> the output (blocks below `merge_blocks`), and the probabilities that each slot received, from the
-// stored scores (the others: 1024 slots of one row and head each).
+// (largest score, sum of exponentials to it) of query m over the pieces of a row and head; the N lanes of a group share them
+template <int N>
+__device__ __forceinline__ f32x2 join_ml(const AttendArgs& a, int2 p, int m) {
+    const f32x2* ml = a.part_ml + m;
+    float top = -INFINITY, sum = 0.f;
+    for (int s = p.x + (int)(threadIdx.x % N); s <= p.y; s += N) {
+        const f32x2 x = ml[(size_t)s * a.m_rows];
+        const float now = fmaxf(top, x[0]);
+        sum = (now == top ? sum : sum * __builtin_amdgcn_exp2f(top - now)) + x[1] * (x[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[0] - now));
+        top = now;
+    }
+    float all = top;
+#pragma unroll
+    for (int o = 1; o < N; o *= 2) all = fmaxf(all, __shfl_xor(all, o));
+    sum *= top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - all);  // (a sum without a maximum is 0 or NaN)
+#pragma unroll
+    for (int o = 1; o < N; o *= 2) sum += __shfl_xor(sum, o);
+    return f32x2{all, sum};
+}
+
+// The rows and heads that were cut into pieces -> the output, and zeros for empty rows.  One workgroup per row, head and query: a
+// long row is cut into up to all workers, so 16 groups of 16 lanes share its pieces.
 template <int TYPE, int D>
-__global__ __launch_bounds__(256) void kv4_join_kernel(AttendArgs a, int merge_blocks, int slot_blocks, float decay) {
+__global__ __launch_bounds__(256) void kv4_join_kernel(AttendArgs a) {
     using T = typename Elem<TYPE>::T;
+    constexpr int W = D / 16;
+    __shared__ float part[16][D];
     const after_kv4& c = a.c;
-    if ((int)blockIdx.x < merge_blocks) {
-        constexpr int W = D / 16;
-        const long long item = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);  // (row, head, query)
-        const int d = (threadIdx.x & 15) * W;
-        if (item >= (long long)c.rows * c.kv_heads * a.m_rows) return;
-        const int rh = (int)(item / a.m_rows), m = (int)(item % a.m_rows), r = rh / c.kv_heads, h = rh % c.kv_heads;
-        const int len = row_length(c, r), chunk = split_chunk(len, a.splits), used = len ? (len + chunk - 1) / chunk : 0;
-        const f32x2 all = join_ml(a, rh, m, used);
+    const int rh = blockIdx.x / a.m_rows, m = blockIdx.x % a.m_rows, r = rh / c.kv_heads, h = rh % c.kv_heads;
+    const int group = threadIdx.x >> 4, d = (threadIdx.x & 15) * W;
+    const int2 p = a.ends[rh];  // (an empty row has none: not looked at)
+    float acc[W] = {};
+    if (row_length(c, r) > 0) {
+        if (p.x == p.y) return;  // (whole: written already)
+        const f32x2 all = join_ml<64>(a, p, m);
         const float inv = all[1] == 0.f ? 0.f : 1.f / all[1];
-        float acc[W] = {};
-        for (int s = 0; s < used; ++s) {
-            const size_t at = ((size_t)rh * a.splits + s) * a.m_rows + m;
-            const float ms = a.part_ml[at][0], f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - all[0]);
+#pragma unroll 4
+        for (int s = p.x + group; s <= p.y; s += 16) {
+            const size_t at = (size_t)s * a.m_rows + m;
+            const float ms = a.part_ml[at][0], f = (ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - all[0])) * inv;
             float x[W];
             load_n<W, float>(a.part_o + at * D + d, x);
 #pragma unroll
             for (int i = 0; i < W; ++i) acc[i] += x[i] * f;
         }
-#pragma unroll
-        for (int i = 0; i < W; ++i) acc[i] *= inv;
-        const int t = m / a.group, g = m - t * a.group;
-        store_n<W, T>((T*)a.out + (((size_t)r * a.tokens + t) * a.heads + h * a.group + g) * D + d, acc);
-        return;
     }
-    const int b = blockIdx.x - merge_blocks, rh = b / slot_blocks, r = rh / c.kv_heads;
-    const int len = row_length(c, r), s0 = (b % slot_blocks) * 1024;
+    store_n<W, float>(&part[group][d], acc);
+    __syncthreads();
+    if (threadIdx.x < D) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += part[i][threadIdx.x];
+        const int t = m / a.group, g = m - t * a.group;
+        ((T*)a.out)[(((size_t)r * a.tokens + t) * a.heads + h * a.group + g) * D + threadIdx.x] = (T)sum;
+    }
+}
+
+// The probabilities that each slot received, from the stored scores: 1024 slots of one row and head.
+__global__ __launch_bounds__(256) void kv4_weights_kernel(AttendArgs a, int slot_blocks, float decay) {
+    const after_kv4& c = a.c;
+    const int rh = blockIdx.x / slot_blocks, r = rh / c.kv_heads;
+    const int len = row_length(c, r), s0 = (blockIdx.x % slot_blocks) * 1024;
     if (s0 >= len) return;
-    const int chunk = split_chunk(len, a.splits), used = (len + chunk - 1) / chunk;
+    const int2 p = a.workers ? a.ends[rh] : int2{rh, rh};
     const int s = s0 + 4 * threadIdx.x;
-    __shared__ f32x2 ml[256];
+    __shared__ f32x2 ml[32];
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (int m0 = 0; m0 < a.m_rows; m0 += 256) {
-        const int n = min(256, a.m_rows - m0);
+    for (int m0 = 0; m0 < a.m_rows; m0 += 32) {
+        const int n = min(32, a.m_rows - m0), mine = threadIdx.x >> 3;
         __syncthreads();
-        if ((int)threadIdx.x < n) {
-            const f32x2 all = join_ml(a, rh, m0 + threadIdx.x, used);
-            ml[threadIdx.x] = f32x2{all[0] == -INFINITY ? 0.f : all[0], all[1] == 0.f ? 0.f : 1.f / all[1]};
+        if (mine < n) {
+            const f32x2 all = join_ml<8>(a, p, m0 + mine);
+            if ((threadIdx.x & 7) == 0) ml[mine] = f32x2{all[0] == -INFINITY ? 0.f : all[0], all[1] == 0.f ? 0.f : 1.f / all[1]};
         }
         __syncthreads();
         if (s < len) {
-            const float* p = a.scores + ((size_t)rh * a.m_rows + m0) * c.capacity + s;
+            const float* x4 = a.scores + ((size_t)rh * a.m_rows + m0) * c.capacity + s;
+#pragma unroll 4
             for (int m = 0; m < n; ++m) {
-                const f32x4 x = *reinterpret_cast<const f32x4*>(p + (size_t)m * c.capacity);
+                const f32x4 x = *reinterpret_cast<const f32x4*>(x4 + (size_t)m * c.capacity);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum[i] += x[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[i] - ml[m][0]) * ml[m][1];
             }
@@ -709,50 +916,56 @@ bool known_type(int t) { return t == AFTER_T_F32 || t == AFTER_T_BF16 || t == AF
 int type_bytes(int t) { return t == AFTER_T_F32 ? 4 : 2; }
 bool aligned16(const void* p) { return ((size_t)p & 15) == 0; }
 
-// Splits of a row: enough workgroups for the chip, none shorter than 256 slots at full length
-int attend_splits(const after_kv4& c, int mgroups) {
-    const long long units = (long long)c.rows * c.kv_heads * mgroups;
-    const long long wanted = (2048 + units - 1) / units, most = (c.capacity + 255) / 256;
-    return (int)(wanted < most ? wanted : most);
-}
-int attend_nm(int m_rows) { return m_rows > 16 ? 2 : 1; }
-
 struct Plan {
-    int m_rows, nm, mgroups, splits;
-    long long o_bytes, ml_bytes, s_bytes;
+    int m_rows, nm, mgroups, wgs;  // wgs: workgroups of four workers, or 0
+    long long pieces, o_bytes, ml_bytes, s_bytes, e_bytes;
 };
-Plan attend_plan(const after_kv4& c, int heads, int tokens, bool count) {
+Plan attend_plan(const after_kv4& c, int type, int heads, int tokens, bool count) {
     Plan p;
     p.m_rows = tokens * (heads / c.kv_heads);
-    p.nm = attend_nm(p.m_rows);
+    p.nm = p.m_rows > 16 ? 2 : 1;
     p.mgroups = cdiv(p.m_rows, 16 * p.nm);
-    p.splits = attend_splits(c, p.mgroups);
-    const long long n = (long long)c.rows * c.kv_heads * p.m_rows;
-    p.o_bytes = p.splits > 1 ? n * p.splits * c.head_dim * 4 : 0;
-    p.ml_bytes = p.splits > 1 || count ? (n * p.splits * 8 + 255) / 256 * 256 : 0;
-    p.s_bytes = count ? n * c.capacity * 4 : 0;
+    const long long n_rh = (long long)c.rows * c.kv_heads, most = cdivll(n_rh * (c.capacity / kStep), 4);
+    // As many workers as the chip holds at once: three workgroups on each of 256 CUs with bf16 queries, two with the others (more
+    // registers).  64 rows of 1 .. 8192, bf16: 60 us, and 64 with two; two rows of 131071, fp16: 59 us, and 69 with three.
+    // Rows of at most 512 slots take a workgroup each and one launch: 5.5 us against 8.5.
+    const int full = type == AFTER_T_BF16 ? 768 : 512;
+    p.wgs = c.capacity <= 512 ? 0 : (int)(most < full ? most : full);
+    p.pieces = 4ll * p.wgs + n_rh;
+    p.o_bytes = p.wgs ? p.pieces * p.m_rows * c.head_dim * 4 : 0;
+    p.ml_bytes = p.wgs || count ? (p.pieces * p.m_rows * 8 + 255) / 256 * 256 : 0;
+    p.s_bytes = count ? n_rh * p.m_rows * c.capacity * 4 : 0;
+    p.e_bytes = p.wgs ? (n_rh * 8 + 255) / 256 * 256 : 0;
     return p;
+}
+
+template <int TYPE, int D, int NM, bool COUNT>
+void launch_attend(const AttendArgs& a, const Plan& p, hipStream_t s) {
+    constexpr size_t ring = 4 * kRing * kTileBytes<D>, out = 4 * 16 * (D + 4) * 4;  // (at most 53 KB: three workgroups a CU)
+    if (p.wgs)
+        hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, NM, COUNT, false>), dim3(p.wgs, p.mgroups), dim3(256), ring, s, a);
+    else
+        hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, NM, COUNT, true>), dim3(a.c.rows * a.c.kv_heads, p.mgroups), dim3(256), ring > out ? ring : out, s, a);
 }
 
 template <int TYPE, int D>
 int run_attend(const AttendArgs& a, const Plan& p, bool count, float decay, hipStream_t s) {
-    const long long units = cdivll((long long)a.c.rows * a.c.kv_heads * a.splits, 8) * 8 * a.mgroups;
-    const dim3 grid((unsigned)units), block(256);
     if (p.nm == 1) {
         if (count)
-            hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, 1, true>), grid, block, 0, s, a);
+            launch_attend<TYPE, D, 1, true>(a, p, s);
         else
-            hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, 1, false>), grid, block, 0, s, a);
+            launch_attend<TYPE, D, 1, false>(a, p, s);
     } else {
         if (count)
-            hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, 2, true>), grid, block, 0, s, a);
+            launch_attend<TYPE, D, 2, true>(a, p, s);
         else
-            hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, 2, false>), grid, block, 0, s, a);
+            launch_attend<TYPE, D, 2, false>(a, p, s);
     }
-    if (a.splits > 1 || count) {
-        const int merge = a.splits > 1 ? (int)cdivll((long long)a.c.rows * a.c.kv_heads * a.m_rows, 16) : 0;
-        const int slots = cdiv(a.c.capacity, 1024), more = count ? a.c.rows * a.c.kv_heads * slots : 0;
-        hipLaunchKernelGGL((kv4_join_kernel<TYPE, D>), dim3(merge + more), block, 0, s, a, merge, slots, decay);
+    if (p.wgs)
+        hipLaunchKernelGGL((kv4_join_kernel<TYPE, D>), dim3(a.c.rows * a.c.kv_heads * a.m_rows), dim3(256), 0, s, a);
+    if (count) {
+        const int slots = cdiv(a.c.capacity, 1024);
+        hipLaunchKernelGGL(kv4_weights_kernel, dim3(a.c.rows * a.c.kv_heads * slots), dim3(256), 0, s, a, slots, decay);
     }
     AFTER_HIP_CHECK(hipGetLastError());
     return AFTER_OK;
@@ -831,36 +1044,37 @@ extern "C" int after_kv4_read(const after_kv4* c, void* k, void* v, int type, co
     return AFTER_OK;
 }
 
-static int check_attend(const after_kv4* c, int heads, int tokens, const char* what) {
+static int check_attend(const after_kv4* c, int type, int heads, int tokens, const char* what) {
     AFTER_TRY(check_cache(c, what));
+    AFTER_REQUIRE(known_type(type), AFTER_E_INVALID, "%s: unknown element type %d", what, type);
     AFTER_REQUIRE(heads > 0 && heads % c->kv_heads == 0, AFTER_E_INVALID, "%s: heads must be a multiple of the cache's %d", what, c->kv_heads);
     AFTER_REQUIRE(tokens > 0 && (long long)tokens * (heads / c->kv_heads) <= 65536, AFTER_E_INVALID, "%s: 1 .. 65536 / (heads / kv_heads) tokens (got %d)",
                   what, tokens);
-    const Plan p = attend_plan(*c, heads, tokens, false);
-    AFTER_REQUIRE((long long)c->rows * c->kv_heads * p.splits * p.mgroups < (1ll << 30), AFTER_E_INVALID, "%s: too many rows x heads x tokens for one call", what);
+    const Plan p = attend_plan(*c, type, heads, tokens, false);
+    AFTER_REQUIRE(p.mgroups < 65536 && p.pieces < (1ll << 31) && (long long)c->rows * c->kv_heads * p.m_rows < (1ll << 31) && (long long)c->rows * c->kv_heads * cdiv(c->capacity, 1024) < (1ll << 31),
+                  AFTER_E_INVALID, "%s: too many rows x heads x tokens for one call", what);
     return AFTER_OK;
 }
 
-extern "C" int after_kv4_attend_workspace(const after_kv4* c, int heads, int tokens, int accumulate, long long* bytes) {
-    AFTER_TRY(check_attend(c, heads, tokens, "kv4_attend_workspace"));
+extern "C" int after_kv4_attend_workspace(const after_kv4* c, int type, int heads, int tokens, int accumulate, long long* bytes) {
+    AFTER_TRY(check_attend(c, type, heads, tokens, "kv4_attend_workspace"));
     AFTER_REQUIRE(bytes, AFTER_E_INVALID, "kv4_attend_workspace: bytes is NULL");
-    const Plan p = attend_plan(*c, heads, tokens, accumulate != 0);
-    *bytes = p.o_bytes + p.ml_bytes + p.s_bytes;
+    const Plan p = attend_plan(*c, type, heads, tokens, accumulate != 0);
+    *bytes = p.o_bytes + p.ml_bytes + p.s_bytes + p.e_bytes;
     return AFTER_OK;
 }
 
 extern "C" int after_kv4_attend(const after_kv4* c, const void* q, void* out, int type, int heads, int tokens, long long q_row_stride,
                                 long long q_token_stride, long long q_head_stride, float scale, int accumulate, float decay, void* workspace,
                                 long long workspace_bytes, void* stream) {
-    AFTER_TRY(check_attend(c, heads, tokens, "kv4_attend"));
-    AFTER_REQUIRE(known_type(type), AFTER_E_INVALID, "kv4_attend: unknown element type %d", type);
+    AFTER_TRY(check_attend(c, type, heads, tokens, "kv4_attend"));
     const int per16 = 16 / type_bytes(type);
     AFTER_REQUIRE(q && out && aligned16(q) && aligned16(out) && q_row_stride % per16 == 0 && q_token_stride % per16 == 0 && q_head_stride % per16 == 0,
                   AFTER_E_INVALID, "kv4_attend: q, its strides and out must be 16-byte aligned");
     AFTER_REQUIRE(std::isfinite(scale) && std::isfinite(decay), AFTER_E_INVALID, "kv4_attend: scale and decay must be finite");
     const bool count = accumulate != 0;
-    const Plan p = attend_plan(*c, heads, tokens, count);
-    const long long need = p.o_bytes + p.ml_bytes + p.s_bytes;
+    const Plan p = attend_plan(*c, type, heads, tokens, count);
+    const long long need = p.o_bytes + p.ml_bytes + p.s_bytes + p.e_bytes;
     AFTER_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need), AFTER_E_CAPACITY,
                   "kv4_attend: needs a 16-byte aligned workspace of %lld bytes (got %lld)", need, workspace_bytes);
     AttendArgs a;
@@ -874,13 +1088,14 @@ extern "C" int after_kv4_attend(const after_kv4* c, const void* q, void* out, in
     a.tokens = tokens;
     a.group = heads / c->kv_heads;
     a.m_rows = p.m_rows;
-    a.splits = p.splits;
-    a.mgroups = p.mgroups;
-    a.scale2 = scale * 1.44269504088896340736f;
+    a.workers = 4 * p.wgs;
+    a.scale2 = std::fmax(std::fabs(scale) * 1.44269504088896340736f, 1e-30f);
+    a.q_sign = scale < 0 ? -1.f : 1.f;
     char* w = (char*)workspace;
     a.scores = count ? (float*)w : nullptr;
     a.part_ml = (f32x2*)(w + p.s_bytes);
-    a.part_o = (float*)(w + p.s_bytes + p.ml_bytes);
+    a.ends = (int2*)(w + p.s_bytes + p.ml_bytes);
+    a.part_o = (float*)(w + p.s_bytes + p.ml_bytes + p.e_bytes);
 #define CALL(T, D) return run_attend<T, D>(a, p, count, decay, (hipStream_t)stream)
     KV4_BY_TYPE(type, c->head_dim, CALL);
 #undef CALL

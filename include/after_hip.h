@@ -629,7 +629,7 @@ int after_kv4_read(const after_kv4* c, void* k, void* v, int type, const int* st
  * tokens than others has its queries at the end.)  accumulate: weights = decay * weights + the probabilities that each slot
  * in use received, summed over tokens and the group's heads (decay = 0: they are replaced).  The workspace is scratch: its
  * size depends on the arguments alone, and two calls that may run at the same time need two. */
-int after_kv4_attend_workspace(const after_kv4* c, int heads, int tokens, int accumulate, long long* bytes);
+int after_kv4_attend_workspace(const after_kv4* c, int type, int heads, int tokens, int accumulate, long long* bytes);
 int after_kv4_attend(const after_kv4* c, const void* q, void* out, int type, int heads, int tokens, long long q_row_stride,
                      long long q_token_stride, long long q_head_stride, float scale, int accumulate, float decay, void* workspace,
                      long long workspace_bytes, void* stream);

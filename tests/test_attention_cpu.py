@@ -54,7 +54,7 @@ def test_cache_refuses(bad):
     assert L.after_kv4_evict(c, ctypes.byref(cache()), 8, 0, P, None) == E_INVALID
     assert L.after_kv4_evict(ctypes.byref(cache()), c, 8, 0, P, None) == E_INVALID
     n = ctypes.c_longlong()
-    assert L.after_kv4_attend_workspace(c, 4, 1, 0, ctypes.byref(n)) == E_INVALID
+    assert L.after_kv4_attend_workspace(c, 1, 4, 1, 0, ctypes.byref(n)) == E_INVALID
     assert L.after_kv4_attend(c, P, P, 1, 4, 1, 256, 256, 64, 0.1, 0, 1.0, P, 1 << 40, None) == E_INVALID
 
 
@@ -80,9 +80,9 @@ def test_cache_calls_refuse():
 def test_attend_refuses():
     L, c, n = _lib.lib(), ctypes.byref(cache(capacity=4096)), ctypes.c_longlong()
     for heads, tokens in ((3, 1), (0, 1), (4, 0), (4, -1), (4, 32769)):
-        assert L.after_kv4_attend_workspace(c, heads, tokens, 0, ctypes.byref(n)) == E_INVALID
-    assert L.after_kv4_attend_workspace(c, 4, 1, 0, None) == E_INVALID
-    assert L.after_kv4_attend_workspace(c, 4, 1, 1, ctypes.byref(n)) == 0 and n.value >= 2 * 2 * 2 * 4096 * 4
+        assert L.after_kv4_attend_workspace(c, 1, heads, tokens, 0, ctypes.byref(n)) == E_INVALID
+    assert L.after_kv4_attend_workspace(c, 1, 4, 1, 0, None) == E_INVALID
+    assert L.after_kv4_attend_workspace(c, 1, 4, 1, 1, ctypes.byref(n)) == 0 and n.value >= 2 * 2 * 2 * 4096 * 4
     ok = (P, P, 1, 4, 1, 256, 256, 64, 0.1, 1, 1.0, P, n.value, None)
     for i, v, code in ((0, None, E_INVALID), (1, P + 8, E_INVALID), (2, 3, E_INVALID), (5, 4, E_INVALID), (7, 1, E_INVALID), (8, float("nan"), E_INVALID),
                        (10, float("inf"), E_INVALID), (11, None, E_CAPACITY), (12, n.value - 1, E_CAPACITY)):
