@@ -322,8 +322,6 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
     extern __shared__ __align__(16) char lds[];  // [4][RING][BYTES]; JOINT: then [4][16][D + 4] floats
     const after_kv4& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, kq = lane >> 4;
-    const int mg = blockIdx.y;
-
     // the first row and head of this worker's share, and where in it the share begins
     const int worker = blockIdx.x * 4 + wave;
     int r, h, step = 0;
@@ -377,7 +375,7 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
     int vis[NM];
 #pragma unroll
     for (int nm = 0; nm < NM; ++nm) {
-        const int m = (mg * NM + nm) * 16 + l15, t = m / a.group, g = m - t * a.group;
+        const int m = nm * 16 + l15, t = m / a.group, g = m - t * a.group;
         const bool in = m < a.m_rows;
         vis[nm] = in ? max(len - a.tokens + t + 1, 0) : 0;
 #pragma unroll
@@ -389,7 +387,7 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
             pieces8<NP>(y, qf[nm][s]);
         }
     }
-    const int all_see = len - a.tokens + mg * NM * 16 / a.group + 1;  // slots below this are seen by every query here
+    const int all_see = len - a.tokens + 1;  // slots below this are seen by every query
 
     f32x4 o[NM][2 * G];
     float mx[NM], l[NM];
@@ -481,7 +479,7 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = fmaxf(top, sc[nm][j >> 2][j & 3]);
             if constexpr (COUNT) {
-                const int m = (mg * NM + nm) * 16 + l15;
+                const int m = nm * 16 + l15;
                 if (m < a.m_rows) {
                     float* to = a.scores + ((size_t)rh * a.m_rows + m) * c.capacity + t0 + 8 * kq;
                     *reinterpret_cast<f32x4*>(to) = sc[nm][0] * a.scale2;
@@ -600,7 +598,7 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
                 for (int e = 0; e < 8; ++e) so[wave][l15][32 * g + 8 * kq + e] = o[nm][2 * g + (e & 1)][e >> 1];
             __syncthreads();
             constexpr int W = D / 16;
-            const int row = threadIdx.x >> 4, d = (threadIdx.x & 15) * W, m = (mg * NM + nm) * 16 + row;
+            const int row = threadIdx.x >> 4, d = (threadIdx.x & 15) * W, m = nm * 16 + row;
             if (m < a.m_rows) {
                 float top = -INFINITY, sum = 0.f, acc[W] = {};
                 for (int w = 0; w < 4; ++w) top = fmaxf(top, sm[w][nm * 16 + row]);
@@ -623,13 +621,13 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
         return;
     } else {
         const size_t piece = (size_t)worker + rh;
-        if (mg == 0 && lane == 0) {
+        if (lane == 0) {
             if (step == 0) a.ends[rh].x = (int)piece;
             if (step + n_steps == steps) a.ends[rh].y = (int)piece;
         }
 #pragma unroll
         for (int nm = 0; nm < NM; ++nm) {
-            const int m = (mg * NM + nm) * 16 + l15;
+            const int m = nm * 16 + l15;
             if (m < a.m_rows) {
                 if ((!whole || COUNT) && kq == 0) a.part_ml[piece * a.m_rows + m] = f32x2{mx[nm], l[nm]};
                 const float inv = l[nm] == 0.f ? 0.f : 1.f / l[nm];
@@ -657,6 +655,279 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
             while (row_length(c, r) == 0);
         }
     }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- many queries
+// More than 32 queries of a row that share a head (a chunk of a prompt, the last tokens that say what is worth keeping): 128 of
+// them per workgroup, 32 to a wave, over the same tiles of 64 tokens.  The tiles are widened to bf16 once for the four waves and
+// kept in LDS in the order in which the matrix instructions take them (a lane's operand is 16 bytes at its own number: no
+// conflicts); while one tile is multiplied the next one's codes are on their way in registers.
+constexpr int kWideRows = 128, kWideTile = 64;
+
+template <int D>
+struct Raw {  // a thread's share of a tile as it lies in memory
+    u32x4 k, v;
+    unsigned vs[D / 16];
+    unsigned char ks;
+};
+
+template <int D>
+struct Widen {
+    static constexpr int G = D / 32, USED = 2 * D;  // threads that hold a piece: 16 bytes of keys and 16 of values each
+    static constexpr int KEYS = kWideTile * D * 2;  // bytes of a widened tile's keys; as many of its values
+    const after_kv4& c;
+    size_t base;
+    int token, group;   // keys: one token's group of 32 channels
+    int block, quad;    // values: four channels of eight tokens
+    unsigned k_to, v_to;
+    __device__ __forceinline__ Widen(const after_kv4& cache, int rh) : c(cache), base((size_t)rh * cache.capacity) {
+        const int t = threadIdx.x % USED;
+        token = t / G;
+        group = t % G;
+        // operand of half f of the 32 tokens: row m is token 8 (m / 4) + 4 f + m % 4; lane 16 kq + m holds channels 32 s + 8 kq ..
+        k_to = ((((token >> 5) * 2 + (token >> 2 & 1)) * G + group) * 64 + ((token & 31) >> 3) * 4 + (token & 3)) * 16;
+        block = t / (D / 4);
+        quad = t % (D / 4);
+        const int l15 = D == 128 ? quad >> 1 : quad, g0 = D == 128 ? 2 * (quad & 1) : 0;
+        // operand (g, i): row l15 is channel 32 g + 2 l15 + i; lane 16 kq + l15 holds tokens 8 kq ..
+        v_to = KEYS + (((block >> 2) * 2 * G + 2 * g0) * 64 + (block & 3) * 16 + l15) * 16;
+    }
+    __device__ __forceinline__ bool mine() const { return USED == 256 || threadIdx.x < USED; }
+    // (a tile may reach past the last 32 slots that are in use: capacity is a multiple of 32)
+    __device__ __forceinline__ void load_keys(Raw<D>& w, int t0) const {
+        const size_t at = base + min(t0 + token, c.capacity - 1);
+        w.k = *reinterpret_cast<const u32x4*>(c.keys + at * (D / 2) + 16 * group);
+        w.ks = c.key_scales[at * G + group];
+    }
+    __device__ __forceinline__ void load_values(Raw<D>& w, int t0) const {
+        const size_t at = base + min(t0 + 8 * block, c.capacity - 8);
+        w.v = *reinterpret_cast<const u32x4*>(c.values + at / 8 * (4 * D) + 16 * quad);
+        const unsigned* ps = reinterpret_cast<const unsigned*>(c.value_scales + at * G);
+#pragma unroll
+        for (int i = 0; i < 2 * G; ++i) w.vs[i] = ps[i];
+    }
+    __device__ __forceinline__ void store_keys(const Raw<D>& w, char* lds) const {
+        const float sc = byte_scale(w.ks);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<bf16x8*>(lds + k_to + i * 256) = widen8(w.k[i], sc);
+    }
+    // A NaN group is left out, its token marked in bad[g]: the queries that see it get their NaN apart from the product, in which
+    // it would reach all of them.
+    __device__ __forceinline__ void store_values(const Raw<D>& w, char* lds, unsigned long long* bad) const {
+        const int g0 = D == 128 ? 2 * (quad & 1) : 0;
+#pragma unroll
+        for (int gg = 0; gg < 2; ++gg) {
+            float sc[8];
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int byte = j * G + g0 + gg;
+                const unsigned b = w.vs[G == 4 ? j : j >> 1] >> 8 * (byte & 3) & 255u;
+                any |= b == kBadByte;
+                sc[j] = byte_scale(b);
+            }
+            if (any) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (sc[j] == INFINITY) {
+                        atomicOr(&bad[g0 + gg], 1ull << (8 * block + j));
+                        sc[j] = 1.f;  // (its codes are zeros)
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const unsigned x = w.v[2 * gg + i];
+                auto pair = [&](bf16x2 lo, bf16x2 hi) { return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, hi), __builtin_bit_cast(unsigned, lo), 0x07060100u); };
+                u32x4 y;
+                y[0] = pair(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc[0], 0), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc[1], 0));
+                y[1] = pair(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc[2], 1), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc[3], 1));
+                y[2] = pair(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc[4], 2), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc[5], 2));
+                y[3] = pair(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc[6], 3), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc[7], 3));
+                *reinterpret_cast<u32x4*>(lds + v_to + (2 * gg + i) * 1024) = y;
+            }
+        }
+    }
+};
+
+// the wave's 32 queries as operands: qf[nm][s][piece], channels 32 s + 8 kq ..; vis: the slots that each sees
+template <int TYPE, int D, int NP>
+__device__ __forceinline__ void load_queries(const AttendArgs& a, int r, int h, int m0, int len, bf16x8 (&qf)[2][D / 32][NP], int (&vis)[2]) {
+    using T = typename Elem<TYPE>::T;
+    const int lane = threadIdx.x & 63, l15 = lane & 15, kq = lane >> 4;
+#pragma unroll
+    for (int nm = 0; nm < 2; ++nm) {
+        const int m = m0 + nm * 16 + l15, t = m / a.group, g = m - t * a.group;
+        const bool in = m < a.m_rows;
+        vis[nm] = in ? max(len - a.tokens + t + 1, 0) : 0;
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) {
+            float y[8] = {};
+            if (in) load_n<8, T>((const T*)a.q + r * a.qrs + t * a.qts + (long long)(h * a.group + g) * a.qhs + 32 * s + 8 * kq, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] *= a.q_sign;
+            pieces8<NP>(y, qf[nm][s]);
+        }
+    }
+}
+
+// scores of 32 tokens: sc[nm][f][i]: token 8 kq + 4 f + i
+template <int D, int NP>
+__device__ __forceinline__ void scores32(const char* keys, const bf16x8 (&qf)[2][D / 32][NP], f32x4 (&sc)[2][2]) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+        sc[0][f] = sc[1][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) {
+            const bf16x8 kf = *reinterpret_cast<const bf16x8*>(keys + ((f * (D / 32) + s) * 64 + lane) * 16);
+#pragma unroll
+            for (int nm = 0; nm < 2; ++nm)
+#pragma unroll
+                for (int p = NP - 1; p >= 0; --p) sc[nm][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[nm][s][p], sc[nm][f], 0, 0, 0);
+        }
+    }
+}
+
+// slots per split of a row: whole tiles
+__device__ __forceinline__ int wide_chunk(int len, int splits) { return ((len + splits - 1) / splits + kWideTile - 1) / kWideTile * kWideTile; }
+
+template <int TYPE, int D>
+__global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_kernel(AttendArgs a, int splits, int mgroups) {
+    using T = typename Elem<TYPE>::T;
+    constexpr int NP = TYPE == AFTER_T_BF16 ? 1 : TYPE == AFTER_T_F16 ? 2 : 3;
+    constexpr int G = D / 32, STAGE = 2 * Widen<D>::KEYS;
+    extern __shared__ __align__(16) char lds[];
+    __shared__ unsigned long long bad[3][G];
+    const after_kv4& c = a.c;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, kq = lane >> 4;
+    // (neighbours are dispatched to different XCDs: the workgroups that read one piece of the cache stand eight apart, on one L2)
+    const int x = blockIdx.x, mg = (x >> 3) % mgroups, unit = (x >> 3) / mgroups * 8 + (x & 7), n_rh = c.rows * c.kv_heads;
+    if (unit >= n_rh * splits) return;
+    const int rh = unit % n_rh, split = unit / n_rh, r = rh / c.kv_heads, h = rh % c.kv_heads;
+    const int len = row_length(c, r), chunk = wide_chunk(len, splits), used = len ? (len + chunk - 1) / chunk : 0;
+    if (split >= used) return;
+    if (mg == 0 && split == 0 && threadIdx.x == 0) a.ends[rh] = int2{rh * splits, rh * splits + used - 1};
+    const int m0 = mg * kWideRows + wave * 32;
+    const int begin = split * chunk, last_m = min((mg + 1) * kWideRows, a.m_rows) - 1;
+    const int end = min(begin + chunk, len - a.tokens + last_m / a.group + 1);  // (what the last query here sees)
+    const int all_see = len - a.tokens + m0 / a.group + 1;                      // every query of the wave sees the slots below
+
+    bf16x8 qf[2][G][NP];
+    int vis[2];
+    load_queries<TYPE, D, NP>(a, r, h, m0, len, qf, vis);
+    f32x4 o[2][2 * G];
+    float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int nm = 0; nm < 2; ++nm)
+#pragma unroll
+        for (int i = 0; i < 2 * G; ++i) o[nm][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    const Widen<D> widen(c, rh);
+    Raw<D> raw;
+    if (threadIdx.x < 3 * G) bad[threadIdx.x / G][threadIdx.x % G] = 0;
+    if (begin < end && widen.mine()) {
+        widen.load_keys(raw, begin);
+        widen.load_values(raw, begin);
+    }
+    __syncthreads();
+    int n = 0;
+    for (int t0 = begin; t0 < end; t0 += kWideTile, ++n) {
+        char* stage = lds + (n & 1) * STAGE;
+        if (widen.mine()) {
+            widen.store_keys(raw, stage);
+            widen.store_values(raw, stage, bad[n % 3]);
+        }
+        __syncthreads();  // (one for each tile: the other stage was read before the last one)
+        if (threadIdx.x < G) bad[(n + 2) % 3][threadIdx.x] = 0;  // (read before this barrier, written again after the next)
+        if (t0 + kWideTile < end && widen.mine()) {
+            widen.load_keys(raw, t0 + kWideTile);
+            widen.load_values(raw, t0 + kWideTile);
+        }
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            const char* keys = stage + part * (Widen<D>::KEYS / 2);
+            const char* values = stage + Widen<D>::KEYS + part * (Widen<D>::KEYS / 2);
+            const int s0 = t0 + 32 * part;
+            f32x4 sc[2][2];
+            scores32<D, NP>(keys, qf, sc);
+            if (s0 + 32 > all_see) {
+#pragma unroll
+                for (int nm = 0; nm < 2; ++nm)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (s0 + 8 * kq + j >= vis[nm]) sc[nm][j >> 2][j & 3] = -INFINITY;
+            }
+            bf16x8 pf[2][NP];
+#pragma unroll
+            for (int nm = 0; nm < 2; ++nm) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) top = fmaxf(top, sc[nm][j >> 2][j & 3]);
+                top *= a.scale2;
+                if (__any(top > mx[nm] + 8.f)) {  // (as in attend_packed: the maximum moves when scores outgrow it by 2^8)
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const float now = fmaxf(mx[nm], top), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[nm] - now);
+                    mx[nm] = now;
+                    l[nm] *= f;
+#pragma unroll
+                    for (int i = 0; i < 2 * G; ++i) o[nm][i] = o[nm][i] * f;
+                }
+                const float off = mx[nm] == -INFINITY ? 0.f : mx[nm];
+                float p[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    p[j] = __builtin_amdgcn_exp2f(fmaf(sc[nm][j >> 2][j & 3], a.scale2, -off));
+                    l[nm] += p[j];
+                }
+                pieces8<NP>(p, pf[nm]);
+            }
+#pragma unroll
+            for (int i = 0; i < 2 * G; ++i) {
+                const bf16x8 vf = *reinterpret_cast<const bf16x8*>(values + (i * 64 + lane) * 16);
+#pragma unroll
+                for (int nm = 0; nm < 2; ++nm)
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; --p) o[nm][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[nm][p], o[nm][i], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const unsigned long long marked = bad[n % 3][g];
+            if (marked) {
+#pragma unroll
+                for (int nm = 0; nm < 2; ++nm) {
+                    const int sees = vis[nm] - t0;
+                    if (sees > 0 && (marked & (sees >= 64 ? ~0ull : (1ull << sees) - 1))) o[nm][2 * g] = o[nm][2 * g + 1] = f32x4{NAN, NAN, NAN, NAN};
+                }
+            }
+        }
+    }
+
+    const size_t piece = (size_t)rh * splits + split;
+#pragma unroll
+    for (int nm = 0; nm < 2; ++nm) {
+        l[nm] += __shfl_xor(l[nm], 16);
+        l[nm] += __shfl_xor(l[nm], 32);
+        const int m = m0 + nm * 16 + l15;
+        if (m >= a.m_rows) continue;
+        if (kq == 0) a.part_ml[piece * a.m_rows + m] = f32x2{mx[nm], l[nm]};
+        const bool whole = used == 1;
+        const float inv = whole ? (l[nm] == 0.f ? 0.f : 1.f / l[nm]) : 1.f;
+        const int t = m / a.group, g0 = m - t * a.group;
+        T* out = (T*)a.out + (((size_t)r * a.tokens + t) * a.heads + h * a.group + g0) * D + 8 * kq;
+        float* part = a.part_o + (piece * a.m_rows + m) * D + 8 * kq;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = o[nm][2 * g + (e & 1)][e >> 1] * inv;
+            if (whole)
+                store_n<8, T>(out + 32 * g, y);
+            else
+                store_n<8, float>(part + 32 * g, y);
+        }
     }
 }
 
@@ -749,6 +1020,75 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(AttendArgs a, int slot
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (s + i < len) w[i] = decay == 0.f ? sum[i] : fmaf(decay, w[i], sum[i]);
+}
+
+// ... for more than 32 queries: the scores are formed again (68 bytes of keys per slot, where storing and reading 33 scores is
+// 264), 256 slots of one row and head to a workgroup, 32 queries to a wave.
+constexpr int kWideSlots = 256;
+template <int TYPE, int D>
+__global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_weights_kernel(AttendArgs a, int slot_blocks, float decay) {
+    constexpr int NP = TYPE == AFTER_T_BF16 ? 1 : TYPE == AFTER_T_F16 ? 2 : 3;
+    constexpr int G = D / 32;
+    extern __shared__ __align__(16) char lds[];  // two stages of keys
+    __shared__ float sums[4][kWideSlots];
+    const after_kv4& c = a.c;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, kq = lane >> 4;
+    const int rh = blockIdx.x / slot_blocks, r = rh / c.kv_heads, h = rh % c.kv_heads;
+    const int len = row_length(c, r), begin = (blockIdx.x % slot_blocks) * kWideSlots, end = min(begin + kWideSlots, len);
+    if (begin >= end) return;
+    const int2 p = a.ends[rh];
+    const Widen<D> widen(c, rh);
+    Raw<D> raw;
+    for (int i = threadIdx.x; i < 4 * kWideSlots; i += 256) sums[i / kWideSlots][i % kWideSlots] = 0.f;
+    int n = 0;
+    for (int mg = 0; mg * kWideRows < a.m_rows; ++mg) {
+        const int m0 = mg * kWideRows + wave * 32;
+        bf16x8 qf[2][G][NP];
+        int vis[2];
+        load_queries<TYPE, D, NP>(a, r, h, m0, len, qf, vis);
+        f32x2 ml = {0.f, 0.f};
+        if (m0 + (lane >> 1) < a.m_rows) ml = join_ml<2>(a, p, m0 + (lane >> 1));
+        float off[2], inv[2];
+#pragma unroll
+        for (int nm = 0; nm < 2; ++nm) {
+            const float top = __shfl(ml[0], 2 * (nm * 16 + l15)), sum = __shfl(ml[1], 2 * (nm * 16 + l15));
+            off[nm] = top == -INFINITY ? 0.f : top;
+            inv[nm] = sum == 0.f ? 0.f : 1.f / sum;
+        }
+        if (widen.mine()) widen.load_keys(raw, begin);
+        for (int t0 = begin; t0 < end; t0 += kWideTile, ++n) {
+            char* stage = lds + (n & 1) * Widen<D>::KEYS;
+            if (widen.mine()) widen.store_keys(raw, stage);
+            __syncthreads();
+            if (t0 + kWideTile < end && widen.mine()) widen.load_keys(raw, t0 + kWideTile);
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+                f32x4 sc[2][2];
+                scores32<D, NP>(stage + part * (Widen<D>::KEYS / 2), qf, sc);
+                const int s0 = t0 + 32 * part + 8 * kq;
+                float w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    w[j] = 0.f;
+#pragma unroll
+                    for (int nm = 0; nm < 2; ++nm)
+                        w[j] += s0 + j < vis[nm] ? __builtin_amdgcn_exp2f(fmaf(sc[nm][j >> 2][j & 3], a.scale2, -off[nm])) * inv[nm] : 0.f;
+#pragma unroll
+                    for (int o = 1; o < 16; o *= 2) w[j] += __shfl_xor(w[j], o);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (l15 == j) sums[wave][t0 - begin + 32 * part + 8 * kq + j] += w[j];
+            }
+        }
+        __syncthreads();  // (the next group's first stage may be the one that is still read)
+    }
+    for (int s = begin + threadIdx.x; s < end; s += 256) {
+        const int i = s - begin;
+        const float sum = (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
+        float* w = c.weights + (size_t)rh * c.capacity + s;
+        *w = decay == 0.f ? sum : fmaf(decay, *w, sum);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------- evict
@@ -917,25 +1257,34 @@ int type_bytes(int t) { return t == AFTER_T_F32 ? 4 : 2; }
 bool aligned16(const void* p) { return ((size_t)p & 15) == 0; }
 
 struct Plan {
-    int m_rows, nm, mgroups, wgs;  // wgs: workgroups of four workers, or 0
+    int m_rows, nm, mgroups;
+    int wgs;     // workgroups of four workers, or 0
+    int splits;  // of a row, for more than 32 queries; or 0
     long long pieces, o_bytes, ml_bytes, s_bytes, e_bytes;
 };
 Plan attend_plan(const after_kv4& c, int type, int heads, int tokens, bool count) {
     Plan p;
     p.m_rows = tokens * (heads / c.kv_heads);
     p.nm = p.m_rows > 16 ? 2 : 1;
-    p.mgroups = cdiv(p.m_rows, 16 * p.nm);
+    p.mgroups = p.m_rows > 32 ? cdiv(p.m_rows, kWideRows) : 1;
+    p.wgs = p.splits = 0;
     const long long n_rh = (long long)c.rows * c.kv_heads, most = cdivll(n_rh * (c.capacity / kStep), 4);
-    // As many workers as the chip holds at once: three workgroups on each of 256 CUs with bf16 queries, two with the others (more
-    // registers).  64 rows of 1 .. 8192, bf16: 60 us, and 64 with two; two rows of 131071, fp16: 59 us, and 69 with three.
-    // Rows of at most 512 slots take a workgroup each and one launch: 5.5 us against 8.5.
-    const int full = type == AFTER_T_BF16 ? 768 : 512;
-    p.wgs = c.capacity <= 512 ? 0 : (int)(most < full ? most : full);
-    p.pieces = 4ll * p.wgs + n_rh;
-    p.o_bytes = p.wgs ? p.pieces * p.m_rows * c.head_dim * 4 : 0;
-    p.ml_bytes = p.wgs || count ? (p.pieces * p.m_rows * 8 + 255) / 256 * 256 : 0;
-    p.s_bytes = count ? n_rh * p.m_rows * c.capacity * 4 : 0;
-    p.e_bytes = p.wgs ? (n_rh * 8 + 255) / 256 * 256 : 0;
+    if (p.m_rows > 32) {
+        // two workgroups on each of 256 CUs, and no split below four tiles
+        const long long wanted = cdivll(512, n_rh * p.mgroups), tiles = cdivll(c.capacity, 4 * kWideTile);
+        p.splits = (int)(wanted < tiles ? wanted : tiles);
+    } else if (c.capacity > 512) {
+        // As many workers as the chip holds at once: three workgroups on each of 256 CUs with bf16 queries, two with the others
+        // (more registers).  64 rows of 1 .. 8192, bf16: 60 us, and 64 with two; two rows of 131071, fp16: 59 us, and 69 with
+        // three.  Rows of at most 512 slots take a workgroup each and one launch: 6.4 us against 9.
+        const int full = type == AFTER_T_BF16 ? 768 : 512;
+        p.wgs = (int)(most < full ? most : full);
+    }
+    p.pieces = p.splits ? n_rh * p.splits : 4ll * p.wgs + n_rh;
+    p.o_bytes = p.wgs || p.splits > 1 ? p.pieces * p.m_rows * c.head_dim * 4 : 0;
+    p.ml_bytes = p.wgs || p.splits || count ? (p.pieces * p.m_rows * 8 + 255) / 256 * 256 : 0;
+    p.s_bytes = count && !p.splits ? n_rh * p.m_rows * c.capacity * 4 : 0;
+    p.e_bytes = p.wgs || p.splits ? (n_rh * 8 + 255) / 256 * 256 : 0;
     return p;
 }
 
@@ -943,13 +1292,29 @@ template <int TYPE, int D, int NM, bool COUNT>
 void launch_attend(const AttendArgs& a, const Plan& p, hipStream_t s) {
     constexpr size_t ring = 4 * kRing * kTileBytes<D>, out = 4 * 16 * (D + 4) * 4;  // (at most 53 KB: three workgroups a CU)
     if (p.wgs)
-        hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, NM, COUNT, false>), dim3(p.wgs, p.mgroups), dim3(256), ring, s, a);
+        hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, NM, COUNT, false>), dim3(p.wgs), dim3(256), ring, s, a);
     else
-        hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, NM, COUNT, true>), dim3(a.c.rows * a.c.kv_heads, p.mgroups), dim3(256), ring > out ? ring : out, s, a);
+        hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, NM, COUNT, true>), dim3(a.c.rows * a.c.kv_heads), dim3(256), ring > out ? ring : out, s, a);
 }
 
 template <int TYPE, int D>
 int run_attend(const AttendArgs& a, const Plan& p, bool count, float decay, hipStream_t s) {
+    const int n_rh = a.c.rows * a.c.kv_heads;
+    if (p.splits) {
+        static LdsAttr attr;
+        constexpr size_t lds = 4 * Widen<D>::KEYS;
+        AFTER_TRY(ensure_lds_attr(attr, (const void*)kv4_wide_kernel<TYPE, D>, lds));
+        const long long grid = cdivll((long long)n_rh * p.splits, 8) * 8 * p.mgroups;
+        hipLaunchKernelGGL((kv4_wide_kernel<TYPE, D>), dim3((unsigned)grid), dim3(256), lds, s, a, p.splits, p.mgroups);
+        // (empty rows have no workgroup: their zeros come from the join)
+        hipLaunchKernelGGL((kv4_join_kernel<TYPE, D>), dim3(n_rh * a.m_rows), dim3(256), 0, s, a);
+        if (count) {
+            const int slots = cdiv(a.c.capacity, kWideSlots);
+            hipLaunchKernelGGL((kv4_wide_weights_kernel<TYPE, D>), dim3((unsigned)(n_rh * slots)), dim3(256), 2 * Widen<D>::KEYS, s, a, slots, decay);
+        }
+        AFTER_HIP_CHECK(hipGetLastError());
+        return AFTER_OK;
+    }
     if (p.nm == 1) {
         if (count)
             launch_attend<TYPE, D, 1, true>(a, p, s);
@@ -962,10 +1327,10 @@ int run_attend(const AttendArgs& a, const Plan& p, bool count, float decay, hipS
             launch_attend<TYPE, D, 2, false>(a, p, s);
     }
     if (p.wgs)
-        hipLaunchKernelGGL((kv4_join_kernel<TYPE, D>), dim3(a.c.rows * a.c.kv_heads * a.m_rows), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((kv4_join_kernel<TYPE, D>), dim3(n_rh * a.m_rows), dim3(256), 0, s, a);
     if (count) {
         const int slots = cdiv(a.c.capacity, 1024);
-        hipLaunchKernelGGL(kv4_weights_kernel, dim3(a.c.rows * a.c.kv_heads * slots), dim3(256), 0, s, a, slots, decay);
+        hipLaunchKernelGGL(kv4_weights_kernel, dim3(n_rh * slots), dim3(256), 0, s, a, slots, decay);
     }
     AFTER_HIP_CHECK(hipGetLastError());
     return AFTER_OK;
@@ -1051,7 +1416,7 @@ static int check_attend(const after_kv4* c, int type, int heads, int tokens, con
     AFTER_REQUIRE(tokens > 0 && (long long)tokens * (heads / c->kv_heads) <= 65536, AFTER_E_INVALID, "%s: 1 .. 65536 / (heads / kv_heads) tokens (got %d)",
                   what, tokens);
     const Plan p = attend_plan(*c, type, heads, tokens, false);
-    AFTER_REQUIRE(p.mgroups < 65536 && p.pieces < (1ll << 31) && (long long)c->rows * c->kv_heads * p.m_rows < (1ll << 31) && (long long)c->rows * c->kv_heads * cdiv(c->capacity, 1024) < (1ll << 31),
+    AFTER_REQUIRE(p.pieces * p.mgroups < (1ll << 30) && (long long)c->rows * c->kv_heads * p.m_rows < (1ll << 31) && (long long)c->rows * c->kv_heads * cdiv(c->capacity, kWideSlots) < (1ll << 31),
                   AFTER_E_INVALID, "%s: too many rows x heads x tokens for one call", what);
     return AFTER_OK;
 }

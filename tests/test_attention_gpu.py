@@ -287,7 +287,9 @@ def check_attend(c, q, lens, out, scale, weights=None, before=None, decay=1.0):
     (4, 1, 3, [2, 1, 0, 257, 100], 512),
     (6, 2, 7, [40, 600], 640),
     (16, 1, 2, [129], 2048),
-    (5, 1, 13, [200, 13], 256)])
+    (5, 1, 13, [200, 13], 256),
+    (8, 1, 17, [700, 3, 0, 90], 736),
+    (4, 2, 40, [39, 1500], 1536)])
 def test_attend(hip_device, kind, dim, heads, kv, tokens, lens, capacity):
     t = TYPES[kind]
     c = filled(hip_device, len(lens), kv, dim, capacity, lens, seed=dim + tokens)
@@ -302,10 +304,11 @@ def test_attend(hip_device, kind, dim, heads, kv, tokens, lens, capacity):
         check_attend(c, q, lens, again, 0.2, c.weights, before, decay)
 
 
-def test_attend_does_not_read_what_is_masked(hip_device):
+@pytest.mark.parametrize("T, capacity", [(4, 128), (4, 640), (24, 128), (12, 640)])
+def test_attend_does_not_read_what_is_masked(hip_device, T, capacity):
     """NaN groups behind a row's length, or in slots that a query does not see yet, have no effect; where they are seen the result is NaN."""
-    lens, T = [70, 33], 4
-    c = filled(hip_device, 2, 2, 128, 128, lens, 13)
+    lens = [70, 33]
+    c = filled(hip_device, 2, 2, 128, capacity, lens, 13)
     q = torch.randn(2, T, 4, 128, generator=gen(14)).to(hip_device, torch.bfloat16)
     good, w = c.attend(q, accumulate=True), c.weights.clone()
     for r, n in enumerate(lens):
@@ -316,11 +319,11 @@ def test_attend_does_not_read_what_is_masked(hip_device):
     c.value_scales[0, 1, 69, 2] = 255  # channels 64 .. 95 of the newest slot: seen by the last token's heads 2 and 3
     c.values[0, 1, 69 // 8].view(16, 4, 2, 4)[:, 2, :, 69 % 8 // 2] &= 0x0F  # (a NaN group's codes are zeros)
     out = c.attend(q)
-    assert torch.equal(out[1], good[1]) and torch.equal(out[0, :3], good[0, :3]) and torch.equal(out[0, 3, :2], good[0, 3, :2])
-    assert torch.isnan(out[0, 3, 2:, 64:96]).all() and torch.equal(out[0, 3, 2:, :64], good[0, 3, 2:, :64])
+    assert torch.equal(out[1], good[1]) and torch.equal(out[0, :-1], good[0, :-1]) and torch.equal(out[0, -1, :2], good[0, -1, :2])
+    assert torch.isnan(out[0, -1, 2:, 64:96]).all() and torch.equal(out[0, -1, 2:, :64], good[0, -1, 2:, :64])
     c.key_scales[1, 0, 32, 0] = 255
     out = c.attend(q)
-    assert torch.isnan(out[1, 3, :2]).all() and torch.equal(out[1, :3], good[1, :3]) and torch.equal(out[1, 3, 2:], good[1, 3, 2:])
+    assert torch.isnan(out[1, -1, :2]).all() and torch.equal(out[1, :-1], good[1, :-1]) and torch.equal(out[1, -1, 2:], good[1, -1, 2:])
 
 
 def test_values_of_every_size(hip_device):
