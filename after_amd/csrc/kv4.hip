@@ -103,81 +103,89 @@ struct NewTokens {
     __device__ __forceinline__ int start(int r) const { return starts ? clampi(starts[r], 0, total) : r * each; }
 };
 
-// One wave rounds the new tokens of one (row, head) that fall into one block of eight slots.  Row r owns the block numbers from
-// start(r) / 8 + 2 r on: at least as many as its tokens touch, wherever in a block they begin, so the grid needs no lengths.
+// the largest of 16 neighbouring lanes' values, in all of them (rotations inside the row: no LDS)
+__device__ __forceinline__ unsigned row_max(unsigned x) {
+    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xF, 0xF, true));
+    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xF, 0xF, true));
+    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xF, 0xF, true));
+    return max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xF, 0xF, true));
+}
+// ... of four
+__device__ __forceinline__ unsigned quad_max(unsigned x) {
+    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, true));         // lanes 1 0 3 2
+    return max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, true));  // lanes 2 3 0 1
+}
+
+struct AppendArgs {
+    after_kv4 c;
+    NewTokens nt;
+    const void *k, *v;
+    long long kts, khs, vts, vhs;
+};
+
+// One wave rounds those of a row's new tokens, len .. end, that fall into block sb of eight slots, for one head; t0: the row's first.
 template <int TYPE, int D>
-__global__ __launch_bounds__(256) void kv4_append_kernel(after_kv4 c, NewTokens nt, const void* kp, const void* vp, long long kts, long long khs,
-                                                         long long vts, long long vhs, int items) {
+__device__ __forceinline__ void append_block(const AppendArgs& a, int r, int h, int t0, int len, int end, int sb) {
     using T = typename Elem<TYPE>::T;
     constexpr int G = D / 32;
+    const after_kv4& c = a.c;
     const int lane = threadIdx.x & 63;
-    const int item = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (item >= items) return;
-    const int h = item % c.kv_heads, fb = item / c.kv_heads;
-    int lo = 0, hi = c.rows - 1;  // the last row that begins at or before fb
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (nt.start(mid) / 8 + 2 * mid <= fb)
-            lo = mid;
-        else
-            hi = mid - 1;
-    }
-    const int r = lo, t0 = nt.start(r), n = nt.start(r + 1) - t0;
-    const int len = row_length(c, r);
-    const int sb = len / 8 + fb - (t0 / 8 + 2 * r);
-    const int end = min(len + max(n, 0), c.capacity);  // tokens that do not fit are dropped (kv4_advance_kernel reports them)
-    if (sb < 0 || 8 * sb >= end) return;
     const size_t rh = (size_t)r * c.kv_heads + h;
-    const T* k = (const T*)kp + (size_t)h * khs;
-    const T* v = (const T*)vp + (size_t)h * vhs;
-
+    const T* k = (const T*)a.k + (size_t)h * a.khs;
+    const T* v = (const T*)a.v + (size_t)h * a.vhs;
+    // keys: eight channels per lane; values: two channels of the eight tokens per lane.  Everything is asked for first.
+    float x[D / 64][8], y[8][2];
+    bool in[D / 64];
+#pragma unroll
+    for (int it = 0; it < D / 64; ++it) {
+        const int id = it * 64 + lane, s = 8 * sb + id / (D / 8);
+        in[it] = s >= len && s < end;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[it][i] = 0.f;
+        if (in[it]) load_n<8, T>(k + (long long)(t0 + s - len) * a.kts + 8 * (id % (D / 8)), x[it]);
+    }
+    const bool holds = 2 * lane < D;
+#pragma unroll
+    for (int tt = 0; tt < 8; ++tt) {
+        const int s = 8 * sb + tt;
+        y[tt][0] = y[tt][1] = 0.f;
+        if (holds && s >= len && s < end) load_n<2, T>(v + (long long)(t0 + s - len) * a.vts + 2 * lane, y[tt]);
+    }
     if (lane < 8) {
         const int s = 8 * sb + lane;
         if (s >= len && s < end) c.weights[rh * c.capacity + s] = 0.f;
     }
-    // keys: eight channels per lane
 #pragma unroll
     for (int it = 0; it < D / 64; ++it) {
-        const int id = it * 64 + lane, tt = id / (D / 8), ch = id % (D / 8), s = 8 * sb + tt;
-        const bool in = s >= len && s < end;
-        float x[8] = {};
-        if (in) load_n<8, T>(k + (long long)(t0 + s - len) * kts + 8 * ch, x);
+        const int id = it * 64 + lane, ch = id % (D / 8), s = 8 * sb + id / (D / 8);
         unsigned top = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, abs_bits(x[i]));
-        top = max(top, (unsigned)__shfl_xor((int)top, 1));
-        top = max(top, (unsigned)__shfl_xor((int)top, 2));
-        const int b = scale_byte(top);
+        for (int i = 0; i < 8; ++i) top = max(top, abs_bits(x[it][i]));
+        const int b = scale_byte(quad_max(top));
         const float sc = byte_scale(b);
-        unsigned w = round4(x[0], x[1], sc) | round4(x[2], x[3], sc) << 8 | round4(x[4], x[5], sc) << 16 | round4(x[6], x[7], sc) << 24;
+        unsigned w = round4(x[it][0], x[it][1], sc) | round4(x[it][2], x[it][3], sc) << 8 | round4(x[it][4], x[it][5], sc) << 16 | round4(x[it][6], x[it][7], sc) << 24;
         if (b == kBadByte) w = 0;
-        if (in) {
+        if (in[it]) {
             *reinterpret_cast<unsigned*>(c.keys + (rh * c.capacity + s) * (D / 2) + 4 * ch) = w;
             if ((ch & 3) == 0) c.key_scales[(rh * c.capacity + s) * G + ch / 4] = (unsigned char)b;
         }
     }
-    // values: two channels of the eight tokens per lane
-    if (2 * lane < D) {
-        unsigned w0 = 0, w1 = 0, mask = 0;
+    unsigned w0 = 0, w1 = 0, mask = 0;
+    int mine = 0;  // lane tt of each 16: token tt's byte
 #pragma unroll
-        for (int tt = 0; tt < 8; ++tt) {
-            const int s = 8 * sb + tt;
-            const bool in = s >= len && s < end;
-            if (!in) continue;  // (uniform)
-            float x[2];
-            load_n<2, T>(v + (long long)(t0 + s - len) * vts + 2 * lane, x);
-            unsigned top = max(abs_bits(x[0]), abs_bits(x[1]));
-#pragma unroll
-            for (int o = 1; o < 16; o *= 2) top = max(top, (unsigned)__shfl_xor((int)top, o));
-            const int b = scale_byte(top);
-            const unsigned u = b == kBadByte ? 0u : round4(x[0], x[1], byte_scale(b));
-            w0 |= (u & 15u) << 4 * tt;
-            w1 |= (u >> 4) << 4 * tt;
-            mask |= 15u << 4 * tt;
-            if ((lane & 15) == 0) c.value_scales[(rh * c.capacity + s) * G + lane / 16] = (unsigned char)b;
-        }
+    for (int tt = 0; tt < 8; ++tt) {
+        const int s = 8 * sb + tt, b = scale_byte(row_max(max(abs_bits(y[tt][0]), abs_bits(y[tt][1]))));
+        const unsigned u = b == kBadByte ? 0u : round4(y[tt][0], y[tt][1], byte_scale(b));
+        w0 |= (u & 15u) << 4 * tt;
+        w1 |= (u >> 4) << 4 * tt;
+        mask |= s >= len && s < end ? 15u << 4 * tt : 0u;
+        mine = (lane & 15) == tt ? b : mine;
+    }
+    if (holds) {
+        const int s = 8 * sb + (lane & 15);
+        if ((lane & 15) < 8 && s >= len && s < end) c.value_scales[(rh * c.capacity + s) * G + lane / 16] = (unsigned char)mine;
         u32x2* at = reinterpret_cast<u32x2*>(c.values + ((rh * (c.capacity / 8) + sb) * D + (lane & 15) * (D / 16) + (lane >> 4) * 2) * 4);
-        u32x2 w = {w0, w1};
+        u32x2 w = {w0 & mask, w1 & mask};
         if (mask != 0xFFFFFFFFu) {  // the other slots of the block keep what they hold
             const u32x2 old = *at;
             w = w | (old & ~mask);
@@ -186,12 +194,46 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(after_kv4 c, NewTokens 
     }
 }
 
-__global__ void kv4_advance_kernel(after_kv4 c, NewTokens nt) {
-    const int r = blockIdx.x * blockDim.x + threadIdx.x;
-    if (r >= c.rows) return;
-    const int len = row_length(c, r), n = max(nt.start(r + 1) - nt.start(r), 0);
+// A wave for each block and head.  Row r owns the block numbers from start(r) / 8 + 2 r on: at least as many as its tokens touch,
+// wherever in a block they begin, so the grid needs no lengths.
+template <int TYPE, int D>
+__global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a, int items) {
+    const after_kv4& c = a.c;
+    const int item = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item >= items) return;
+    const int h = item % c.kv_heads, fb = item / c.kv_heads;
+    int lo = 0, hi = c.rows - 1;  // the last row that begins at or before fb
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a.nt.start(mid) / 8 + 2 * mid <= fb)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    const int r = lo, t0 = a.nt.start(r), n = a.nt.start(r + 1) - t0, len = row_length(c, r);
+    const int sb = len / 8 + fb - (t0 / 8 + 2 * r), end = min(len + max(n, 0), c.capacity);  // tokens that do not fit are dropped
+    if (sb >= 0 && 8 * sb < end) append_block<TYPE, D>(a, r, h, t0, len, end, sb);
+}
+
+__device__ __forceinline__ void advance(const after_kv4& c, const NewTokens& nt, int r, int len) {
+    const int n = max(nt.start(r + 1) - nt.start(r), 0);
     if (n > c.capacity - len) *c.failed = 1;
     c.lengths[r] = min(n, c.capacity - len) + len;
+}
+__global__ void kv4_advance_kernel(after_kv4 c, NewTokens nt) {
+    const int r = blockIdx.x * blockDim.x + threadIdx.x;
+    if (r < c.rows) advance(c, nt, r, row_length(c, r));
+}
+
+// The same with a workgroup for each row, which also moves the row's length: one launch where there are few tokens.
+template <int TYPE, int D>
+__global__ __launch_bounds__(512) void kv4_append_rows_kernel(AppendArgs a) {
+    const after_kv4& c = a.c;
+    const int r = blockIdx.x, t0 = a.nt.start(r), n = a.nt.start(r + 1) - t0, len = row_length(c, r), end = min(len + max(n, 0), c.capacity);
+    const int first = len / 8, blocks = end > len ? (end - 1) / 8 - first + 1 : 0;
+    for (int i = threadIdx.x >> 6; i < blocks * c.kv_heads; i += 8) append_block<TYPE, D>(a, r, i % c.kv_heads, t0, len, end, first + i / c.kv_heads);
+    __syncthreads();  // (every wave has read the length)
+    if (threadIdx.x == 0) advance(c, a.nt, r, len);
 }
 
 __global__ void kv4_truncate_kernel(after_kv4 c, const int* lengths) {
@@ -771,8 +813,9 @@ __device__ __forceinline__ void load_queries(const AttendArgs& a, int r, int h, 
     }
 }
 
-// scores of 32 tokens: sc[nm][f][i]: token 8 kq + 4 f + i
-template <int D, int NP>
+// scores of 32 tokens.  BY_TOKEN: sc[nm][f][i] is query l15 (a column), token 8 kq + 4 f + i; otherwise query 4 kq + i, token
+// 8 (l15 / 4) + 4 f + l15 % 4 (a column): the operands are alike, only their order differs.
+template <int D, int NP, bool BY_TOKEN>
 __device__ __forceinline__ void scores32(const char* keys, const bf16x8 (&qf)[2][D / 32][NP], f32x4 (&sc)[2][2]) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -784,7 +827,9 @@ __device__ __forceinline__ void scores32(const char* keys, const bf16x8 (&qf)[2]
 #pragma unroll
             for (int nm = 0; nm < 2; ++nm)
 #pragma unroll
-                for (int p = NP - 1; p >= 0; --p) sc[nm][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[nm][s][p], sc[nm][f], 0, 0, 0);
+                for (int p = NP - 1; p >= 0; --p)
+                    sc[nm][f] = BY_TOKEN ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[nm][s][p], sc[nm][f], 0, 0, 0)
+                                         : __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[nm][s][p], kf, sc[nm][f], 0, 0, 0);
         }
     }
 }
@@ -850,7 +895,7 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_ker
             const char* values = stage + Widen<D>::KEYS + part * (Widen<D>::KEYS / 2);
             const int s0 = t0 + 32 * part;
             f32x4 sc[2][2];
-            scores32<D, NP>(keys, qf, sc);
+            scores32<D, NP, true>(keys, qf, sc);
             if (s0 + 32 > all_see) {
 #pragma unroll
                 for (int nm = 0; nm < 2; ++nm)
@@ -1023,10 +1068,10 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(AttendArgs a, int slot
 }
 
 // ... for more than 32 queries: the scores are formed again (68 bytes of keys per slot, where storing and reading 33 scores is
-// 264), 256 slots of one row and head to a workgroup, 32 queries to a wave.
-constexpr int kWideSlots = 256;
+// 264), up to 1024 slots of one row and head to a workgroup (its beginning costs as much as some 300), 32 queries to a wave.
+constexpr int kWideSlots = 1024;  // at most
 template <int TYPE, int D>
-__global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_weights_kernel(AttendArgs a, int slot_blocks, float decay) {
+__global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_weights_kernel(AttendArgs a, int slot_blocks, int slots, float decay) {
     constexpr int NP = TYPE == AFTER_T_BF16 ? 1 : TYPE == AFTER_T_F16 ? 2 : 3;
     constexpr int G = D / 32;
     extern __shared__ __align__(16) char lds[];  // two stages of keys
@@ -1034,7 +1079,7 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_wei
     const after_kv4& c = a.c;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, kq = lane >> 4;
     const int rh = blockIdx.x / slot_blocks, r = rh / c.kv_heads, h = rh % c.kv_heads;
-    const int len = row_length(c, r), begin = (blockIdx.x % slot_blocks) * kWideSlots, end = min(begin + kWideSlots, len);
+    const int len = row_length(c, r), begin = (blockIdx.x % slot_blocks) * slots, end = min(begin + slots, len);
     if (begin >= end) return;
     const int2 p = a.ends[rh];
     const Widen<D> widen(c, rh);
@@ -1048,13 +1093,19 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_wei
         load_queries<TYPE, D, NP>(a, r, h, m0, len, qf, vis);
         f32x2 ml = {0.f, 0.f};
         if (m0 + (lane >> 1) < a.m_rows) ml = join_ml<2>(a, p, m0 + (lane >> 1));
-        float off[2], inv[2];
+        float off[2][4], inv[2][4];  // of query 16 nm + 4 kq + i
+        int sees[2][4];
 #pragma unroll
-        for (int nm = 0; nm < 2; ++nm) {
-            const float top = __shfl(ml[0], 2 * (nm * 16 + l15)), sum = __shfl(ml[1], 2 * (nm * 16 + l15));
-            off[nm] = top == -INFINITY ? 0.f : top;
-            inv[nm] = sum == 0.f ? 0.f : 1.f / sum;
-        }
+        for (int nm = 0; nm < 2; ++nm)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int m = nm * 16 + 4 * kq + i;
+                const float top = __shfl(ml[0], 2 * m), sum = __shfl(ml[1], 2 * m);
+                off[nm][i] = top == -INFINITY ? 0.f : top;
+                inv[nm][i] = sum == 0.f ? 0.f : 1.f / sum;
+                sees[nm][i] = __shfl(vis[nm], 4 * kq + i);
+            }
+        const int all_see = m0 + 32 <= a.m_rows ? len - a.tokens + m0 / a.group + 1 : 0;
         if (widen.mine()) widen.load_keys(raw, begin);
         for (int t0 = begin; t0 < end; t0 += kWideTile, ++n) {
             char* stage = lds + (n & 1) * Widen<D>::KEYS;
@@ -1064,21 +1115,22 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_wei
 #pragma unroll
             for (int part = 0; part < 2; ++part) {
                 f32x4 sc[2][2];
-                scores32<D, NP>(stage + part * (Widen<D>::KEYS / 2), qf, sc);
-                const int s0 = t0 + 32 * part + 8 * kq;
-                float w[8];
+                scores32<D, NP, false>(stage + part * (Widen<D>::KEYS / 2), qf, sc);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    w[j] = 0.f;
+                for (int f = 0; f < 2; ++f) {
+                    const int tok = 32 * part + 8 * (l15 >> 2) + 4 * f + (l15 & 3), s = t0 + tok;
+                    float w = 0.f;
 #pragma unroll
                     for (int nm = 0; nm < 2; ++nm)
-                        w[j] += s0 + j < vis[nm] ? __builtin_amdgcn_exp2f(fmaf(sc[nm][j >> 2][j & 3], a.scale2, -off[nm])) * inv[nm] : 0.f;
 #pragma unroll
-                    for (int o = 1; o < 16; o *= 2) w[j] += __shfl_xor(w[j], o);
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = __builtin_amdgcn_exp2f(fmaf(sc[nm][f][i], a.scale2, -off[nm][i]));
+                            w = t0 + kWideTile <= all_see || s < sees[nm][i] ? fmaf(x, inv[nm][i], w) : w;
+                        }
+                    w += __shfl_xor(w, 16);
+                    w += __shfl_xor(w, 32);
+                    if (kq == f) sums[wave][t0 - begin + tok] += w;
                 }
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (l15 == j) sums[wave][t0 - begin + 32 * part + 8 * kq + j] += w[j];
             }
         }
         __syncthreads();  // (the next group's first stage may be the one that is still read)
@@ -1099,36 +1151,18 @@ __device__ __forceinline__ unsigned order_key(float x) {
     return u == 0x80000000u ? 0x80000000u : (u >> 31) ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelThreads = 1024;
-
-// inclusive sum over the workgroup's threads; *total = the last one's.  `tmp`: one word per wave
-__device__ __forceinline__ int block_scan(int x, int* tmp, int* total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const int y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 63) tmp[wave] = x;
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int w = 0; w < kSelThreads / 64; ++w) {
-        if (w < wave) before += tmp[w];
-        all += tmp[w];
-    }
-    *total = all;
-    return x + before;
-}
+constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
 
 // One workgroup per (row, head): which slots stay, in order.  The `recent` newest stay; of the others the `want` with the
-// largest weights: the value of the smallest of those is found eleven bits at a time (a histogram of the next digit of the
-// candidates), then one ordered pass writes the slots above it, and the first of those equal to it.
+// largest weights.  The value of the smallest of those is found eleven bits at a time: a histogram of the next digit of the
+// candidates (in four copies: a few digits hold most of the weights, and the same address twice in an instruction costs twice),
+// and where from the top its sums pass `want`.  Then each wave looks through a sixteenth of the slots: once to count what stays,
+// and, knowing what the waves before it keep, once to write them: those above the value, and the first `want` equal to it.
 __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(after_kv4 c, int keep, int recent, int* slots) {
-    __shared__ int hist[2048];
-    __shared__ int tmp[kSelThreads / 64];
+    __shared__ int hist[2048][4];
+    __shared__ int tmp[kSelWaves][2];
     __shared__ int found[2];
-    const int rh = blockIdx.x, r = rh / c.kv_heads, tid = threadIdx.x;
+    const int rh = blockIdx.x, r = rh / c.kv_heads, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int len = row_length(c, r);
     int* out = slots + (size_t)rh * keep;
     const float* w = c.weights + (size_t)rh * c.capacity;
@@ -1139,34 +1173,51 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(after_kv4 c, in
     }
     const int old = len - recent;  // (recent <= keep < len)
     int want = keep - recent;
-    unsigned prefix = 0;
-    int total;
+    unsigned prefix = 0xFFFFFFFFu;  // (want = 0: nothing is above, and nothing that is equal is wanted)
     if (want > 0) {
+        prefix = 0;
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, bins = 1 << bits;
-            for (int i = tid; i < bins; i += kSelThreads) hist[i] = 0;
+            for (int i = tid; i < bins * 4; i += kSelThreads) hist[i >> 2][i & 3] = 0;
             __syncthreads();
-            for (int i = tid; i < old; i += kSelThreads) {
-                const unsigned k = order_key(w[i]);
-                if (pass == 0 || (k >> (shift + bits)) == (prefix >> (shift + bits))) atomicAdd(&hist[k >> shift & (bins - 1)], 1);
+            auto add = [&](float x) {
+                const unsigned k = order_key(x);
+                if (pass == 0 || (k >> (shift + bits)) == (prefix >> (shift + bits))) atomicAdd(&hist[k >> shift & (bins - 1)][lane & 3], 1);
+            };
+            // (rows of weights begin and end at multiples of 128 bytes)
+            for (int i = 4 * tid; i < old; i += 16 * kSelThreads) {
+                f32x4 x[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (i + u * 4 * kSelThreads < old) x[u] = *reinterpret_cast<const f32x4*>(w + i + u * 4 * kSelThreads);
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (i + u * 4 * kSelThreads + j < old) add(x[u][j]);
             }
             __syncthreads();
-            // the digit in which the want-th largest lies: thread t looks at bins from the top, two each
+            // thread t looks at two bins (one, in the last pass), from the top
             const int per = bins / kSelThreads;
-            int mine = 0;
-            for (int i = 0; i < per; ++i) mine += hist[bins - 1 - (tid * per + i)];
-            const int upto = block_scan(mine, tmp, &total);
+            int mine = 0, bin_sum[2] = {0, 0};
+            for (int j = 0; j < per; ++j) {
+                const int bin = bins - 1 - (tid * per + j);
+                bin_sum[j] = (hist[bin][0] + hist[bin][1]) + (hist[bin][2] + hist[bin][3]);
+                mine += bin_sum[j];
+            }
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 64; o *= 2) {
+                const int y = __shfl_up(upto, o);
+                if (lane >= o) upto += y;
+            }
+            if (lane == 63) tmp[wave][0] = upto;
+            __syncthreads();
+            for (int v = 0; v < wave; ++v) upto += tmp[v][0];
             if (upto >= want && upto - mine < want) {
-                int above = upto - mine;
-                for (int i = 0; i < per; ++i) {
-                    const int bin = bins - 1 - (tid * per + i);
-                    if (above + hist[bin] >= want) {
-                        found[0] = bin;
-                        found[1] = want - above;
-                        break;
-                    }
-                    above += hist[bin];
-                }
+                const int above = upto - mine, second = above + bin_sum[0] < want;
+                found[0] = bins - 1 - (tid * per + second);
+                found[1] = want - above - (second ? bin_sum[0] : 0);
             }
             __syncthreads();
             prefix |= (unsigned)found[0] << shift;
@@ -1174,28 +1225,46 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(after_kv4 c, in
             __syncthreads();
         }
     }
-    // slots above the value, the first `want` equal to it, and the newest, in order
-    int done = 0, equal_done = 0;
-    const bool any = keep > recent;
-    for (int i0 = 0; i0 < len; i0 += kSelThreads) {
-        const int i = i0 + tid;
-        int above = 0, equal = 0;
-        if (i < len) {
-            if (i >= old)
-                above = 1;
-            else if (any) {
-                const unsigned k = order_key(w[i]);
-                above = k > prefix;
-                equal = k == prefix;
-            }
+    const int per = (len + kSelThreads - 1) / kSelThreads * 64, begin = wave * per, end = min(begin + per, len);
+    constexpr int U = 8;  // loads on their way at a time
+    int above = 0, equal = 0;
+    for (int i0 = begin; i0 < end; i0 += U * 64) {
+        unsigned k[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) k[u] = i0 + u * 64 + lane < end ? order_key(w[i0 + u * 64 + lane]) : 0u;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * 64 + lane;
+            above += __popcll(__ballot(i < end && (i >= old || k[u] > prefix)));
+            equal += __popcll(__ballot(i < min(end, old) && k[u] == prefix));
         }
-        int n_equal, n_stay;
-        const int eq = block_scan(equal, tmp, &n_equal);
-        const int stay = above | (equal && equal_done + eq <= want);
-        const int at = block_scan(stay, tmp, &n_stay);
-        if (stay) out[done + at - 1] = i;
-        done += n_stay;
-        equal_done += n_equal;
+    }
+    if (lane == 0) {
+        tmp[wave][0] = above;
+        tmp[wave][1] = equal;
+    }
+    __syncthreads();
+    int done = 0, equal_done = 0;  // kept / equal before this wave
+    for (int v = 0; v < wave; ++v) {
+        done += tmp[v][0];
+        equal_done += tmp[v][1];
+    }
+    done += min(equal_done, want);
+    const unsigned long long before = (1ull << lane) - 1;
+    for (int i0 = begin; i0 < end; i0 += U * 64) {
+        unsigned k[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) k[u] = i0 + u * 64 + lane < end ? order_key(w[i0 + u * 64 + lane]) : 0u;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * 64 + lane;
+            const unsigned long long eq = __ballot(i < min(end, old) && k[u] == prefix);
+            const bool is_equal = eq >> lane & 1, stay = i < end && (i >= old || k[u] > prefix || (is_equal && equal_done + __popcll(eq & before) < want));
+            const unsigned long long all = __ballot(stay);
+            if (stay) out[done + __popcll(all & before)] = i;
+            done += __popcll(all);
+            equal_done += __popcll(eq);
+        }
     }
 }
 
@@ -1203,40 +1272,47 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(after_kv4 c, in
 template <int D>
 __global__ __launch_bounds__(256) void kv4_move_kernel(after_kv4 c, after_kv4 to, int keep, const int* slots, int nb, long long items) {
     constexpr int G = D / 32;
-    const int lane = threadIdx.x & 63;
-    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long item = (long long)blockIdx.x * 4 + wave;
     if (item >= items) return;
-    const size_t rh = item / nb;
-    const int sb = (int)(item % nb), r = (int)(rh / c.kv_heads);
-    const int n = min(row_length(c, r), keep);
+    const int rh = (int)(item / nb), sb = (int)(item % nb), r = rh / c.kv_heads;
+    const int n = min(row_length(c, r), keep), m = min(n - 8 * sb, 8);
     if (sb == 0 && lane == 0 && rh % c.kv_heads == 0) to.lengths[r] = n;
-    if (8 * sb >= n) return;
-    const int* pick = slots + rh * keep + 8 * sb;
-    const size_t src = rh * c.capacity, dst = rh * to.capacity + 8 * sb;
-    if (lane < 8 && 8 * sb + lane < n) to.weights[dst + lane] = c.weights[src + pick[lane]];
-#pragma unroll
-    for (int it = 0; it < D / 64; ++it) {  // a dword (eight channels) per lane
-        const int id = it * 64 + lane, tt = id / (D / 8), ch = id % (D / 8);
-        if (8 * sb + tt < n)
-            reinterpret_cast<unsigned*>(to.keys + (dst + tt) * (D / 2))[ch] = reinterpret_cast<const unsigned*>(c.keys + (src + pick[tt]) * (D / 2))[ch];
-    }
-    if (lane < 8 * G) {
-        const int tt = lane / G, g = lane % G;
-        if (8 * sb + tt < n) {
-            to.key_scales[(dst + tt) * G + g] = c.key_scales[(src + pick[tt]) * G + g];
-            to.value_scales[(dst + tt) * G + g] = c.value_scales[(src + pick[tt]) * G + g];
-        }
-    }
+    if (m <= 0) return;
+    const size_t src = (size_t)rh * c.capacity, dst = (size_t)rh * to.capacity + 8 * sb;
+    const int pick = lane < m ? slots[(size_t)rh * keep + 8 * sb + lane] : 0;  // (slot 0 for what is not there: read, not used)
+    u32x2 x[8];
     if (2 * lane < D) {
-        u32x2 w = {0, 0};
 #pragma unroll
         for (int tt = 0; tt < 8; ++tt) {
-            if (8 * sb + tt >= n) continue;
-            const int s = pick[tt];
-            const u32x2 x = reinterpret_cast<const u32x2*>(c.values + (src / 8 + s / 8) * (size_t)(4 * D))[lane];
-            w = w | (x >> 4 * (s & 7) & 15u) << 4 * tt;
+            const int s = __builtin_amdgcn_readlane(pick, tt);
+            x[tt] = reinterpret_cast<const u32x2*>(c.values + (src + s) / 8 * (4 * D))[lane];
         }
-        reinterpret_cast<u32x2*>(to.values + (dst / 8) * (size_t)(4 * D))[lane] = w;
+    }
+    // keys: 16 bytes per lane; scales: a token's group per lane
+    const int kt = lane / (D / 32), kc = lane % (D / 32), gt = lane / G, g = lane % G;
+    u32x4 k;
+    unsigned char ks, vs;
+    const size_t from = src + __shfl(pick, gt);
+    if (lane < 8 * G) {
+        k = reinterpret_cast<const u32x4*>(c.keys + (src + __shfl(pick, kt)) * (D / 2))[kc];
+        ks = c.key_scales[from * G + g];
+        vs = c.value_scales[from * G + g];
+    }
+    if (lane < m) to.weights[dst + lane] = c.weights[src + pick];
+    if (lane < m * G) {
+        reinterpret_cast<u32x4*>(to.keys + (dst + kt) * (D / 2))[kc] = k;
+        to.key_scales[(dst + gt) * G + g] = ks;
+        to.value_scales[(dst + gt) * G + g] = vs;
+    }
+    if (2 * lane < D) {
+        u32x2 y = {0, 0};
+#pragma unroll
+        for (int tt = 0; tt < 8; ++tt) {
+            const int s = __builtin_amdgcn_readlane(pick, tt);
+            if (tt < m) y = y | (x[tt] >> 4 * (s & 7) & 15u) << 4 * tt;
+        }
+        reinterpret_cast<u32x2*>(to.values + dst / 8 * (4 * D))[lane] = y;
     }
 }
 
@@ -1309,8 +1385,9 @@ int run_attend(const AttendArgs& a, const Plan& p, bool count, float decay, hipS
         // (empty rows have no workgroup: their zeros come from the join)
         hipLaunchKernelGGL((kv4_join_kernel<TYPE, D>), dim3(n_rh * a.m_rows), dim3(256), 0, s, a);
         if (count) {
-            const int slots = cdiv(a.c.capacity, kWideSlots);
-            hipLaunchKernelGGL((kv4_wide_weights_kernel<TYPE, D>), dim3((unsigned)(n_rh * slots)), dim3(256), 2 * Widen<D>::KEYS, s, a, slots, decay);
+            const long long even = cdivll((long long)n_rh * a.c.capacity, 512 * kWideTile) * kWideTile;  // two workgroups a CU
+            const int slots = (int)(even < 256 ? 256 : even < kWideSlots ? even : kWideSlots), blocks = cdiv(a.c.capacity, slots);
+            hipLaunchKernelGGL((kv4_wide_weights_kernel<TYPE, D>), dim3((unsigned)(n_rh * blocks)), dim3(256), 2 * Widen<D>::KEYS, s, a, blocks, slots, decay);
         }
         AFTER_HIP_CHECK(hipGetLastError());
         return AFTER_OK;
@@ -1369,12 +1446,18 @@ extern "C" int after_kv4_append(const after_kv4* c, const void* k, const void* v
     const NewTokens nt{starts, tokens, (int)total};
     const long long items = (total / 8 + 2ll * c->rows) * c->kv_heads;
     AFTER_REQUIRE(items < (1ll << 31), AFTER_E_INVALID, "kv4_append: too many new tokens x heads for one call");
-#define CALL(T, D)                                                                                                                            \
-    hipLaunchKernelGGL((kv4_append_kernel<T, D>), dim3((unsigned)cdivll(items, 4)), dim3(256), 0, s, *c, nt, k, v, k_token_stride, k_head_stride, \
-                       v_token_stride, v_head_stride, (int)items)
-    KV4_BY_TYPE(type, c->head_dim, CALL);
+    const AppendArgs a{*c, nt, k, v, k_token_stride, k_head_stride, v_token_stride, v_head_stride};
+    // A workgroup per row where no row can have many: 64 rows of one token each in one launch.  (`starts` may give all to one row.)
+    if (starts ? total <= 2ll * c->rows && total <= 256 : tokens <= 16) {
+#define CALL(T, D) hipLaunchKernelGGL((kv4_append_rows_kernel<T, D>), dim3(c->rows), dim3(512), 0, s, a)
+        KV4_BY_TYPE(type, c->head_dim, CALL);
 #undef CALL
-    hipLaunchKernelGGL(kv4_advance_kernel, dim3(cdiv(c->rows, 256)), dim3(256), 0, s, *c, nt);
+    } else {
+#define CALL(T, D) hipLaunchKernelGGL((kv4_append_kernel<T, D>), dim3((unsigned)cdivll(items, 4)), dim3(256), 0, s, a, (int)items)
+        KV4_BY_TYPE(type, c->head_dim, CALL);
+#undef CALL
+        hipLaunchKernelGGL(kv4_advance_kernel, dim3(cdiv(c->rows, 256)), dim3(256), 0, s, *c, nt);
+    }
     AFTER_HIP_CHECK(hipGetLastError());
     return AFTER_OK;
 }
@@ -1416,7 +1499,7 @@ static int check_attend(const after_kv4* c, int type, int heads, int tokens, con
     AFTER_REQUIRE(tokens > 0 && (long long)tokens * (heads / c->kv_heads) <= 65536, AFTER_E_INVALID, "%s: 1 .. 65536 / (heads / kv_heads) tokens (got %d)",
                   what, tokens);
     const Plan p = attend_plan(*c, type, heads, tokens, false);
-    AFTER_REQUIRE(p.pieces * p.mgroups < (1ll << 30) && (long long)c->rows * c->kv_heads * p.m_rows < (1ll << 31) && (long long)c->rows * c->kv_heads * cdiv(c->capacity, kWideSlots) < (1ll << 31),
+    AFTER_REQUIRE(p.pieces * p.mgroups < (1ll << 30) && (long long)c->rows * c->kv_heads * p.m_rows < (1ll << 31) && (long long)c->rows * c->kv_heads * cdiv(c->capacity, 256) < (1ll << 31),
                   AFTER_E_INVALID, "%s: too many rows x heads x tokens for one call", what);
     return AFTER_OK;
 }
