@@ -104,6 +104,13 @@ __device__ __forceinline__ bool odd_value(u32x4 w) {
     return bad;
 }
 
+// a barrier for what is in LDS: loads on their way stay on their way (__syncthreads waits for them)
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 template <int TYPE, int D>
 __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 : 2) void attend_packed_kernel(PackedArgs a) {
     using E = Elem<TYPE>;
@@ -113,19 +120,20 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
     constexpr int DT = D / 32;
     constexpr unsigned STAGE = 2 * BN * PIECES * 16;
     extern __shared__ __align__(16) char lds[];
-    __shared__ unsigned long long odd_rows;
+    __shared__ unsigned long long odd_rows[3];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, half = lane >> 5;
     // neighbouring workgroups are dispatched to different XCDs: a key head's workgroups stay on one L2 where there are eight.
     // Tiles from the last to the first: with a causal mask the longest first.
     const int h = blockIdx.x % a.kv_heads, tile = a.tiles - 1 - blockIdx.x / a.kv_heads;
+    // the last sequence that begins at or before this tile: 64 candidates at a time
     int lo = 0, hi = a.n_seqs;
     while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if ((int)((long long)q_start(a, mid) * a.group / BM) + mid <= tile)
-            lo = mid;
-        else
-            hi = mid - 1;
+        const int step = (hi - lo + 64) / 64, at = min(lo + lane * step, hi);
+        const bool begun = (int)((long long)q_start(a, at) * a.group / BM) + at <= tile;
+        const unsigned long long all = __ballot(begun && lo + lane * step <= hi) | 1;  // (sequence lo has begun)
+        lo += (63 - __clzll(all)) * step;
+        hi = min(hi, lo + step - 1);
     }
     const int b = lo, q0 = q_start(a, b), nq = q_start(a, b + 1) - q0;
     const int row0 = (tile - ((int)((long long)q0 * a.group / BM) + b)) * BM;
@@ -144,6 +152,13 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
     seen(a, t + nk - nq, nk, first, last);
     seen(a, row0 / a.group + nk - nq, nk, t_first, dummy);
     seen(a, (min(row0 + BM, rows) - 1) / a.group + nk - nq, nk, dummy, t_last);
+    // the keys that some query of the wave sees
+    int w_first = 0, w_last = 0;
+    const int w_row = __builtin_amdgcn_readfirstlane(row0 + wave * 32);
+    if (w_row < rows) {
+        seen(a, w_row / a.group + nk - nq, nk, w_first, dummy);
+        seen(a, (min(w_row + 32, rows) - 1) / a.group + nk - nq, nk, dummy, w_last);
+    }
     // every query of the workgroup sees [all_first, all_last)
     int all_first, all_last;
     seen(a, row0 / a.group + nk - nq, nk, dummy, all_last);
@@ -196,6 +211,8 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
         }
     };
     if (n_first < n_last) fetch(n_first, 0);
+    int checked = 0;
+    if (tid < 3) odd_rows[tid] = 0;
     for (int n = n_first; n < n_last; ++n) {
         const bool masked = n * BN < all_first || (n + 1) * BN > all_last;
         const int stage = (n - n_first) & 1;
@@ -206,21 +223,23 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
         if (n + 1 < n_last) fetch(n + 1, stage ^ 1);
         unsigned long long odd = 0;
         if (masked) {  // what a query does not see must not reach it, but 0 x NaN would
-            if (tid == 0) odd_rows = 0;
-            __syncthreads();
 #pragma unroll
             for (int i = 0; i < LOADS; ++i)
-                if (odd_value<TYPE>(lv[i * 256 + tid])) atomicOr(&odd_rows, 1ull << (i * 256 + tid) / PIECES);
-            __syncthreads();
-            odd = odd_rows;
+                if (odd_value<TYPE>(lv[i * 256 + tid])) atomicOr(&odd_rows[checked], 1ull << (i * 256 + tid) / PIECES);
+            lds_barrier();
+            odd = odd_rows[checked];
             if (odd) {  // (rare) such rows are taken out of the product and added one by one below
 #pragma unroll
                 for (int i = 0; i < LOADS; ++i)
                     if (odd >> (i * 256 + tid) / PIECES & 1) lv[i * 256 + tid] = u32x4{0, 0, 0, 0};
-                __syncthreads();
+                lds_barrier();
             }
+            // (three words in turn: this one has been read by all before the next barrier, and is written again two barriers on)
+            checked = checked == 2 ? 0 : checked + 1;
+            if (tid == 0) odd_rows[checked == 2 ? 0 : checked + 1] = 0;
         }
 
+        if (masked && (n * BN >= w_last || (n + 1) * BN <= w_first)) continue;  // (nothing in it that this wave sees)
         f32x16 sc[2];
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
