@@ -165,7 +165,9 @@ class KVCache4:
                     raise ValueError(f"buffers[{name!r}] must be a contiguous, 16-byte aligned {dtype} tensor {shape} on {self.device}")
             setattr(self, name, t)
         self._failed = torch.zeros(1, dtype=torch.int32, device=self.device)
-        self._c = _lib.KV4(*(t.data_ptr() for t in self.buffers().values()), self._failed.data_ptr(), rows, kv_heads, head_dim, C)
+        pointers = [t.data_ptr() for t in self.buffers().values()]
+        self._pointers = frozenset(pointers)
+        self._c = _lib.KV4(*pointers, self._failed.data_ptr(), rows, kv_heads, head_dim, C)
         self._ref = ctypes.byref(self._c)
         self._work = {}  # (type, heads, tokens, accumulate) -> bytes of an attend call's scratch
 
@@ -259,8 +261,7 @@ class KVCache4:
             raise ValueError("evict moves into another KVCache4")
         if (into.rows, into.kv_heads, into.head_dim, into.device) != (self.rows, self.kv_heads, self.head_dim, self.device):
             raise ValueError("both caches need the same rows, kv_heads, head_dim and device")
-        mine = {t.data_ptr() for t in self.buffers().values()}
-        if any(t.data_ptr() in mine for t in into.buffers().values()):
+        if not self._pointers.isdisjoint(into._pointers):
             raise ValueError("the two caches share buffers")
         if not 1 <= keep <= into.capacity or not 0 <= recent <= keep:
             raise ValueError(f"1 <= keep <= {into.capacity} and 0 <= recent <= keep, got {keep} and {recent}")

@@ -307,6 +307,7 @@ struct AttendArgs {
     float q_sign;     // the scale's sign, on the queries
     float* part_o;    // [pieces][m_rows][D]: a piece is one worker's part of a row and head, number worker + row * H + head
     f32x2* part_ml;   // [pieces][m_rows]: largest score, sum of exponentials to it
+    f32x2* final_ml;  // [rows * H][m_rows]: the same over all pieces, if weights are wanted
     int2* ends;       // [rows * H]: the first and the last piece of a row and head, written by the workers that hold its ends
     float* scores;    // [rows * H][m_rows][C] or nullptr
 };
@@ -657,7 +658,7 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
                 for (int i = 0; i < W; ++i) acc[i] *= inv;
                 const int t = m / a.group, g = m - t * a.group;
                 store_n<W, T>((T*)a.out + (((size_t)r * a.tokens + t) * a.heads + h * a.group + g) * D + d, acc);
-                if (COUNT && (threadIdx.x & 15) == 0) a.part_ml[(size_t)rh * a.m_rows + m] = f32x2{top, sum};
+                if (COUNT && (threadIdx.x & 15) == 0) a.final_ml[(size_t)rh * a.m_rows + m] = f32x2{top, sum};
             }
         }
         return;
@@ -976,12 +977,11 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_ker
     }
 }
 
-// (largest score, sum of exponentials to it) of query m over the pieces of a row and head; the N lanes of a group share them
-template <int N>
+// (largest score, sum of exponentials to it) of query m over the pieces of a row and head, in every lane of the wave
 __device__ __forceinline__ f32x2 join_ml(const AttendArgs& a, int2 p, int m) {
     const f32x2* ml = a.part_ml + m;
     float top = -INFINITY, sum = 0.f;
-    for (int s = p.x + (int)(threadIdx.x % N); s <= p.y; s += N) {
+    for (int s = p.x + (int)(threadIdx.x & 63); s <= p.y; s += 64) {
         const f32x2 x = ml[(size_t)s * a.m_rows];
         const float now = fmaxf(top, x[0]);
         sum = (now == top ? sum : sum * __builtin_amdgcn_exp2f(top - now)) + x[1] * (x[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[0] - now));
@@ -989,10 +989,10 @@ __device__ __forceinline__ f32x2 join_ml(const AttendArgs& a, int2 p, int m) {
     }
     float all = top;
 #pragma unroll
-    for (int o = 1; o < N; o *= 2) all = fmaxf(all, __shfl_xor(all, o));
+    for (int o = 1; o < 64; o *= 2) all = fmaxf(all, __shfl_xor(all, o));
     sum *= top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - all);  // (a sum without a maximum is 0 or NaN)
 #pragma unroll
-    for (int o = 1; o < N; o *= 2) sum += __shfl_xor(sum, o);
+    for (int o = 1; o < 64; o *= 2) sum += __shfl_xor(sum, o);
     return f32x2{all, sum};
 }
 
@@ -1009,8 +1009,10 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttendArgs a) {
     const int2 p = a.ends[rh];  // (an empty row has none: not looked at)
     float acc[W] = {};
     if (row_length(c, r) > 0) {
-        if (p.x == p.y) return;  // (whole: written already)
-        const f32x2 all = join_ml<64>(a, p, m);
+        if (p.x == p.y && !a.final_ml) return;  // (whole: written already)
+        const f32x2 all = join_ml(a, p, m);
+        if (a.final_ml && threadIdx.x == 0) a.final_ml[blockIdx.x] = all;
+        if (p.x == p.y) return;
         const float inv = all[1] == 0.f ? 0.f : 1.f / all[1];
 #pragma unroll 4
         for (int s = p.x + group; s <= p.y; s += 16) {
@@ -1033,38 +1035,35 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttendArgs a) {
     }
 }
 
-// The probabilities that each slot received, from the stored scores: 1024 slots of one row and head.
+// The probabilities that each slot received, from the stored scores: 1024 slots of one row and head, up to 32 queries.
 __global__ __launch_bounds__(256) void kv4_weights_kernel(AttendArgs a, int slot_blocks, float decay) {
     const after_kv4& c = a.c;
     const int rh = blockIdx.x / slot_blocks, r = rh / c.kv_heads;
-    const int len = row_length(c, r), s0 = (blockIdx.x % slot_blocks) * 1024;
-    if (s0 >= len) return;
-    const int2 p = a.workers ? a.ends[rh] : int2{rh, rh};
-    const int s = s0 + 4 * threadIdx.x;
-    __shared__ f32x2 ml[32];
+    const int len = row_length(c, r), s = (blockIdx.x % slot_blocks) * 1024 + 4 * threadIdx.x;
+    if (s >= len) return;
+    const f32x2* ml = a.final_ml + (size_t)rh * a.m_rows;
+    const float* scores = a.scores + (size_t)rh * a.m_rows * c.capacity + s;
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (int m0 = 0; m0 < a.m_rows; m0 += 32) {
-        const int n = min(32, a.m_rows - m0), mine = threadIdx.x >> 3;
-        __syncthreads();
-        if (mine < n) {
-            const f32x2 all = join_ml<8>(a, p, m0 + mine);
-            if ((threadIdx.x & 7) == 0) ml[mine] = f32x2{all[0] == -INFINITY ? 0.f : all[0], all[1] == 0.f ? 0.f : 1.f / all[1]};
-        }
-        __syncthreads();
-        if (s < len) {
-            const float* x4 = a.scores + ((size_t)rh * a.m_rows + m0) * c.capacity + s;
-#pragma unroll 4
-            for (int m = 0; m < n; ++m) {
-                const f32x4 x = *reinterpret_cast<const f32x4*>(x4 + (size_t)m * c.capacity);
+#pragma unroll 8
+    for (int m = 0; m < a.m_rows; ++m) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(scores + (size_t)m * c.capacity);
+        const float top = ml[m][0], off = top == -INFINITY ? 0.f : top, inv = ml[m][1] == 0.f ? 0.f : 1.f / ml[m][1];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[i] += x[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[i] - ml[m][0]) * ml[m][1];
-            }
-        }
+        for (int i = 0; i < 4; ++i) sum[i] += x[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[i] - off) * inv;
     }
     float* w = c.weights + (size_t)rh * c.capacity + s;
+    // (the four slots are inside the capacity; those past the length keep what they hold)
+    if (s + 3 < len) {
+        f32x4 old = {0.f, 0.f, 0.f, 0.f};
+        if (decay != 0.f) old = *reinterpret_cast<const f32x4*>(w);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (s + i < len) w[i] = decay == 0.f ? sum[i] : fmaf(decay, w[i], sum[i]);
+        for (int i = 0; i < 4; ++i) old[i] = decay == 0.f ? sum[i] : fmaf(decay, old[i], sum[i]);
+        *reinterpret_cast<f32x4*>(w) = old;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (s + i < len) w[i] = decay == 0.f ? sum[i] : fmaf(decay, w[i], sum[i]);
+    }
 }
 
 // ... for more than 32 queries: the scores are formed again (68 bytes of keys per slot, where storing and reading 33 scores is
@@ -1081,7 +1080,6 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_wei
     const int rh = blockIdx.x / slot_blocks, r = rh / c.kv_heads, h = rh % c.kv_heads;
     const int len = row_length(c, r), begin = (blockIdx.x % slot_blocks) * slots, end = min(begin + slots, len);
     if (begin >= end) return;
-    const int2 p = a.ends[rh];
     const Widen<D> widen(c, rh);
     Raw<D> raw;
     for (int i = threadIdx.x; i < 4 * kWideSlots; i += 256) sums[i / kWideSlots][i % kWideSlots] = 0.f;
@@ -1092,7 +1090,7 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_wei
         int vis[2];
         load_queries<TYPE, D, NP>(a, r, h, m0, len, qf, vis);
         f32x2 ml = {0.f, 0.f};
-        if (m0 + (lane >> 1) < a.m_rows) ml = join_ml<2>(a, p, m0 + (lane >> 1));
+        if (m0 + (lane & 31) < a.m_rows) ml = a.final_ml[(size_t)rh * a.m_rows + m0 + (lane & 31)];
         float off[2][4], inv[2][4];  // of query 16 nm + 4 kq + i
         int sees[2][4];
 #pragma unroll
@@ -1100,7 +1098,7 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_wei
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int m = nm * 16 + 4 * kq + i;
-                const float top = __shfl(ml[0], 2 * m), sum = __shfl(ml[1], 2 * m);
+                const float top = __shfl(ml[0], m), sum = __shfl(ml[1], m);
                 off[nm][i] = top == -INFINITY ? 0.f : top;
                 inv[nm][i] = sum == 0.f ? 0.f : 1.f / sum;
                 sees[nm][i] = __shfl(vis[nm], 4 * kq + i);
@@ -1336,7 +1334,8 @@ struct Plan {
     int m_rows, nm, mgroups;
     int wgs;     // workgroups of four workers, or 0
     int splits;  // of a row, for more than 32 queries; or 0
-    long long pieces, o_bytes, ml_bytes, s_bytes, e_bytes;
+    long long pieces, o_bytes, ml_bytes, s_bytes, e_bytes, f_bytes;
+    long long total() const { return o_bytes + ml_bytes + s_bytes + e_bytes + f_bytes; }
 };
 Plan attend_plan(const after_kv4& c, int type, int heads, int tokens, bool count) {
     Plan p;
@@ -1358,7 +1357,8 @@ Plan attend_plan(const after_kv4& c, int type, int heads, int tokens, bool count
     }
     p.pieces = p.splits ? n_rh * p.splits : 4ll * p.wgs + n_rh;
     p.o_bytes = p.wgs || p.splits > 1 ? p.pieces * p.m_rows * c.head_dim * 4 : 0;
-    p.ml_bytes = p.wgs || p.splits || count ? (p.pieces * p.m_rows * 8 + 255) / 256 * 256 : 0;
+    p.ml_bytes = p.wgs || p.splits ? (p.pieces * p.m_rows * 8 + 255) / 256 * 256 : 0;
+    p.f_bytes = count ? (n_rh * p.m_rows * 8 + 255) / 256 * 256 : 0;
     p.s_bytes = count && !p.splits ? n_rh * p.m_rows * c.capacity * 4 : 0;
     p.e_bytes = p.wgs || p.splits ? (n_rh * 8 + 255) / 256 * 256 : 0;
     return p;
@@ -1508,7 +1508,7 @@ extern "C" int after_kv4_attend_workspace(const after_kv4* c, int type, int head
     AFTER_TRY(check_attend(c, type, heads, tokens, "kv4_attend_workspace"));
     AFTER_REQUIRE(bytes, AFTER_E_INVALID, "kv4_attend_workspace: bytes is NULL");
     const Plan p = attend_plan(*c, type, heads, tokens, accumulate != 0);
-    *bytes = p.o_bytes + p.ml_bytes + p.s_bytes + p.e_bytes;
+    *bytes = p.total();
     return AFTER_OK;
 }
 
@@ -1522,7 +1522,7 @@ extern "C" int after_kv4_attend(const after_kv4* c, const void* q, void* out, in
     AFTER_REQUIRE(std::isfinite(scale) && std::isfinite(decay), AFTER_E_INVALID, "kv4_attend: scale and decay must be finite");
     const bool count = accumulate != 0;
     const Plan p = attend_plan(*c, type, heads, tokens, count);
-    const long long need = p.o_bytes + p.ml_bytes + p.s_bytes + p.e_bytes;
+    const long long need = p.total();
     AFTER_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need), AFTER_E_CAPACITY,
                   "kv4_attend: needs a 16-byte aligned workspace of %lld bytes (got %lld)", need, workspace_bytes);
     AttendArgs a;
@@ -1540,10 +1540,11 @@ extern "C" int after_kv4_attend(const after_kv4* c, const void* q, void* out, in
     a.scale2 = std::fmax(std::fabs(scale) * 1.44269504088896340736f, 1e-30f);
     a.q_sign = scale < 0 ? -1.f : 1.f;
     char* w = (char*)workspace;
-    a.scores = count ? (float*)w : nullptr;
-    a.part_ml = (f32x2*)(w + p.s_bytes);
-    a.ends = (int2*)(w + p.s_bytes + p.ml_bytes);
-    a.part_o = (float*)(w + p.s_bytes + p.ml_bytes + p.e_bytes);
+    a.scores = (float*)w;
+    a.part_ml = (f32x2*)(w += p.s_bytes);
+    a.final_ml = count ? (f32x2*)(w + p.ml_bytes) : nullptr;
+    a.ends = (int2*)(w += p.ml_bytes + p.f_bytes);
+    a.part_o = (float*)(w += p.e_bytes);
 #define CALL(T, D) return run_attend<T, D>(a, p, count, decay, (hipStream_t)stream)
     KV4_BY_TYPE(type, c->head_dim, CALL);
 #undef CALL
