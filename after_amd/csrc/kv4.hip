@@ -1157,7 +1157,7 @@ constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
 // and where from the top its sums pass `want`.  Then each wave looks through a sixteenth of the slots: once to count what stays,
 // and, knowing what the waves before it keep, once to write them: those above the value, and the first `want` equal to it.
 __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(after_kv4 c, int keep, int recent, int* slots) {
-    __shared__ int hist[2048][4];
+    __shared__ int4 hist[2048];
     __shared__ int tmp[kSelWaves][2];
     __shared__ int found[2];
     const int rh = blockIdx.x, r = rh / c.kv_heads, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -1174,33 +1174,37 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(after_kv4 c, in
     unsigned prefix = 0xFFFFFFFFu;  // (want = 0: nothing is above, and nothing that is equal is wanted)
     if (want > 0) {
         prefix = 0;
+        constexpr int SPAN = 16 * kSelThreads;  // weights held in registers: a row of up to 16384 is read once
+        f32x4 x[4];
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, bins = 1 << bits;
-            for (int i = tid; i < bins * 4; i += kSelThreads) hist[i >> 2][i & 3] = 0;
+            for (int i = tid; i < bins; i += kSelThreads) hist[i] = int4{0, 0, 0, 0};
             __syncthreads();
-            auto add = [&](float x) {
-                const unsigned k = order_key(x);
-                if (pass == 0 || (k >> (shift + bits)) == (prefix >> (shift + bits))) atomicAdd(&hist[k >> shift & (bins - 1)][lane & 3], 1);
-            };
-            // (rows of weights begin and end at multiples of 128 bytes)
-            for (int i = 4 * tid; i < old; i += 16 * kSelThreads) {
-                f32x4 x[4];
+            for (int i0 = 0; i0 < old; i0 += SPAN) {
+                const int i = i0 + 4 * tid;  // (rows of weights begin and end at multiples of 128 bytes)
+                if (pass == 0 || old > SPAN) {
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (i + u * 4 * kSelThreads < old) x[u] = *reinterpret_cast<const f32x4*>(w + i + u * 4 * kSelThreads);
+                    for (int u = 0; u < 4; ++u)
+                        if (i + u * 4 * kSelThreads < old) x[u] = *reinterpret_cast<const f32x4*>(w + i + u * 4 * kSelThreads);
+                }
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
+                for (int u = 0; u < 4; ++u) {
+                    if (i0 + u * 4 * kSelThreads >= old) break;  // (uniform)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (i + u * 4 * kSelThreads + j < old) add(x[u][j]);
+                    for (int j = 0; j < 4; ++j) {
+                        const unsigned k = order_key(x[u][j]);
+                        if (i + u * 4 * kSelThreads + j < old && (pass == 0 || (k >> (shift + bits)) == (prefix >> (shift + bits))))
+                            atomicAdd(reinterpret_cast<int*>(hist) + (k >> shift & (bins - 1)) * 4 + (lane & 3), 1);
+                    }
+                }
             }
             __syncthreads();
             // thread t looks at two bins (one, in the last pass), from the top
             const int per = bins / kSelThreads;
             int mine = 0, bin_sum[2] = {0, 0};
             for (int j = 0; j < per; ++j) {
-                const int bin = bins - 1 - (tid * per + j);
-                bin_sum[j] = (hist[bin][0] + hist[bin][1]) + (hist[bin][2] + hist[bin][3]);
+                const int4 n = hist[bins - 1 - (tid * per + j)];
+                bin_sum[j] = (n.x + n.y) + (n.z + n.w);
                 mine += bin_sum[j];
             }
             int upto = mine;
@@ -1219,19 +1223,24 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(after_kv4 c, in
             }
             __syncthreads();
             prefix |= (unsigned)found[0] << shift;
-            want = found[1];  // of those equal to the prefix so far
-            __syncthreads();
+            want = found[1];  // of those equal to the prefix so far (the next write of `found` is three barriers on)
         }
     }
+    // a sixteenth of the slots for each wave; up to 512 of them stay in registers between the two looks
+    constexpr int U = 8;
     const int per = (len + kSelThreads - 1) / kSelThreads * 64, begin = wave * per, end = min(begin + per, len);
-    constexpr int U = 8;  // loads on their way at a time
+    unsigned k[U];
+    auto look = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * 64 < end) k[u] = i0 + u * 64 + lane < end ? order_key(w[i0 + u * 64 + lane]) : 0u;
+    };
     int above = 0, equal = 0;
     for (int i0 = begin; i0 < end; i0 += U * 64) {
-        unsigned k[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) k[u] = i0 + u * 64 + lane < end ? order_key(w[i0 + u * 64 + lane]) : 0u;
+        look(i0);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+            if (i0 + u * 64 >= end) break;  // (uniform)
             const int i = i0 + u * 64 + lane;
             above += __popcll(__ballot(i < end && (i >= old || k[u] > prefix)));
             equal += __popcll(__ballot(i < min(end, old) && k[u] == prefix));
@@ -1250,11 +1259,10 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(after_kv4 c, in
     done += min(equal_done, want);
     const unsigned long long before = (1ull << lane) - 1;
     for (int i0 = begin; i0 < end; i0 += U * 64) {
-        unsigned k[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) k[u] = i0 + u * 64 + lane < end ? order_key(w[i0 + u * 64 + lane]) : 0u;
+        if (per > U * 64) look(i0);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+            if (i0 + u * 64 >= end) break;  // (uniform)
             const int i = i0 + u * 64 + lane;
             const unsigned long long eq = __ballot(i < min(end, old) && k[u] == prefix);
             const bool is_equal = eq >> lane & 1, stay = i < end && (i >= old || k[u] > prefix || (is_equal && equal_done + __popcll(eq & before) < want));
