@@ -1174,8 +1174,8 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(after_kv4 c, in
     unsigned prefix = 0xFFFFFFFFu;  // (want = 0: nothing is above, and nothing that is equal is wanted)
     if (want > 0) {
         prefix = 0;
-        constexpr int SPAN = 16 * kSelThreads;  // weights held in registers: a row of up to 16384 is read once
-        f32x4 x[4];
+        constexpr int SPAN = 32 * kSelThreads;  // weights held in registers: a row of up to 32768 is read once
+        f32x4 x[8];
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, bins = 1 << bits;
             for (int i = tid; i < bins; i += kSelThreads) hist[i] = int4{0, 0, 0, 0};
@@ -1184,11 +1184,11 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(after_kv4 c, in
                 const int i = i0 + 4 * tid;  // (rows of weights begin and end at multiples of 128 bytes)
                 if (pass == 0 || old > SPAN) {
 #pragma unroll
-                    for (int u = 0; u < 4; ++u)
+                    for (int u = 0; u < 8; ++u)
                         if (i + u * 4 * kSelThreads < old) x[u] = *reinterpret_cast<const f32x4*>(w + i + u * 4 * kSelThreads);
                 }
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
+                for (int u = 0; u < 8; ++u) {
                     if (i0 + u * 4 * kSelThreads >= old) break;  // (uniform)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -1226,8 +1226,8 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(after_kv4 c, in
             want = found[1];  // of those equal to the prefix so far (the next write of `found` is three barriers on)
         }
     }
-    // a sixteenth of the slots for each wave; up to 512 of them stay in registers between the two looks
-    constexpr int U = 8;
+    // a sixteenth of the slots for each wave; up to 2048 of them stay in registers between the two looks
+    constexpr int U = 32;
     const int per = (len + kSelThreads - 1) / kSelThreads * 64, begin = wave * per, end = min(begin + per, len);
     unsigned k[U];
     auto look = [&](int i0) {
