@@ -47,33 +47,48 @@ struct Elem<AFTER_T_F16> {
     static __device__ __forceinline__ f32x16 mfma(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 
+// n / d for 0 <= n < 2^31 by a product (d is the same for all: found on the host)
+struct Divisor {
+    unsigned d, magic, shift;
+    __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi((unsigned)n, magic) + (unsigned)n) >> shift); }
+};
+Divisor divisor(unsigned d) {
+    unsigned shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    return Divisor{d, (unsigned)((((1ull << shift) - d) << 32) / d + 1), shift};
+}
+
 struct PackedArgs {
     const void *q, *k, *v;
     void* out;
     const int *qs, *ks;
     long long qts, qhs, kts, khs, vts, vhs, ots, ohs;
     int q_rows, k_rows, n_seqs, heads, kv_heads, group, tiles;
+    Divisor by_group, by_chunk, by_kv_heads;
     float scale2;     // |scale| log2 e, > 0 (a masked score, -inf, stays -inf)
     unsigned q_sign;  // the sign bits of a word of q, if scale is negative
-    int causal, window, chunk, zero_rest;
+    int causal, window, zero_rest;
 };
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
 
 // Sequence b of the queries begins at row ...; one more "sequence" without keys stands for the rows behind the last
 __device__ __forceinline__ int q_start(const PackedArgs& a, int b) {
-    return b <= 0 ? 0 : b > a.n_seqs ? a.q_rows : clampi(a.qs[b], 0, a.q_rows);
+    const int x = a.qs[min(b, a.n_seqs)];
+    return b <= 0 ? 0 : b > a.n_seqs ? a.q_rows : clampi(x, 0, a.q_rows);
+}
+__device__ __forceinline__ int k_start(const PackedArgs& a, int b) {
+    const int x = a.ks[min(b, a.n_seqs)];
+    return b <= 0 ? 0 : clampi(x, 0, a.k_rows);
 }
 
-// [first, last) of the keys that the query at position p of its sequence sees
+// [first, last) of the keys that the query at position p of its sequence sees (a query older than the keys: p < 0, none)
 __device__ __forceinline__ void seen(const PackedArgs& a, int p, int keys, int& first, int& last) {
     first = 0;
     last = keys;
     if (a.causal) {
-        // (floor: a query older than the keys has a negative position)
-        const int q = p >= 0 ? p / a.chunk : -((a.chunk - 1 - p) / a.chunk);
-        const int begin = q * a.chunk;
-        last = clampi(begin + a.chunk, 0, keys);
+        const int chunk = (int)a.by_chunk.d, begin = a.by_chunk(max(p, 0)) * chunk;
+        last = p < 0 ? 0 : min(begin + chunk, keys);
         if (a.window > 0) first = max(0, min(begin, p - a.window + 1));
     }
 }
@@ -125,44 +140,46 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, half = lane >> 5;
     // neighbouring workgroups are dispatched to different XCDs: a key head's workgroups stay on one L2 where there are eight.
     // Tiles from the last to the first: with a causal mask the longest first.
-    const int h = blockIdx.x % a.kv_heads, tile = a.tiles - 1 - blockIdx.x / a.kv_heads;
-    // the last sequence that begins at or before this tile: 64 candidates at a time
-    int lo = 0, hi = a.n_seqs;
-    while (lo < hi) {
-        const int step = (hi - lo + 64) / 64, at = min(lo + lane * step, hi);
-        const bool begun = (int)((long long)q_start(a, at) * a.group / BM) + at <= tile;
-        const unsigned long long all = __ballot(begun && lo + lane * step <= hi) | 1;  // (sequence lo has begun)
-        lo += (63 - __clzll(all)) * step;
+    const int back = a.by_kv_heads(blockIdx.x), h = blockIdx.x - back * a.kv_heads, tile = a.tiles - 1 - back;
+    // the last sequence that begins at or before this tile: 64 candidates at a time; the last look holds its ends
+    int lo = 0, hi = a.n_seqs, b, q0, q1, k0, k1;
+    for (;;) {
+        const int step = (hi - lo + 64) >> 6, at = lo + lane * step, qs = q_start(a, at), ks = k_start(a, at);
+        const bool begun = (int)((long long)qs * a.group / BM) + at <= tile;
+        const int j = 63 - __clzll(__ballot(begun && at <= hi) | 1);  // (sequence lo has begun)
+        if (step == 1) {
+            b = lo + j;
+            q0 = __builtin_amdgcn_readlane(qs, j);
+            k0 = __builtin_amdgcn_readlane(ks, j);
+            q1 = j < 63 ? __builtin_amdgcn_readlane(qs, (j + 1) & 63) : q_start(a, b + 1);
+            k1 = j < 63 ? __builtin_amdgcn_readlane(ks, (j + 1) & 63) : k_start(a, b + 1);
+            break;
+        }
+        lo += j * step;
         hi = min(hi, lo + step - 1);
     }
-    const int b = lo, q0 = q_start(a, b), nq = q_start(a, b + 1) - q0;
-    const int row0 = (tile - ((int)((long long)q0 * a.group / BM) + b)) * BM;
+    const int nq = q1 - q0, row0 = (tile - ((int)((long long)q0 * a.group / BM) + b)) * BM;
     const int rows = nq * a.group;  // (< 2^31: checked on the host)
-    if (row0 < 0 || row0 >= rows) return;
-    int k0 = 0, nk = 0;
-    if (b < a.n_seqs) {
-        k0 = b == 0 ? 0 : clampi(a.ks[b], 0, a.k_rows);
-        nk = max(clampi(a.ks[b + 1], 0, a.k_rows) - k0, 0);
-    } else if (!a.zero_rest)
-        return;
+    if (row0 < 0 || row0 >= rows || (b == a.n_seqs && !a.zero_rest)) return;
+    const int nk = b < a.n_seqs ? max(k1 - k0, 0) : 0;
 
     // this lane's query, and the keys that it and its workgroup see
-    const int row = row0 + wave * 32 + l31, t = min(row, rows - 1) / a.group, g = min(row, rows - 1) - t * a.group;
+    const int row = row0 + wave * 32 + l31, t = a.by_group(min(row, rows - 1)), g = min(row, rows - 1) - t * a.group;
     int first, last, t_first, t_last, dummy;
     seen(a, t + nk - nq, nk, first, last);
-    seen(a, row0 / a.group + nk - nq, nk, t_first, dummy);
-    seen(a, (min(row0 + BM, rows) - 1) / a.group + nk - nq, nk, dummy, t_last);
+    seen(a, a.by_group(row0) + nk - nq, nk, t_first, dummy);
+    seen(a, a.by_group(min(row0 + BM, rows) - 1) + nk - nq, nk, dummy, t_last);
     // the keys that some query of the wave sees
     int w_first = 0, w_last = 0;
     const int w_row = __builtin_amdgcn_readfirstlane(row0 + wave * 32);
     if (w_row < rows) {
-        seen(a, w_row / a.group + nk - nq, nk, w_first, dummy);
-        seen(a, (min(w_row + 32, rows) - 1) / a.group + nk - nq, nk, dummy, w_last);
+        seen(a, a.by_group(w_row) + nk - nq, nk, w_first, dummy);
+        seen(a, a.by_group(min(w_row + 32, rows) - 1) + nk - nq, nk, dummy, w_last);
     }
     // every query of the workgroup sees [all_first, all_last)
     int all_first, all_last;
-    seen(a, row0 / a.group + nk - nq, nk, dummy, all_last);
-    seen(a, (min(row0 + BM, rows) - 1) / a.group + nk - nq, nk, all_first, dummy);
+    seen(a, a.by_group(row0) + nk - nq, nk, dummy, all_last);
+    seen(a, a.by_group(min(row0 + BM, rows) - 1) + nk - nq, nk, all_first, dummy);
 
     const T* qp = (const T*)a.q + (long long)(q0 + t) * a.qts + (long long)(h * a.group + g) * a.qhs;
     const T* kp = (const T*)a.k + (long long)k0 * a.kts + (long long)h * a.khs;
@@ -346,10 +363,12 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
         }
     }
 
+    // to memory by way of LDS: a lane holds one row's every eighth group of four channels, a store of whole rows takes half the time
     l += __shfl_xor(l, 32);
-    if (row >= rows) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* op = (T*)a.out + (long long)(q0 + t) * a.ots + (long long)(h * a.group + g) * a.ohs;
+    constexpr int PITCH = D * (int)sizeof(T) + 16;
+    char* mine = lds + wave * (32 * PITCH);
+    lds_barrier();  // (the tiles are no longer read)
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -358,13 +377,22 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
             T4 y;
 #pragma unroll
             for (int w = 0; w < 4; ++w) y[w] = (T)(o[i][e + w] * inv);
-            *reinterpret_cast<T4*>(op + 32 * i + 2 * e + 4 * half) = y;
+            *reinterpret_cast<T4*>(mine + l31 * PITCH + (32 * i + 2 * e + 4 * half) * sizeof(T)) = y;
         }
+#pragma unroll
+    for (int i = 0; i < 32 * PIECES / 64; ++i) {
+        const int id = i * 64 + lane, r = id / PIECES, c = id % PIECES, at = row0 + wave * 32 + r;
+        if (at < rows) {
+            const int tr = a.by_group(at), gr = at - tr * a.group;
+            *reinterpret_cast<u32x4*>((T*)a.out + (long long)(q0 + tr) * a.ots + (long long)(h * a.group + gr) * a.ohs + c * (16 / (int)sizeof(T))) =
+                *reinterpret_cast<const u32x4*>(mine + r * PITCH + c * 16);
+        }
+    }
 }
 
 template <int TYPE, int D>
 int run_packed(const PackedArgs& a, hipStream_t s) {
-    constexpr size_t lds = 4 * BN * D * sizeof(typename Elem<TYPE>::T);
+    constexpr size_t tiles = 4 * BN * D * sizeof(typename Elem<TYPE>::T), out = 4 * 32 * (D * sizeof(typename Elem<TYPE>::T) + 16), lds = tiles > out ? tiles : out;
     static LdsAttr attr;
     AFTER_TRY(ensure_lds_attr(attr, (const void*)attend_packed_kernel<TYPE, D>, lds));
     hipLaunchKernelGGL((attend_packed_kernel<TYPE, D>), dim3((unsigned)a.tiles * a.kv_heads), dim3(256), lds, s, a);
@@ -409,7 +437,8 @@ extern "C" int after_attend_packed(const void* q, const void* k, const void* v, 
     a.tiles = (int)(q_rows * group / BM) + n_seqs + 1;
     a.scale2 = std::fmax(std::fabs(scale) * 1.44269504088896340736f, 1e-30f);
     a.q_sign = scale < 0 ? (type == AFTER_T_F32 ? 0x80000000u : 0x80008000u) : 0u;
-    a.causal = causal != 0, a.window = window < (1 << 30) ? window : 1 << 30, a.chunk = chunk, a.zero_rest = zero_rest;
+    a.causal = causal != 0, a.window = window < (1 << 30) ? window : 1 << 30, a.zero_rest = zero_rest;
+    a.by_group = divisor(group), a.by_chunk = divisor(chunk), a.by_kv_heads = divisor(kv_heads);
     AFTER_REQUIRE((long long)a.tiles * kv_heads < (1ll << 31), AFTER_E_INVALID, "attend_packed: too many tokens x heads for one call");
     hipStream_t s = (hipStream_t)stream;
     if (head_dim == 64) {
