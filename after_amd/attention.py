@@ -15,6 +15,7 @@ hand-written HIP kernels behind the C ABI of include/after_hip.h, no fallback.
 """
 import ctypes
 import math
+import weakref
 
 import torch
 
@@ -131,7 +132,8 @@ class KVCache4:
 
     The state is six tensors of the object -- `keys`, `key_scales`, `values`, `value_scales` (uint8), `weights` (fp32
     [rows, kv_heads, capacity]: attention received, summed up by `attend(accumulate=True)`), `lengths` (int32 [rows]: slots in
-    use) -- which `buffers()` returns and `KVCache4(..., buffers=...)` takes over as they are.
+    use) -- which `buffers()` returns and `KVCache4(..., buffers=...)` takes over as they are.  They can be written in place, not
+    replaced.
 
     Every call enqueues on the current stream, never synchronises and can be captured into a graph; the lengths live on the
     device.  One call at a time works on a cache: order calls on different streams with events, as for any tensor."""
@@ -155,6 +157,7 @@ class KVCache4:
                       weights=((rows, kv_heads, C), torch.float32), lengths=((rows, ), torch.int32))
         if buffers is not None and set(buffers) != set(layout):
             raise ValueError(f"buffers must hold {sorted(layout)}, got {sorted(buffers)}")
+        tensors = {}
         for name, (shape, dtype) in layout.items():
             if buffers is None:
                 t = torch.zeros(shape, dtype=dtype, device=self.device)
@@ -163,18 +166,24 @@ class KVCache4:
                 if not isinstance(t, torch.Tensor) or tuple(t.shape) != shape or t.dtype != dtype or t.device != self.device \
                         or not t.is_contiguous() or t.data_ptr() % 16:
                     raise ValueError(f"buffers[{name!r}] must be a contiguous, 16-byte aligned {dtype} tensor {shape} on {self.device}")
-            setattr(self, name, t)
+            tensors[name] = t
         self._failed = torch.zeros(1, dtype=torch.int32, device=self.device)
-        pointers = [t.data_ptr() for t in self.buffers().values()]
-        self._pointers = frozenset(pointers)
-        self._c = _lib.KV4(*pointers, self._failed.data_ptr(), rows, kv_heads, head_dim, C)
+        self._tensors = tensors  # (their addresses are in _c: the attributes cannot be set to others)
+        self._evicted_into = None
+        self._c = _lib.KV4(*(t.data_ptr() for t in tensors.values()), self._failed.data_ptr(), rows, kv_heads, head_dim, C)
         self._ref = ctypes.byref(self._c)
         self._work = {}  # (type, heads, tokens, accumulate) -> bytes of an attend call's scratch
 
+    keys = property(lambda self: self._tensors["keys"])
+    key_scales = property(lambda self: self._tensors["key_scales"])
+    values = property(lambda self: self._tensors["values"])
+    value_scales = property(lambda self: self._tensors["value_scales"])
+    weights = property(lambda self: self._tensors["weights"])
+    lengths = property(lambda self: self._tensors["lengths"])
+
     def buffers(self):
         """The six tensors of the state, by name."""
-        return dict(keys=self.keys, key_scales=self.key_scales, values=self.values, value_scales=self.value_scales,
-                    weights=self.weights, lengths=self.lengths)
+        return dict(self._tensors)
 
     def _row_values(self, t, name):
         if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != (self.rows, ) or t.device != self.device:
@@ -259,10 +268,13 @@ class KVCache4:
         keep, recent = int(keep), int(recent)
         if not isinstance(into, KVCache4) or into is self:
             raise ValueError("evict moves into another KVCache4")
-        if (into.rows, into.kv_heads, into.head_dim, into.device) != (self.rows, self.kv_heads, self.head_dim, self.device):
-            raise ValueError("both caches need the same rows, kv_heads, head_dim and device")
-        if not self._pointers.isdisjoint(into._pointers):
-            raise ValueError("the two caches share buffers")
+        if self._evicted_into is None or self._evicted_into() is not into:
+            if (into.rows, into.kv_heads, into.head_dim, into.device) != (self.rows, self.kv_heads, self.head_dim, self.device):
+                raise ValueError("both caches need the same rows, kv_heads, head_dim and device")
+            ranges = [[(t.data_ptr(), t.data_ptr() + t.nbytes) for t in c.buffers().values()] for c in (self, into)]
+            if any(a < d and b < e for a, e in ranges[0] for b, d in ranges[1]):
+                raise ValueError("the two caches share memory")
+            self._evicted_into = weakref.ref(into)  # (looked at once)
         if not 1 <= keep <= into.capacity or not 0 <= recent <= keep:
             raise ValueError(f"1 <= keep <= {into.capacity} and 0 <= recent <= keep, got {keep} and {recent}")
         slots = torch.empty(self.rows, self.kv_heads, keep, dtype=torch.int32, device=self.device)
@@ -270,7 +282,7 @@ class KVCache4:
         return slots
 
     def check(self):
-        """Waits for the work on this cache and raises AFTERHipError if an append has dropped tokens since the last look."""
+        """Waits for the current stream and raises AFTERHipError if an append has dropped tokens since the last look."""
         if int(self._failed.item()):
             self._failed.zero_()
             raise _lib.AFTERHipError(f"KVCache4.append: a row had no room for all of its new tokens ({self.capacity} slots)")

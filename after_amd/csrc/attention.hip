@@ -439,7 +439,8 @@ extern "C" int after_attend_packed(const void* q, const void* k, const void* v, 
     a.q_sign = scale < 0 ? (type == AFTER_T_F32 ? 0x80000000u : 0x80008000u) : 0u;
     a.causal = causal != 0, a.window = window < (1 << 30) ? window : 1 << 30, a.zero_rest = zero_rest;
     a.by_group = divisor(group), a.by_chunk = divisor(chunk), a.by_kv_heads = divisor(kv_heads);
-    AFTER_REQUIRE((long long)a.tiles * kv_heads < (1ll << 31), AFTER_E_INVALID, "attend_packed: too many tokens x heads for one call");
+    // (a grid's threads are counted in 32 bits)
+    AFTER_REQUIRE((long long)a.tiles * kv_heads < (1 << 24), AFTER_E_INVALID, "attend_packed: too many tokens x heads for one call");
     hipStream_t s = (hipStream_t)stream;
     if (head_dim == 64) {
         if (type == AFTER_T_F32) return run_packed<AFTER_T_F32, 64>(a, s);

@@ -199,18 +199,24 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, int r, int h, 
 template <int TYPE, int D>
 __global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a, int items) {
     const after_kv4& c = a.c;
-    const int item = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (item >= items) return;
-    const int h = item % c.kv_heads, fb = item / c.kv_heads;
-    int lo = 0, hi = c.rows - 1;  // the last row that begins at or before fb
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (a.nt.start(mid) / 8 + 2 * mid <= fb)
-            lo = mid;
-        else
-            hi = mid - 1;
+    const int h = item % c.kv_heads, fb = item / c.kv_heads, lane = threadIdx.x & 63;
+    // the last row that begins at or before fb: 64 candidates at a time; the last look holds its tokens and length
+    int lo = 0, hi = c.rows - 1, r, t0, n, len;
+    for (;;) {
+        const int step = (hi - lo + 64) >> 6, at = min(lo + lane * step, hi), t = a.nt.start(at), next = a.nt.start(at + 1), l = row_length(c, at);
+        const int j = 63 - __clzll(__ballot(t / 8 + 2 * at <= fb && lo + lane * step <= hi) | 1);
+        if (step == 1) {
+            r = lo + j;
+            t0 = __builtin_amdgcn_readlane(t, j);
+            n = __builtin_amdgcn_readlane(next, j) - t0;
+            len = __builtin_amdgcn_readlane(l, j);
+            break;
+        }
+        lo += j * step;
+        hi = min(hi, lo + step - 1);
     }
-    const int r = lo, t0 = a.nt.start(r), n = a.nt.start(r + 1) - t0, len = row_length(c, r);
     const int sb = len / 8 + fb - (t0 / 8 + 2 * r), end = min(len + max(n, 0), c.capacity);  // tokens that do not fit are dropped
     if (sb >= 0 && 8 * sb < end) append_block<TYPE, D>(a, r, h, t0, len, end, sb);
 }
@@ -1334,6 +1340,8 @@ int check_cache(const after_kv4* c, const char* what) {
     AFTER_REQUIRE((long long)c->rows * c->kv_heads <= (1 << 20), AFTER_E_INVALID, "%s: rows x kv_heads is at most 2^20", what);
     return AFTER_OK;
 }
+// (a grid's threads are counted in 32 bits: at most 2^24 - 1 workgroups of 256)
+constexpr long long kMaxGroups = (1 << 24) - 1;
 bool known_type(int t) { return t == AFTER_T_F32 || t == AFTER_T_BF16 || t == AFTER_T_F16; }
 int type_bytes(int t) { return t == AFTER_T_F32 ? 4 : 2; }
 bool aligned16(const void* p) { return ((size_t)p & 15) == 0; }
@@ -1453,7 +1461,7 @@ extern "C" int after_kv4_append(const after_kv4* c, const void* k, const void* v
     hipStream_t s = (hipStream_t)stream;
     const NewTokens nt{starts, tokens, (int)total};
     const long long items = (total / 8 + 2ll * c->rows) * c->kv_heads;
-    AFTER_REQUIRE(items < (1ll << 31), AFTER_E_INVALID, "kv4_append: too many new tokens x heads for one call");
+    AFTER_REQUIRE(cdivll(items, 4) <= kMaxGroups, AFTER_E_INVALID, "kv4_append: too many new tokens x heads for one call");
     const AppendArgs a{*c, nt, k, v, k_token_stride, k_head_stride, v_token_stride, v_head_stride};
     // A workgroup per row where no row can have many: 64 rows of one token each in one launch.  (`starts` may give all to one row.)
     if (starts ? total <= 2ll * c->rows && total <= 256 : tokens <= 16) {
@@ -1485,7 +1493,7 @@ extern "C" int after_kv4_read(const after_kv4* c, void* k, void* v, int type, co
     AFTER_REQUIRE(k && v && aligned16(k) && aligned16(v), AFTER_E_INVALID, "kv4_read: k and v must be 16-byte aligned");
     const int nb = count / 8 + 2;
     const long long items = (long long)c->rows * c->kv_heads * nb;
-    AFTER_REQUIRE(items < (1ll << 32), AFTER_E_INVALID, "kv4_read: too many slots x heads for one call");
+    AFTER_REQUIRE(cdivll(items, 4) <= kMaxGroups, AFTER_E_INVALID, "kv4_read: too many slots x heads for one call");
 #define CALL(T, D) \
     hipLaunchKernelGGL((kv4_read_kernel<T, D>), dim3((unsigned)cdivll(items, 4)), dim3(256), 0, (hipStream_t)stream, *c, k, v, start, count, nb, items)
     if (c->head_dim == 64) {
@@ -1507,7 +1515,9 @@ static int check_attend(const after_kv4* c, int type, int heads, int tokens, con
     AFTER_REQUIRE(tokens > 0 && (long long)tokens * (heads / c->kv_heads) <= 65536, AFTER_E_INVALID, "%s: 1 .. 65536 / (heads / kv_heads) tokens (got %d)",
                   what, tokens);
     const Plan p = attend_plan(*c, type, heads, tokens, false);
-    AFTER_REQUIRE(p.pieces * p.mgroups < (1ll << 30) && (long long)c->rows * c->kv_heads * p.m_rows < (1ll << 31) && (long long)c->rows * c->kv_heads * cdiv(c->capacity, 256) < (1ll << 31),
+    const long long n_rh = (long long)c->rows * c->kv_heads;
+    AFTER_REQUIRE((p.splits ? n_rh * p.splits + 8 : n_rh) * p.mgroups <= kMaxGroups && n_rh * p.m_rows <= kMaxGroups &&
+                      n_rh * cdiv(c->capacity, 256) <= kMaxGroups,
                   AFTER_E_INVALID, "%s: too many rows x heads x tokens for one call", what);
     return AFTER_OK;
 }
@@ -1571,7 +1581,7 @@ extern "C" int after_kv4_evict(const after_kv4* c, const after_kv4* to, int keep
     hipStream_t s = (hipStream_t)stream;
     const int n_rh = c->rows * c->kv_heads, nb = cdiv(keep, 8);
     const long long items = (long long)n_rh * nb;
-    AFTER_REQUIRE(items < (1ll << 32), AFTER_E_INVALID, "kv4_evict: too many slots x heads for one call");
+    AFTER_REQUIRE(cdivll(items, 4) <= kMaxGroups && n_rh <= kMaxGroups / 4, AFTER_E_INVALID, "kv4_evict: too many slots x heads for one call");
     hipLaunchKernelGGL(kv4_select_kernel, dim3(n_rh), dim3(kSelThreads), 0, s, *c, keep, recent, slots);
     if (c->head_dim == 64)
         hipLaunchKernelGGL((kv4_move_kernel<64>), dim3((unsigned)cdivll(items, 4)), dim3(256), 0, s, *c, *to, keep, slots, nb, items);

@@ -77,6 +77,18 @@ def test_cache_calls_refuse():
         assert L.after_kv4_evict(c, ctypes.byref(cache(keys=P + (1 << 19), lengths=P + 64, **k)), 8, 0, P, None) == E_INVALID
 
 
+def test_grids_that_would_not_fit_are_refused():
+    """A grid's threads are counted in 32 bits."""
+    L, n = _lib.lib(), ctypes.c_longlong()
+    big = dict(rows=1 << 14, kv_heads=1 << 6, capacity=1 << 20)
+    c = ctypes.byref(cache(**big))
+    assert L.after_kv4_read(c, P, P, 1, None, 1 << 20, None) == E_INVALID and "too many" in error()
+    assert L.after_kv4_append(c, P, P, 1, None, 512, 512 << 14, 4096, 64, 4096, 64, None) == E_INVALID and "too many" in error()
+    assert L.after_kv4_evict(c, ctypes.byref(cache(keys=P + (1 << 19), lengths=P + 64, **big)), 1 << 20, 0, P, None) == E_INVALID and "too many" in error()
+    assert L.after_kv4_attend_workspace(c, 1, 64, 1, 0, ctypes.byref(n)) == E_INVALID and "too many" in error()
+    assert packed(q_rows=(1 << 30) - 1, kv=1 << 20, heads=1 << 20) == E_INVALID and "too many" in error()
+
+
 def test_attend_refuses():
     L, c, n = _lib.lib(), ctypes.byref(cache(capacity=4096)), ctypes.c_longlong()
     for heads, tokens in ((3, 1), (0, 1), (4, 0), (4, -1), (4, 32769)):

@@ -367,8 +367,13 @@ def test_strided_queries_and_refusals(hip_device):
     for a in ((c, 8), (other, 33), (other, 0), (other, 8, 9), (KVCache4(2, 1, 64, 32, hip_device), 8), (KVCache4(2, 2, 64, 64, hip_device, c.buffers()), 8)):
         with pytest.raises(ValueError):
             c.evict(*a)
+    part = dict(other.buffers(), weights=c.weights.view(-1)[128:256].view(2, 2, 32))  # memory of c in the middle of one of its buffers
+    with pytest.raises(ValueError):
+        c.evict(KVCache4(2, 2, 64, 32, hip_device, part), 8)
     with pytest.raises(ValueError):
         KVCache4(2, 2, 64, 96, hip_device, c.buffers())
+    with pytest.raises(AttributeError):  # the kernels would go on with the old one
+        c.lengths = c.lengths + 1
     q = torch.zeros(4, 2, 64, device=hip_device)
     s = starts([4], hip_device)
     for bad in (dict(q_starts=s.long()), dict(k_starts=starts([2, 2], hip_device)), dict(chunk=0), dict(window=0), dict(causal=False, window=3),
