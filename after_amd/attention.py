@@ -42,7 +42,7 @@ def _operand(t, name, dims, device=None, dtype=None):
     if t.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError(f"{name} requires a gradient: after_amd is inference only (use torch.no_grad())")
     if not t.numel():
-        return t
+        return t.new_empty(t.shape)  # (whatever its strides were)
     *outer, last = t.stride()
     each = 3 if t.dtype == torch.float32 else 7  # (elements in 16 bytes, less one)
     odd = 0
@@ -78,6 +78,16 @@ def _starts(t, name, n, device):
     return t.contiguous()
 
 
+def _ranges(tensors):
+    """[first, last) address of each (contiguous or not; empty ones have none)."""
+    return [(t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))))
+            for t in tensors if t.numel()]
+
+
+def _share(a, b):
+    return any(x < v and u < y for x, y in _ranges(a) for u, v in _ranges(b))
+
+
 def _scale(scale, dim):
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
     if not math.isfinite(scale):
@@ -96,7 +106,12 @@ def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=True, window=None,
     causal: a query sees the keys up to its own position; with `chunk` > 1 also the rest of its chunk, and with `window` only the
     newest `window` keys outside its chunk: the mask of DenoiserV2's local attention (transformerv2.py:62-96).  A query that
     sees nothing gets zeros.  Rows behind the last sequence are zeros in a new tensor and left alone in `out`, which must be
-    contiguous and must not overlap k or v (it may be q)."""
+    contiguous and must not overlap q, k or v; it may be q itself."""
+    chunk, window = int(chunk), None if window is None else int(window)
+    if not 1 <= chunk <= 1 << 24 or (window is not None and window < 1):
+        raise ValueError(f"chunk must be 1 .. 2^24 and window at least 1, got {chunk} and {window}")
+    if not causal and (chunk != 1 or window is not None):
+        raise ValueError("chunk and window belong to causal attention")
     q = _operand(q, "q", 3)
     k = _operand(k, "k", 3, q.device, q.dtype)
     v = _operand(v, "v", 3, q.device, q.dtype)
@@ -105,12 +120,9 @@ def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=True, window=None,
         raise ValueError(f"bad shapes q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)}: k and v alike, heads a multiple of kv_heads, one head_dim")
     if dim not in (64, 128):
         raise ValueError(f"head_dim must be 64 or 128, got {dim}")
-    chunk, window = int(chunk), None if window is None else int(window)
-    if chunk < 1 or (window is not None and window < 1):
-        raise ValueError(f"chunk and window must be at least 1, got {chunk} and {window}")
-    if not causal and (chunk != 1 or window is not None):
-        raise ValueError("chunk and window belong to causal attention")
     q_starts = _starts(q_starts, "q_starts", None, q.device)
+    if q_starts.numel() > 1 << 24:
+        raise ValueError(f"at most 2^24 - 1 sequences, got {q_starts.numel() - 1}")
     k_starts = q_starts if k_starts is None else _starts(k_starts, "k_starts", q_starts.numel() - 1, q.device)
     scale = _scale(scale, dim)
     fresh = out is None
@@ -119,9 +131,13 @@ def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=True, window=None,
     elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device \
             or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f"out must be a contiguous, 16-byte aligned {q.dtype} tensor {tuple(q.shape)} on {q.device}")
+    elif out.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("out requires a gradient: after_amd is inference only (use torch.no_grad())")
+    elif _share([out], [k, v] if out.data_ptr() == q.data_ptr() and q.is_contiguous() else [q, k, v]):
+        raise ValueError("out shares memory with q, k or v (it may be q itself, if that is contiguous)")
     _enqueue("after_attend_packed", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _TYPES[q.dtype], n, k.shape[0],
              q_starts.data_ptr(), k_starts.data_ptr(), q_starts.numel() - 1, heads, k.shape[1], dim, *q.stride()[:2], *k.stride()[:2],
-             *v.stride()[:2], *out.stride()[:2], scale, int(bool(causal)), window or 0, chunk, int(fresh))
+             *v.stride()[:2], heads * dim, dim, scale, int(bool(causal)), min(window or 0, 1 << 30), chunk, int(fresh))
     return out
 
 
@@ -135,8 +151,8 @@ class KVCache4:
     use) -- which `buffers()` returns and `KVCache4(..., buffers=...)` takes over as they are.  They can be written in place, not
     replaced.
 
-    Every call enqueues on the current stream, never synchronises and can be captured into a graph; the lengths live on the
-    device.  One call at a time works on a cache: order calls on different streams with events, as for any tensor."""
+    Every call but `check` enqueues on the current stream, never synchronises and can be captured into a graph; the lengths live
+    on the device.  One call at a time works on a cache: order calls on different streams with events, as for any tensor."""
 
     def __init__(self, rows, kv_heads, head_dim, capacity, device="cuda", buffers=None):
         rows, kv_heads, head_dim, capacity = int(rows), int(kv_heads), int(head_dim), int(capacity)
@@ -167,6 +183,8 @@ class KVCache4:
                         or not t.is_contiguous() or t.data_ptr() % 16:
                     raise ValueError(f"buffers[{name!r}] must be a contiguous, 16-byte aligned {dtype} tensor {shape} on {self.device}")
             tensors[name] = t
+        if buffers is not None and any(_share([t], [u]) for i, t in enumerate(tensors.values()) for u in list(tensors.values())[:i]):
+            raise ValueError("two of the buffers share memory")
         self._failed = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._tensors = tensors  # (their addresses are in _c: the attributes cannot be set to others)
         self._evicted_into = None
@@ -271,8 +289,7 @@ class KVCache4:
         if self._evicted_into is None or self._evicted_into() is not into:
             if (into.rows, into.kv_heads, into.head_dim, into.device) != (self.rows, self.kv_heads, self.head_dim, self.device):
                 raise ValueError("both caches need the same rows, kv_heads, head_dim and device")
-            ranges = [[(t.data_ptr(), t.data_ptr() + t.nbytes) for t in c.buffers().values()] for c in (self, into)]
-            if any(a < d and b < e for a, e in ranges[0] for b, d in ranges[1]):
+            if _share(self._tensors.values(), into._tensors.values()):
                 raise ValueError("the two caches share memory")
             self._evicted_into = weakref.ref(into)  # (looked at once)
         if not 1 <= keep <= into.capacity or not 0 <= recent <= keep:

@@ -111,6 +111,10 @@ def test_python_refuses_without_a_gpu():
     for bad in (dict(rows=0), dict(kv_heads=0), dict(head_dim=80), dict(capacity=0), dict(capacity=(1 << 24) + 1)):
         with pytest.raises(ValueError):
             KVCache4(**{**dict(rows=1, kv_heads=1, head_dim=64, capacity=32), **bad}, device="cpu")
+    # numbers that 32 bits would cut down to allowed ones
+    for bad in (dict(chunk=(1 << 32) + 1), dict(chunk=0), dict(window=0), dict(window=4, causal=False)):
+        with pytest.raises(ValueError):
+            attend_packed(t, t, t, torch.zeros(2, dtype=torch.int32), **bad)
 
 
 def test_reference_rounding_of_the_format():

@@ -137,6 +137,44 @@ def test_views_out_and_rows_behind_the_last_sequence(hip_device):
     assert torch.equal(attend_packed(q, shared, v, s), attend_packed(q, shared.contiguous(), v, s))
 
 
+def test_a_window_wider_than_32_bits_is_none(hip_device):
+    q, k, v = (torch.randn(300, 2, 64, generator=gen(i)).to(hip_device) for i in (71, 72, 73))
+    s = starts([300], hip_device)
+    want = attend_packed(q, k, v, s)
+    for window in (300, 1 << 30, (1 << 32) + 5):
+        assert torch.equal(attend_packed(q, k, v, s, window=window), want)
+    assert not torch.equal(attend_packed(q, k, v, s, window=5), want)
+
+
+def test_strides_that_mean_nothing(hip_device):
+    """Of empty tensors, and of dimensions of one: whatever they are, they are not looked at."""
+    wide = torch.randn(5, 1001, generator=gen(74)).to(hip_device)
+    none = wide[:0, 1:129].unflatten(1, (2, 64))
+    q = torch.randn(5, 2, 64, generator=gen(75)).to(hip_device)
+    zeros = attend_packed(q, none, none, starts([5], hip_device), starts([0], hip_device))
+    assert torch.equal(zeros, torch.zeros_like(q)) and attend_packed(none, q, q, starts([0], hip_device), starts([5], hip_device)).shape == (0, 2, 64)
+    out = torch.zeros(4, 1001, device=hip_device)[0:1, :128].unflatten(1, (2, 64))
+    one = starts([1], hip_device)
+    assert out.is_contiguous() and attend_packed(q[:1], q[:1], q[:1], one, out=out) is out
+    assert torch.equal(out, attend_packed(q[:1], q[:1], q[:1], one))
+    c = KVCache4(2, 2, 64, 32, hip_device)
+    c.append(none, none, starts([0, 0], hip_device))
+    assert c.lengths.tolist() == [0, 0]
+
+
+def test_memory_that_is_shared_is_refused(hip_device):
+    both = torch.zeros(9, 2, 64, device=hip_device)
+    q, k, s = both[:8], torch.zeros(8, 2, 64, device=hip_device), starts([8], hip_device)
+    for out, a in ((both[1:], (q, k, k)), (k, (q, k, both[:8])), (k, (q, both[:8], k)), (q, (q[:, :1].expand(-1, 2, -1), k, k))):
+        with pytest.raises(ValueError):
+            attend_packed(*a, s, out=out)
+    with torch.enable_grad(), pytest.raises(NotImplementedError):
+        attend_packed(q, k, k, s, out=torch.zeros(8, 2, 64, device=hip_device, requires_grad=True))
+    b = KVCache4(1, 2, 64, 32, hip_device).buffers()
+    with pytest.raises(ValueError):
+        KVCache4(1, 2, 64, 32, hip_device, dict(b, value_scales=b["key_scales"]))
+
+
 def test_starts_outside_the_rows_are_taken_as_the_nearest(hip_device):
     q, k, v = (torch.randn(20, 2, 64, generator=gen(4)).to(hip_device) for _ in range(3))
     out = attend_packed(q, k, v, torch.tensor([-5, 8, 90], dtype=torch.int32, device=hip_device))
