@@ -155,7 +155,8 @@ SIGNATURES = {
     "after_gemm_x6": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int,
                               c_int, c_int, c_int, c_int, c_void_p]),
     "after_attend_packed": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_void_p, c_void_p,
-                                    c_int, c_int, c_int, c_int] + [c_longlong] * 8 + [c_float, c_int, c_int, c_int, c_int, c_void_p]),
+                                    c_int, c_int, c_int, c_int] + [c_longlong] * 8 + [c_float, c_int, c_int, c_int, c_int, c_void_p, c_longlong, c_void_p]),
+    "after_attend_packed_workspace": (c_int, [c_int, c_longlong, c_longlong] + [c_int] * 5 + [POINTER(c_longlong)]),
     "after_kv4_append": (c_int, [POINTER(KV4), c_void_p, c_void_p, c_int, c_void_p, c_int] + [c_longlong] * 5 + [c_void_p]),
     "after_kv4_truncate": (c_int, [POINTER(KV4), c_void_p, c_void_p]),
     "after_kv4_read": (c_int, [POINTER(KV4), c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p]),

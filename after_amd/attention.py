@@ -14,6 +14,7 @@ hand-written HIP kernels behind the C ABI of include/after_hip.h, no fallback.
         y = small.attend(q1)                                 # [rows, 1, heads, head_dim]
 """
 import ctypes
+import functools
 import math
 import weakref
 
@@ -24,41 +25,35 @@ from . import _lib
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _operand(t, name, dims, device=None, dtype=None):
+def _operand(t, name, dims, index=None, dtype=None):
     """A tensor the kernels can address: fp32 / bf16 / fp16 on the GPU, channels contiguous, strides and base multiples of 16
     bytes -- a view of a fused projection is taken as it is, anything else is copied."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if not t.is_cuda:
         raise _lib.AFTERHipError(f"{name} is on {t.device}: after_amd runs on MI355X only (HIP kernels)")
-    if t.dtype not in _TYPES:
-        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-    if t.dim() != dims:
+    kind, strides = t.dtype, t.stride()
+    if kind not in _TYPES:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {kind}")
+    if len(strides) != dims:
         raise ValueError(f"{name} must have {dims} dimensions, got {tuple(t.shape)}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if dtype is not None and t.dtype != dtype:
-        raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
+    if index is not None and t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
+    if dtype is not None and kind is not dtype:
+        raise TypeError(f"{name} is {kind}, expected {dtype}")
     if t.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError(f"{name} requires a gradient: after_amd is inference only (use torch.no_grad())")
-    if not t.numel():
-        return t.new_empty(t.shape)  # (whatever its strides were)
-    *outer, last = t.stride()
-    each = 3 if t.dtype == torch.float32 else 7  # (elements in 16 bytes, less one)
-    odd = 0
-    for s in outer:
-        odd |= s
-    # (a token's place in a tile is addressed with 32 bits)
-    if last != 1 or odd & each or t.data_ptr() & 15 or outer[-2] >= 1 << 22:
+    odd = strides[0] | strides[1] | (strides[2] if dims == 4 else 0) | t.data_ptr() // t.element_size()
+    # (a token's place in a tile is addressed with 32 bits; what the strides of an empty tensor are does not matter)
+    if odd & (3 if kind is torch.float32 else 7) or strides[-1] != 1 or strides[-3] >= 1 << 22:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _enqueue(name, device, *args):
-    """One call of the C ABI on the device's current stream."""
-    index, fn = device.index, getattr(_lib.lib(), name)
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch.cuda.current_device() == index:
+def _enqueue(name, index, *args):
+    """One call of the C ABI on the current stream of device `index`."""
+    fn, stream = getattr(_lib.lib(), name), torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
         rc = fn(*args, stream)
     else:
         with torch.cuda.device(index):
@@ -67,12 +62,12 @@ def _enqueue(name, device, *args):
         _lib.check(rc, name)
 
 
-def _starts(t, name, n, device):
-    """int32 [n + 1] on the device (n None: any)."""
+def _starts(t, name, n, index):
+    """int32 [n + 1] on device `index` (n None: any)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype != torch.int32 or t.dim() != 1 or t.device != device:
-        raise ValueError(f"{name} must be a one-dimensional int32 tensor on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.get_device() != index:
+        raise ValueError(f"{name} must be a one-dimensional int32 tensor on cuda:{index}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     if t.numel() != n + 1 if n is not None else t.numel() < 1:
         raise ValueError(f"{name} has {t.numel()} entries, expected {'one more than sequences' if n is None else n + 1}")
     return t.contiguous()
@@ -95,6 +90,14 @@ def _scale(scale, dim):
     return scale
 
 
+@functools.lru_cache(maxsize=1024)
+def _packed_workspace(*sizes):
+    """Bytes of scratch that a call of these sizes takes (a function of the sizes alone)."""
+    size = ctypes.c_longlong()
+    _lib.check(_lib.lib().after_attend_packed_workspace(*sizes, ctypes.byref(size)), "after_attend_packed_workspace")
+    return size.value
+
+
 def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=True, window=None, chunk=1, scale=None, out=None):
     """Attention of packed sequences (include/after_hip.h: after_attend_packed).
 
@@ -113,31 +116,38 @@ def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=True, window=None,
     if not causal and (chunk != 1 or window is not None):
         raise ValueError("chunk and window belong to causal attention")
     q = _operand(q, "q", 3)
-    k = _operand(k, "k", 3, q.device, q.dtype)
-    v = _operand(v, "v", 3, q.device, q.dtype)
+    index, dtype = q.get_device(), q.dtype
+    k = _operand(k, "k", 3, index, dtype)
+    v = _operand(v, "v", 3, index, dtype)
     n, heads, dim = q.shape
-    if k.shape != v.shape or k.shape[2] != dim or k.shape[1] == 0 or heads == 0 or heads % k.shape[1]:
+    keys, kv_heads, k_dim = k.shape
+    if k.shape != v.shape or k_dim != dim or kv_heads == 0 or heads == 0 or heads % kv_heads:
         raise ValueError(f"bad shapes q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)}: k and v alike, heads a multiple of kv_heads, one head_dim")
     if dim not in (64, 128):
         raise ValueError(f"head_dim must be 64 or 128, got {dim}")
-    q_starts = _starts(q_starts, "q_starts", None, q.device)
-    if q_starts.numel() > 1 << 24:
-        raise ValueError(f"at most 2^24 - 1 sequences, got {q_starts.numel() - 1}")
-    k_starts = q_starts if k_starts is None else _starts(k_starts, "k_starts", q_starts.numel() - 1, q.device)
+    q_starts = _starts(q_starts, "q_starts", None, index)
+    seqs = q_starts.numel() - 1
+    if seqs >= 1 << 24:
+        raise ValueError(f"at most 2^24 - 1 sequences, got {seqs}")
+    k_starts = q_starts if k_starts is None else _starts(k_starts, "k_starts", seqs, index)
     scale = _scale(scale, dim)
     fresh = out is None
     if fresh:
-        out = torch.empty(n, heads, dim, device=q.device, dtype=q.dtype)
-    elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device \
+        out = q.new_empty((n, heads, dim))
+    elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != dtype or out.device != q.device \
             or not out.is_contiguous() or out.data_ptr() % 16:
-        raise ValueError(f"out must be a contiguous, 16-byte aligned {q.dtype} tensor {tuple(q.shape)} on {q.device}")
+        raise ValueError(f"out must be a contiguous, 16-byte aligned {dtype} tensor {tuple(q.shape)} on {q.device}")
     elif out.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("out requires a gradient: after_amd is inference only (use torch.no_grad())")
     elif _share([out], [k, v] if out.data_ptr() == q.data_ptr() and q.is_contiguous() else [q, k, v]):
         raise ValueError("out shares memory with q, k or v (it may be q itself, if that is contiguous)")
-    _enqueue("after_attend_packed", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _TYPES[q.dtype], n, k.shape[0],
-             q_starts.data_ptr(), k_starts.data_ptr(), q_starts.numel() - 1, heads, k.shape[1], dim, *q.stride()[:2], *k.stride()[:2],
-             *v.stride()[:2], heads * dim, dim, scale, int(bool(causal)), min(window or 0, 1 << 30), chunk, int(fresh))
+    window, kind = min(window or 0, 1 << 30), _TYPES[dtype]
+    size = _packed_workspace(kind, n, keys, seqs, heads, kv_heads, dim, window)
+    work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None  # (as in KVCache4.attend)
+    q_at, k_at, v_at = q.stride(), k.stride(), v.stride()
+    _enqueue("after_attend_packed", index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), kind, n, keys, q_starts.data_ptr(),
+             k_starts.data_ptr(), seqs, heads, kv_heads, dim, q_at[0], q_at[1], k_at[0], k_at[1], v_at[0], v_at[1], heads * dim, dim, scale,
+             1 if causal else 0, window, chunk, 1 if fresh else 0, work.data_ptr() if size else None, size)
     return out
 
 
@@ -168,6 +178,7 @@ class KVCache4:
         if device.type != "cuda":
             raise _lib.AFTERHipError(f"KVCache4 on {device}: after_amd runs on MI355X only (HIP kernels)")
         self.device = torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)
+        self._index = self.device.index
         layout = dict(keys=((rows, kv_heads, C, head_dim // 2), torch.uint8), key_scales=((rows, kv_heads, C, head_dim // 32), torch.uint8),
                       values=((rows, kv_heads, C // 8, head_dim, 4), torch.uint8), value_scales=((rows, kv_heads, C, head_dim // 32), torch.uint8),
                       weights=((rows, kv_heads, C), torch.float32), lengths=((rows, ), torch.int32))
@@ -213,8 +224,8 @@ class KVCache4:
         [total, kv_heads, head_dim] with `starts` (int32 [rows + 1]): those of row r are starts[r] .. starts[r + 1] - 1.  Tokens
         for which a row has no room are dropped; `check()` reports that."""
         dims = 4 if starts is None else 3
-        k = _operand(k, "k", dims, self.device)
-        v = _operand(v, "v", dims, self.device, k.dtype)
+        k = _operand(k, "k", dims, self._index)
+        v = _operand(v, "v", dims, self._index, k.dtype)
         if k.shape != v.shape or tuple(k.shape[-2:]) != (self.kv_heads, self.head_dim) or (starts is None and k.shape[0] != self.rows):
             raise ValueError(f"bad shapes k{tuple(k.shape)} v{tuple(v.shape)} for {self.rows} rows of {self.kv_heads} heads of {self.head_dim}")
         tokens = 0
@@ -224,14 +235,14 @@ class KVCache4:
                 raise ValueError(f"{tokens} new tokens, the cache has {self.capacity} slots per row")
             k, v = k.flatten(0, 1), v.flatten(0, 1)
         else:
-            starts = _starts(starts, "starts", self.rows, self.device)
-        _enqueue("after_kv4_append", self.device, self._ref, k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], None if starts is None else starts.data_ptr(),
+            starts = _starts(starts, "starts", self.rows, self._index)
+        _enqueue("after_kv4_append", self._index, self._ref, k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], None if starts is None else starts.data_ptr(),
                  tokens, k.shape[0], *k.stride()[:2], *v.stride()[:2])
 
     def truncate(self, lengths=None):
         """Takes back the newest slots: row r keeps the first lengths[r] (int32 [rows] on the device); None empties the cache."""
         lengths = None if lengths is None else self._row_values(lengths, "lengths")
-        _enqueue("after_kv4_truncate", self.device, self._ref, None if lengths is None else lengths.data_ptr())
+        _enqueue("after_kv4_truncate", self._index, self._ref, None if lengths is None else lengths.data_ptr())
 
     def read(self, start=None, count=None, dtype=torch.bfloat16):
         """(k, v) [rows, kv_heads, count, head_dim]: the values that the slots start[r] .. start[r] + count - 1 stand for (int32
@@ -243,7 +254,7 @@ class KVCache4:
             raise TypeError(f"values are read as bfloat16 or float32, got {dtype}")
         start = None if start is None else self._row_values(start, "start")
         k, v = (torch.empty(self.rows, self.kv_heads, count, self.head_dim, dtype=dtype, device=self.device) for _ in range(2))
-        _enqueue("after_kv4_read", self.device, self._ref, k.data_ptr(), v.data_ptr(), _TYPES[dtype], None if start is None else start.data_ptr(), count)
+        _enqueue("after_kv4_read", self._index, self._ref, k.data_ptr(), v.data_ptr(), _TYPES[dtype], None if start is None else start.data_ptr(), count)
         return k, v
 
     def attend(self, q, scale=None, accumulate=False, decay=1.0):
@@ -253,7 +264,7 @@ class KVCache4:
 
         accumulate: `weights` = decay * weights + the probability that each slot received, summed over the tokens and the heads
         of its group (decay = 0 replaces them)."""
-        q = _operand(q, "q", 4, self.device)
+        q = _operand(q, "q", 4, self._index)
         rows, tokens, heads, dim = q.shape
         if rows != self.rows or dim != self.head_dim or heads == 0 or heads % self.kv_heads:
             raise ValueError(f"bad shape q{tuple(q.shape)} for {self.rows} rows of {self.kv_heads} key heads of {self.head_dim}")
@@ -274,7 +285,7 @@ class KVCache4:
         # (scratch of this call: the allocator gives it to later calls of this stream only, and to a captured graph its own)
         size = self._work[key]
         work = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
-        _enqueue("after_kv4_attend", self.device, self._ref, q.data_ptr(), out.data_ptr(), _TYPES[q.dtype], heads, tokens, *q.stride()[:3],
+        _enqueue("after_kv4_attend", self._index, self._ref, q.data_ptr(), out.data_ptr(), _TYPES[q.dtype], heads, tokens, *q.stride()[:3],
                  scale, accumulate, decay, None if work is None else work.data_ptr(), size)
         return out
 
@@ -295,7 +306,7 @@ class KVCache4:
         if not 1 <= keep <= into.capacity or not 0 <= recent <= keep:
             raise ValueError(f"1 <= keep <= {into.capacity} and 0 <= recent <= keep, got {keep} and {recent}")
         slots = torch.empty(self.rows, self.kv_heads, keep, dtype=torch.int32, device=self.device)
-        _enqueue("after_kv4_evict", self.device, self._ref, into._ref, keep, recent, slots.data_ptr())
+        _enqueue("after_kv4_evict", self._index, self._ref, into._ref, keep, recent, slots.data_ptr())
         return slots
 
     def check(self):

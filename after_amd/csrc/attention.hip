@@ -10,8 +10,15 @@
 // Rows.  The `group` heads that share a key head are rows of one tile, row = token * group + head: short sequences fill tiles,
 // and a key tile is read once for all of them.  A workgroup holds 128 rows, 32 to a wave; its tile number alone says which
 // sequence it serves (sequence b owns the numbers from floor(start_b * group / 128) + b on), so the grid needs no lengths.
+//
+// What bounds it.  Long prompts: the matrix pipes, with the softmax's exponentials between two products; 16384 causal tokens, bf16,
+// 32 / 8 heads of 128: 2120 us, 1037 TFLOP/s, where a large product of the library reaches 1155 (fp16 heads of 128 in a batch of
+// 1 .. 2047 tokens: 306 us, 710; heads of 64, 8192 tokens: 330 us, 830; fp32 heads of 128, 4096 tokens: 585 us, 118 of 153).
+// Tiles of 64 keys, two of them in LDS and two workgroups on a CU: one computes while the other waits.  Measured and left out:
+// V read by instructions that wait by themselves (2240 us), skipping the unseen half of a masked tile (2330), scheduling hints (2120).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "common.h"
@@ -20,6 +27,7 @@
 namespace after {
 namespace {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -63,11 +71,13 @@ struct PackedArgs {
     void* out;
     const int *qs, *ks;
     long long qts, qhs, kts, khs, vts, vhs, ots, ohs;
-    int q_rows, k_rows, n_seqs, heads, kv_heads, group, tiles;
-    Divisor by_group, by_chunk, by_kv_heads;
+    int q_rows, k_rows, n_seqs, heads, kv_heads, group, tiles, splits;
+    Divisor by_group, by_chunk, by_kv_heads, by_splits;
     float scale2;     // |scale| log2 e, > 0 (a masked score, -inf, stays -inf)
     unsigned q_sign;  // the sign bits of a word of q, if scale is negative
     int causal, window, zero_rest;
+    float* part_o;    // [tiles][kv_heads][splits][kFewRows][D], if splits > 1
+    f32x2* part_ml;   // the same rows' maxima and sums
 };
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
@@ -91,6 +101,37 @@ __device__ __forceinline__ void seen(const PackedArgs& a, int p, int keys, int& 
         last = p < 0 ? 0 : min(begin + chunk, keys);
         if (a.window > 0) first = max(0, min(begin, p - a.window + 1));
     }
+}
+
+// Which sequence a tile of ROWS rows serves, and where in it: rows [row0, row0 + ROWS) of the sequence's nq * group; false: none
+struct Place {
+    int b, q0, nq, k0, nk, row0, rows;
+};
+template <int ROWS>
+__device__ __forceinline__ bool find_tile(const PackedArgs& a, int tile, Place& p) {
+    const int lane = threadIdx.x & 63;
+    // the last sequence that begins at or before this tile: 64 candidates at a time; the last look holds its ends
+    int lo = 0, hi = a.n_seqs, q1, k1;
+    for (;;) {
+        const int step = (hi - lo + 64) >> 6, at = lo + lane * step, qs = q_start(a, at), ks = k_start(a, at);
+        const bool begun = (int)((long long)qs * a.group / ROWS) + at <= tile;
+        const int j = 63 - __clzll(__ballot(begun && at <= hi) | 1);  // (sequence lo has begun)
+        if (step == 1) {
+            p.b = lo + j;
+            p.q0 = __builtin_amdgcn_readlane(qs, j);
+            p.k0 = __builtin_amdgcn_readlane(ks, j);
+            q1 = j < 63 ? __builtin_amdgcn_readlane(qs, (j + 1) & 63) : q_start(a, p.b + 1);
+            k1 = j < 63 ? __builtin_amdgcn_readlane(ks, (j + 1) & 63) : k_start(a, p.b + 1);
+            break;
+        }
+        lo += j * step;
+        hi = min(hi, lo + step - 1);
+    }
+    p.nq = q1 - p.q0;
+    p.row0 = (tile - ((int)((long long)p.q0 * a.group / ROWS) + p.b)) * ROWS;
+    p.rows = p.nq * a.group;  // (< 2^31: checked on the host)
+    p.nk = p.b < a.n_seqs ? max(k1 - p.k0, 0) : 0;
+    return p.row0 >= 0 && p.row0 < p.rows && (p.b < a.n_seqs || a.zero_rest);
 }
 
 // 16-byte pieces of a 64-row tile in LDS.  Keys: a wave reads the same piece of 32 rows, so a row's pieces are permuted by its
@@ -141,27 +182,9 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
     // neighbouring workgroups are dispatched to different XCDs: a key head's workgroups stay on one L2 where there are eight.
     // Tiles from the last to the first: with a causal mask the longest first.
     const int back = a.by_kv_heads(blockIdx.x), h = blockIdx.x - back * a.kv_heads, tile = a.tiles - 1 - back;
-    // the last sequence that begins at or before this tile: 64 candidates at a time; the last look holds its ends
-    int lo = 0, hi = a.n_seqs, b, q0, q1, k0, k1;
-    for (;;) {
-        const int step = (hi - lo + 64) >> 6, at = lo + lane * step, qs = q_start(a, at), ks = k_start(a, at);
-        const bool begun = (int)((long long)qs * a.group / BM) + at <= tile;
-        const int j = 63 - __clzll(__ballot(begun && at <= hi) | 1);  // (sequence lo has begun)
-        if (step == 1) {
-            b = lo + j;
-            q0 = __builtin_amdgcn_readlane(qs, j);
-            k0 = __builtin_amdgcn_readlane(ks, j);
-            q1 = j < 63 ? __builtin_amdgcn_readlane(qs, (j + 1) & 63) : q_start(a, b + 1);
-            k1 = j < 63 ? __builtin_amdgcn_readlane(ks, (j + 1) & 63) : k_start(a, b + 1);
-            break;
-        }
-        lo += j * step;
-        hi = min(hi, lo + step - 1);
-    }
-    const int nq = q1 - q0, row0 = (tile - ((int)((long long)q0 * a.group / BM) + b)) * BM;
-    const int rows = nq * a.group;  // (< 2^31: checked on the host)
-    if (row0 < 0 || row0 >= rows || (b == a.n_seqs && !a.zero_rest)) return;
-    const int nk = b < a.n_seqs ? max(k1 - k0, 0) : 0;
+    Place place;
+    if (!find_tile<BM>(a, tile, place)) return;
+    const int q0 = place.q0, nq = place.nq, k0 = place.k0, nk = place.nk, row0 = place.row0, rows = place.rows;
 
     // this lane's query, and the keys that it and its workgroup see
     const int row = row0 + wave * 32 + l31, t = a.by_group(min(row, rows - 1)), g = min(row, rows - 1) - t * a.group;
@@ -390,8 +413,350 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
     }
 }
 
+// ---------------------------------------------------------------------------------------------------------------- few rows
+// Where tiles of 128 rows would leave most of the chip idle (short prompts, a few new tokens over many keys): 32 rows to a
+// workgroup, whose four waves share out their keys, 32 at a time.  Each wave has one buffer for keys and one for values in LDS:
+// the next keys are asked for when the scores are formed, the next values when they are added up, and no wave waits for another
+// until the four are joined.  With `splits` > 1 that many workgroups share the keys, and attend_join_kernel joins them.
+constexpr int kFewRows = 32;
+// steps of 32 keys per wave, and the workgroups that have any
+__device__ __forceinline__ int few_share(const PackedArgs& a, int steps) { return max(1, (steps + 4 * a.splits - 1) / (4 * a.splits)); }
+__device__ __forceinline__ int few_used(int steps, int share) { return (steps + 4 * share - 1) / (4 * share); }
+// the keys that some / every query of the tile sees
+__device__ __forceinline__ void few_seen(const PackedArgs& a, const Place& p, int& t_first, int& t_last, int& all_first, int& all_last) {
+    const int p0 = p.nk - p.nq;
+    seen(a, a.by_group(p.row0) + p0, p.nk, t_first, all_last);
+    seen(a, a.by_group(min(p.row0 + kFewRows, p.rows) - 1) + p0, p.nk, all_first, t_last);
+}
+
 template <int TYPE, int D>
-int run_packed(const PackedArgs& a, hipStream_t s) {
+__global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 : 2) void attend_few_kernel(PackedArgs a) {
+    using E = Elem<TYPE>;
+    using T = typename E::T;
+    constexpr int PIECES = D * (int)sizeof(T) / 16, LOADS = PIECES / 2, DT = D / 32;
+    constexpr int RW = 64 / PIECES;                // rows that one piece per lane covers
+    constexpr unsigned HALF = kFewRows * D * sizeof(T);  // bytes of 32 keys
+    extern __shared__ __align__(16) char lds[];    // [4][keys, values]; then [4][32][D + 4] floats
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, half = lane >> 5;
+    const int back = a.by_kv_heads(blockIdx.x), h = blockIdx.x - back * a.kv_heads, of = a.by_splits(back), split = back - of * a.splits;
+    const int tile = a.tiles - 1 - of;
+    Place place;
+    if (!find_tile<kFewRows>(a, tile, place)) return;
+    const int q0 = place.q0, nq = place.nq, nk = place.nk, row0 = place.row0, rows = place.rows;
+    int t_first, t_last, all_first, all_last;
+    few_seen(a, place, t_first, t_last, all_first, all_last);
+    const int steps = (max(t_last - t_first, 0) + 31) / 32, share = few_share(a, steps), used = few_used(steps, share);
+    if (split > 0 && split >= used) return;
+    const int begin = min((split * 4 + wave) * share, steps), end = min(begin + share, steps);
+
+    const int row = min(row0 + l31, rows - 1), t = a.by_group(row), g = row - t * a.group;
+    int first, last;
+    seen(a, t + nk - nq, nk, first, last);
+    const T* qp = (const T*)a.q + (long long)(q0 + t) * a.qts + (long long)(h * a.group + g) * a.qhs;
+    const T* kp = (const T*)a.k + (long long)place.k0 * a.kts + (long long)h * a.khs;
+    const T* vp = (const T*)a.v + (long long)place.k0 * a.vts + (long long)h * a.vhs;
+    constexpr int QN = sizeof(T) == 4 ? D / 8 : D / 16;
+    u32x4 qf[QN];
+#pragma unroll
+    for (int s = 0; s < QN; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qp + (2 * s + half) * (16 / (int)sizeof(T)));
+    __builtin_amdgcn_sched_barrier(0);  // (asked for before the first keys, so that they need not be waited for together)
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+    float mx = -INFINITY, l = 0.f;
+
+    const unsigned k_lds = (unsigned)(unsigned long)(__attribute__((address_space(3))) char*)lds + wave * (2 * HALF), v_lds = k_lds + HALF;
+    u32x4* lk = reinterpret_cast<u32x4*>(lds + wave * (2 * HALF));
+    u32x4* lv = lk + kFewRows * PIECES;
+    const int fr = lane / PIECES, fc = lane % PIECES;
+    const unsigned kb = (unsigned)a.kts * (unsigned)sizeof(T), vb = (unsigned)a.vts * (unsigned)sizeof(T);
+    // (rows behind the sequence repeat its last one: they are masked)
+    auto fetch = [&](int j0, const T* from, unsigned pitch, unsigned to, bool keys) {
+        const unsigned long long at = reinterpret_cast<unsigned long long>(from) + (unsigned long long)j0 * pitch;
+        const int left = nk - 1 - j0;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int r = i * RW + fr;
+            const unsigned piece = keys ? fc ^ k_flip<PIECES>(r) : sizeof(T) == 4 ? fc : fc ^ v_flip<PIECES>(r);
+            lds_dma16(to + i * 1024, (unsigned)min(r, left) * pitch + piece * 16, at);
+        }
+    };
+    if (begin < end) {
+        fetch(t_first + 32 * begin, kp, kb, k_lds, true);
+        fetch(t_first + 32 * begin, vp, vb, v_lds, false);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int s = 0; s < QN; ++s) qf[s] = qf[s] ^ a.q_sign;
+    for (int n = begin; n < end; ++n) {
+        const int j0 = t_first + 32 * n;
+        const bool masked = j0 < all_first || j0 + 32 > all_last, more = n + 1 < end;
+        wait_vmcnt_imm<LOADS>();  // (the keys; the values asked for after them are still on their way)
+        f32x16 sc;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+#pragma unroll
+        for (int s = 0; s < QN; ++s) {
+            const u32x4 kf = lk[l31 * PIECES + ((2 * s + half) ^ k_flip<PIECES>(l31))];
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]), __uint_as_float(qf[s][e]), sc, 0, 0, 0);
+            } else
+                sc = E::mfma(__builtin_bit_cast(typename E::V8, kf), __builtin_bit_cast(typename E::V8, qf[s]), sc);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the keys have been read)
+        if (more) fetch(j0 + 32, kp, kb, k_lds, true);
+        if (masked) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int j = j0 + 4 * half + 8 * (e >> 2) + (e & 3);
+                sc[e] = j >= first && j < last ? sc[e] : -INFINITY;
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[e]);
+        top = fmaxf(top, __shfl_xor(top, 32)) * a.scale2;
+        if (__any(top > mx + 8.f)) {  // (as above)
+            const float now = fmaxf(mx, top), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - now);
+            mx = now;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < DT; ++i) o[i] = o[i] * f;
+        }
+        const float off = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale2, -off));
+            l += sc[e];
+        }
+        if (more)
+            wait_vmcnt_imm<LOADS>();
+        else
+            wait_vmcnt_imm<0>();
+        unsigned odd = 0;  // rows of V with infinities or NaN, in a masked step
+        if (masked) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const bool bad = odd_value<TYPE>(lv[i * 64 + lane]);
+                unsigned long long at = __ballot(bad);
+                while (at) {  // (rare)
+                    odd |= 1u << (i * RW + (__ffsll(at) - 1) / PIECES);
+                    at &= at - 1;
+                }
+            }
+            if (odd) {
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i)
+                    if (odd >> (i * RW + fr) & 1) lv[i * 64 + lane] = u32x4{0, 0, 0, 0};
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            }
+        }
+        if constexpr (sizeof(T) == 4) {
+            const float* vv = reinterpret_cast<const float*>(lv);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int j = 8 * (e >> 2) + 4 * half + (e & 3);
+#pragma unroll
+                for (int i = 0; i < DT; ++i) o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(vv[j * D + 32 * i + l31], sc[e], o[i], 0, 0, 0);
+            }
+        } else {
+            const char* vv = reinterpret_cast<const char*>(lv);
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                typename E::V8 pf;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) pf[e] = (T)sc[8 * s + e];
+#pragma unroll
+                for (int i = 0; i < DT; ++i) {
+                    union {
+                        typename E::V8 v;
+                        s16x4 p[2];
+                    } vf;
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const int r = 16 * s + 8 * w + 4 * half + ((lane & 15) >> 2);
+                        const int byte = 64 * i + (lane & 16) * 2 + (lane & 3) * 8;
+                        vf.p[w] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) s16x4*)(vv + 16 * (r * PIECES + ((byte >> 4) ^ v_flip<PIECES>(r))) + (byte & 15)));
+                    }
+                    o[i] = E::mfma(vf.v, pf, o[i]);
+                }
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the values have been read)
+        if (more) fetch(j0 + 32, vp, vb, v_lds, false);
+        while (odd) {  // (uniform) only for the queries that see them
+            const int j = __ffs(odd) - 1, at = j0 + j, e_at = (j >> 3) * 4 + (j & 3);
+            odd &= odd - 1;
+            float p = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (e == e_at) p = sc[e];
+            p = __shfl(p, (j >> 2 & 1) * 32 + l31);
+            if (at >= first && at < last) {
+#pragma unroll
+                for (int i = 0; i < DT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        o[i][e] = fmaf(p, (float)vp[(long long)at * a.vts + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3)], o[i][e]);
+            }
+        }
+    }
+
+    // the four waves' shares -> one
+    l += __shfl_xor(l, 32);
+    constexpr int PITCH = D + 4;
+    float* so = reinterpret_cast<float*>(lds);
+    float* sm = so + 4 * kFewRows * PITCH;  // [4][32], then the sums
+    lds_barrier();                          // (keys and values are no longer read)
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<f32x4*>(so + (wave * kFewRows + l31) * PITCH + 32 * i + 2 * e + 4 * half) = f32x4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+    if (half == 0) {
+        sm[wave * 32 + l31] = mx;
+        sm[128 + wave * 32 + l31] = l;
+    }
+    lds_barrier();
+    constexpr int W = D / 8;
+    const int r = tid >> 3, c = (tid & 7) * 4;  // channels c + 32 i ..: eight neighbours read and write 128 bytes
+    float all = -INFINITY, sum = 0.f, acc[W] = {};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) all = fmaxf(all, sm[w * 32 + r]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float m = sm[w * 32 + r], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - all);
+        sum += sm[128 + w * 32 + r] * f;  // (0 without a key; all scores NaN: NaN)
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(so + (w * kFewRows + r) * PITCH + 32 * i + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[4 * i + e] += x[e] * f;
+        }
+    }
+    if (row0 + r >= rows) return;
+    if (used <= 1) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int tr = a.by_group(row0 + r), gr = row0 + r - tr * a.group;
+        T* out = (T*)a.out + (long long)(q0 + tr) * a.ots + (long long)(h * a.group + gr) * a.ohs + c;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+            typedef T T4 __attribute__((ext_vector_type(4)));
+            T4 y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = (T)(acc[4 * i + e] * inv);
+            *reinterpret_cast<T4*>(out + 32 * i) = y;
+        }
+    } else {
+        const size_t at = (((size_t)tile * a.kv_heads + h) * a.splits + split) * kFewRows + r;
+        if (c == 0) a.part_ml[at] = f32x2{all, sum};
+#pragma unroll
+        for (int i = 0; i < DT; ++i) *reinterpret_cast<f32x4*>(a.part_o + at * D + 32 * i + c) = f32x4{acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]};
+    }
+}
+
+// The rows whose keys were split.  One workgroup per row: 16 groups of 16 lanes share its pieces.
+template <int TYPE, int D>
+__global__ __launch_bounds__(256) void attend_join_kernel(PackedArgs a) {
+    using T = typename Elem<TYPE>::T;
+    constexpr int W = D / 16;
+    typedef float fw __attribute__((ext_vector_type(W)));
+    __shared__ float part[16][D];
+    const int x = blockIdx.x, r = x % kFewRows, back = a.by_kv_heads(x / kFewRows), h = x / kFewRows - back * a.kv_heads, tile = back;
+    Place place;
+    if (!find_tile<kFewRows>(a, tile, place) || place.row0 + r >= place.rows) return;
+    int t_first, t_last, dummy, steps;
+    few_seen(a, place, t_first, t_last, dummy, dummy);
+    steps = (max(t_last - t_first, 0) + 31) / 32;
+    const int used = few_used(steps, few_share(a, steps));
+    if (used <= 1) return;  // (written already)
+    const size_t at = ((size_t)tile * a.kv_heads + h) * a.splits * kFewRows + r;
+    const int lane = threadIdx.x & 63, group = threadIdx.x >> 4, d = (threadIdx.x & 15) * W;
+    // (at most 64 pieces: a lane for each)
+    f32x2 ml = {-INFINITY, 0.f};
+    if (lane < used) ml = a.part_ml[at + (size_t)lane * kFewRows];
+    float all = ml[0];
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) all = fmaxf(all, __shfl_xor(all, o));
+    const float f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - all);
+    float sum = ml[1] * f;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) sum += __shfl_xor(sum, o);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    fw acc;
+#pragma unroll
+    for (int i = 0; i < W; ++i) acc[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int s = 16 * i + group;
+        const float fs = __shfl(f, s) * inv;
+        if (s < used) {
+            const fw y = *reinterpret_cast<const fw*>(a.part_o + (at + (size_t)s * kFewRows) * D + d);
+#pragma unroll
+            for (int e = 0; e < W; ++e) acc[e] = fmaf(y[e], fs, acc[e]);
+        }
+    }
+    *reinterpret_cast<fw*>(&part[group][d]) = acc;
+    __syncthreads();
+    if (threadIdx.x < D) {
+        float y = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y += part[i][threadIdx.x];
+        const int tr = a.by_group(place.row0 + r), gr = place.row0 + r - tr * a.group;
+        ((T*)a.out)[(long long)(place.q0 + tr) * a.ots + (long long)(h * a.group + gr) * a.ohs + threadIdx.x] = (T)y;
+    }
+}
+
+struct PackedPlan {
+    bool few;
+    int tiles, splits;
+    long long ml_bytes, bytes;
+};
+PackedPlan packed_plan(int type, long long q_rows, long long k_rows, int n_seqs, int heads, int kv_heads, int head_dim, int window) {
+    const int group = heads / kv_heads;
+    PackedPlan p;
+    const long long wide = (q_rows * group / BM + n_seqs + 1) * kv_heads;  // workgroups of 128 rows (some without any)
+    long long keys = n_seqs > 0 ? k_rows / n_seqs : 0;
+    if (window > 0 && window < keys) keys = window;
+    // 32 rows to a workgroup while that many of 128 are too few for 256 CUs.  fp32, where a tile takes longest: 3 x 256 tokens of
+    // 8 heads of 64, window 8 (80 workgroups) 8.9 us against 20.9, 6000 of 8 / 2 heads of 128 (378) 706 / 778, 8192 (516) 1285 /
+    // 1129.  16 bits, long sequences: 2048 tokens of 8 heads of 64 (144) 17.5 / 34.3, of 8 / 2 heads of 128 6000 (378) 132 / 132 and
+    // 7000 (440) 171 / 159; short ones, where the beginning of a workgroup counts: 8 x 200 of 8 heads of 128 (168) 10.0 / 12.0,
+    // 12 x 200 (248) 15.7 / 12.5.
+    p.few = wide <= (type == AFTER_T_F32 ? 512 : keys >= 1024 ? 384 : 192);
+    p.tiles = (int)(q_rows * group / (p.few ? kFewRows : BM)) + n_seqs + 1;
+    p.splits = 1;
+    if (p.few) {
+        // The keys are split where a quarter of the chip is not filled, at 512 keys and more to a workgroup.  bf16, 32 / 8 heads of
+        // 128, one query: over 32768 keys 28.4 us against 276, over 2048 12.4 / 21.8, over 1024 12.5 / 13.1; 4 x one query over
+        // 2000 16.5 / 22.5, 16 x (152 workgroups) 34.1 / 25.6.
+        const long long fill = 512 / ((long long)p.tiles * kv_heads), most = keys / 512;
+        if (fill >= 4) p.splits = (int)std::max(1ll, std::min(std::min(fill, most), 64ll));
+    }
+    const long long parts = p.splits > 1 ? (long long)p.tiles * kv_heads * p.splits * kFewRows : 0;
+    p.ml_bytes = parts * 8;
+    p.bytes = p.ml_bytes + parts * head_dim * 4;
+    return p;
+}
+
+template <int TYPE, int D>
+int run_packed(const PackedArgs& a, bool few, hipStream_t s) {
+    using T = typename Elem<TYPE>::T;
+    if (few) {
+        constexpr size_t tiles = 8 * kFewRows * D * sizeof(T), joined = 4 * kFewRows * (D + 4) * 4 + 1024, lds = tiles > joined ? tiles : joined;
+        static LdsAttr attr;
+        AFTER_TRY(ensure_lds_attr(attr, (const void*)attend_few_kernel<TYPE, D>, lds));
+        hipLaunchKernelGGL((attend_few_kernel<TYPE, D>), dim3((unsigned)a.tiles * a.kv_heads * a.splits), dim3(256), lds, s, a);
+        if (a.splits > 1) hipLaunchKernelGGL((attend_join_kernel<TYPE, D>), dim3((unsigned)a.tiles * a.kv_heads * kFewRows), dim3(256), 0, s, a);
+        AFTER_HIP_CHECK(hipGetLastError());
+        return AFTER_OK;
+    }
     constexpr size_t tiles = 4 * BN * D * sizeof(typename Elem<TYPE>::T), out = 4 * 32 * (D * sizeof(typename Elem<TYPE>::T) + 16), lds = tiles > out ? tiles : out;
     static LdsAttr attr;
     AFTER_TRY(ensure_lds_attr(attr, (const void*)attend_packed_kernel<TYPE, D>, lds));
@@ -405,19 +770,34 @@ int run_packed(const PackedArgs& a, hipStream_t s) {
 
 using namespace after;
 
-extern "C" int after_attend_packed(const void* q, const void* k, const void* v, void* out, int type, long long q_rows, long long k_rows,
-                                   const int* q_starts, const int* k_starts, int n_seqs, int heads, int kv_heads, int head_dim,
-                                   long long q_token_stride, long long q_head_stride, long long k_token_stride, long long k_head_stride,
-                                   long long v_token_stride, long long v_head_stride, long long out_token_stride, long long out_head_stride,
-                                   float scale, int causal, int window, int chunk, int zero_rest, void* stream) {
+static int check_sizes(int type, long long q_rows, long long k_rows, int n_seqs, int heads, int kv_heads, int head_dim, int window) {
     AFTER_REQUIRE(type == AFTER_T_F32 || type == AFTER_T_BF16 || type == AFTER_T_F16, AFTER_E_INVALID, "attend_packed: unknown element type %d", type);
     AFTER_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, AFTER_E_INVALID, "attend_packed: heads must be a multiple of kv_heads (got %d, %d)", heads,
                   kv_heads);
     AFTER_REQUIRE(head_dim == 64 || head_dim == 128, AFTER_E_INVALID, "attend_packed: head_dim 64 or 128 (got %d)", head_dim);
     AFTER_REQUIRE(n_seqs >= 0 && n_seqs <= (1 << 24) && q_rows >= 0 && k_rows >= 0 && k_rows < (1ll << 30), AFTER_E_INVALID,
                   "attend_packed: 0 <= n_seqs <= 2^24, 0 <= rows < 2^30");
+    AFTER_REQUIRE(q_rows * (heads / kv_heads) < (1ll << 30), AFTER_E_INVALID, "attend_packed: q_rows x heads / kv_heads must stay below 2^30");
+    const PackedPlan p = packed_plan(type, q_rows, k_rows, n_seqs, heads, kv_heads, head_dim, window);
+    // (a grid's threads are counted in 32 bits)
+    AFTER_REQUIRE(p.tiles < (1 << 24) / kv_heads, AFTER_E_INVALID, "attend_packed: too many tokens x heads for one call");
+    return AFTER_OK;
+}
+
+extern "C" int after_attend_packed_workspace(int type, long long q_rows, long long k_rows, int n_seqs, int heads, int kv_heads, int head_dim, int window, long long* bytes) {
+    AFTER_REQUIRE(bytes, AFTER_E_INVALID, "attend_packed_workspace: bytes is NULL");
+    AFTER_TRY(check_sizes(type, q_rows, k_rows, n_seqs, heads, kv_heads, head_dim, window));
+    *bytes = packed_plan(type, q_rows, k_rows, n_seqs, heads, kv_heads, head_dim, window).bytes;
+    return AFTER_OK;
+}
+
+extern "C" int after_attend_packed(const void* q, const void* k, const void* v, void* out, int type, long long q_rows, long long k_rows,
+                                   const int* q_starts, const int* k_starts, int n_seqs, int heads, int kv_heads, int head_dim,
+                                   long long q_token_stride, long long q_head_stride, long long k_token_stride, long long k_head_stride,
+                                   long long v_token_stride, long long v_head_stride, long long out_token_stride, long long out_head_stride,
+                                   float scale, int causal, int window, int chunk, int zero_rest, void* workspace, long long workspace_bytes, void* stream) {
+    AFTER_TRY(check_sizes(type, q_rows, k_rows, n_seqs, heads, kv_heads, head_dim, window));
     const int group = heads / kv_heads;
-    AFTER_REQUIRE(q_rows * group < (1ll << 30), AFTER_E_INVALID, "attend_packed: q_rows x heads / kv_heads must stay below 2^30");
     AFTER_REQUIRE(std::isfinite(scale), AFTER_E_INVALID, "attend_packed: scale must be finite");
     AFTER_REQUIRE(window >= 0 && chunk >= 1 && chunk <= (1 << 24) && (causal || (window == 0 && chunk == 1)), AFTER_E_INVALID,
                   "attend_packed: window >= 0 (0: none) and chunk >= 1, both for causal attention only");
@@ -434,20 +814,23 @@ extern "C" int after_attend_packed(const void* q, const void* k, const void* v, 
     a.qts = q_token_stride, a.qhs = q_head_stride, a.kts = k_token_stride, a.khs = k_head_stride;
     a.vts = v_token_stride, a.vhs = v_head_stride, a.ots = out_token_stride, a.ohs = out_head_stride;
     a.q_rows = (int)q_rows, a.k_rows = (int)k_rows, a.n_seqs = n_seqs, a.heads = heads, a.kv_heads = kv_heads, a.group = group;
-    a.tiles = (int)(q_rows * group / BM) + n_seqs + 1;
+    PackedPlan p = packed_plan(type, q_rows, k_rows, n_seqs, heads, kv_heads, head_dim, window);
+    AFTER_REQUIRE(!workspace || (((size_t)workspace & 15) == 0 && workspace_bytes >= p.bytes), AFTER_E_CAPACITY,
+                  "attend_packed: a workspace has to be 16-byte aligned, here of %lld bytes (got %lld)", p.bytes, workspace_bytes);
+    if (!workspace) p.splits = 1;
+    a.tiles = p.tiles, a.splits = p.splits, a.by_splits = divisor(p.splits);
+    a.part_ml = (f32x2*)workspace, a.part_o = (float*)((char*)workspace + p.ml_bytes);
     a.scale2 = std::fmax(std::fabs(scale) * 1.44269504088896340736f, 1e-30f);
     a.q_sign = scale < 0 ? (type == AFTER_T_F32 ? 0x80000000u : 0x80008000u) : 0u;
     a.causal = causal != 0, a.window = window < (1 << 30) ? window : 1 << 30, a.zero_rest = zero_rest;
     a.by_group = divisor(group), a.by_chunk = divisor(chunk), a.by_kv_heads = divisor(kv_heads);
-    // (a grid's threads are counted in 32 bits)
-    AFTER_REQUIRE((long long)a.tiles * kv_heads < (1 << 24), AFTER_E_INVALID, "attend_packed: too many tokens x heads for one call");
     hipStream_t s = (hipStream_t)stream;
     if (head_dim == 64) {
-        if (type == AFTER_T_F32) return run_packed<AFTER_T_F32, 64>(a, s);
-        if (type == AFTER_T_BF16) return run_packed<AFTER_T_BF16, 64>(a, s);
-        return run_packed<AFTER_T_F16, 64>(a, s);
+        if (type == AFTER_T_F32) return run_packed<AFTER_T_F32, 64>(a, p.few, s);
+        if (type == AFTER_T_BF16) return run_packed<AFTER_T_BF16, 64>(a, p.few, s);
+        return run_packed<AFTER_T_F16, 64>(a, p.few, s);
     }
-    if (type == AFTER_T_F32) return run_packed<AFTER_T_F32, 128>(a, s);
-    if (type == AFTER_T_BF16) return run_packed<AFTER_T_BF16, 128>(a, s);
-    return run_packed<AFTER_T_F16, 128>(a, s);
+    if (type == AFTER_T_F32) return run_packed<AFTER_T_F32, 128>(a, p.few, s);
+    if (type == AFTER_T_BF16) return run_packed<AFTER_T_BF16, 128>(a, p.few, s);
+    return run_packed<AFTER_T_F16, 128>(a, p.few, s);
 }

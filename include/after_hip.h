@@ -580,12 +580,17 @@ long long after_conv1_act_launches(void);
  * before (chunk = 1: the keys up to its own), and with window > 0 of the earlier chunks only keys > p - window, as DenoiserV2's
  * mask does (transformerv2.py:62-96).  causal = 0: all keys.  A query that sees no key gets zeros; what a query does not see
  * has no effect on it, NaN and infinities included.  Rows of out behind the last sequence stay as they are, or are set to
- * zero with zero_rest.  D = 64 or 128.  fp32: fp32 products; bf16 / fp16: products of that type, sums and softmax in fp32. */
+ * zero with zero_rest.  D = 64 or 128.  fp32: fp32 products; bf16 / fp16: products of that type, sums and softmax in fp32.
+ * workspace: scratch of the size that _workspace names (its answer depends on the arguments alone; two calls that may run at the
+ * same time need two), with which the keys of a few queries are shared out over the chip; NULL: they are not. */
+int after_attend_packed_workspace(int type, long long q_rows, long long k_rows, int n_seqs, int heads, int kv_heads, int head_dim,
+                                  int window, long long* bytes);
 int after_attend_packed(const void* q, const void* k, const void* v, void* out, int type, long long q_rows, long long k_rows,
                         const int* q_starts, const int* k_starts, int n_seqs, int heads, int kv_heads, int head_dim,
                         long long q_token_stride, long long q_head_stride, long long k_token_stride, long long k_head_stride,
                         long long v_token_stride, long long v_head_stride, long long out_token_stride, long long out_head_stride,
-                        float scale, int causal, int window, int chunk, int zero_rest, void* stream);
+                        float scale, int causal, int window, int chunk, int zero_rest, void* workspace, long long workspace_bytes,
+                        void* stream);
 
 /* A cache of keys and values in four bits.  The caller owns the (device) buffers; the struct itself is passed from the host.
  * 32 neighbouring channels of a token share one scale byte b, 2^(b - 127): the smallest power of two (16 <= b <= 252) with

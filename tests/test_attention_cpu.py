@@ -17,10 +17,10 @@ def error():
 
 def packed(**k):
     a = dict(q=P, k=P, v=P, out=P, type=1, q_rows=8, k_rows=8, qs=P, ks=P, n=1, heads=4, kv=2, dim=64, strides=[256, 64, 128, 64, 128, 64, 256, 64],
-             scale=0.1, causal=1, window=0, chunk=1, rest=0)
+             scale=0.1, causal=1, window=0, chunk=1, rest=0, work=None, bytes=0)
     a.update(k)
     return _lib.lib().after_attend_packed(a["q"], a["k"], a["v"], a["out"], a["type"], a["q_rows"], a["k_rows"], a["qs"], a["ks"], a["n"], a["heads"],
-                                          a["kv"], a["dim"], *a["strides"], a["scale"], a["causal"], a["window"], a["chunk"], a["rest"], None)
+                                          a["kv"], a["dim"], *a["strides"], a["scale"], a["causal"], a["window"], a["chunk"], a["rest"], a["work"], a["bytes"], None)
 
 
 @pytest.mark.parametrize("bad", [
@@ -31,6 +31,21 @@ def packed(**k):
     dict(q_rows=(1 << 24), n=1 << 24, heads=512, kv=512)])
 def test_packed_refuses(bad):
     assert packed(**bad) == E_INVALID and "attend_packed" in error()
+
+
+def test_packed_workspace():
+    """Only few queries over many keys take one, and its size is checked."""
+    L, n = _lib.lib(), ctypes.c_longlong()
+    size = lambda *a: (L.after_attend_packed_workspace(1, *a, ctypes.byref(n)), n.value)
+    assert size(8, 8, 1, 4, 2, 64, 0) == (0, 0) and size(1 << 20, 1 << 20, 1, 4, 2, 64, 0) == (0, 0) and size(8, 1 << 20, 0, 4, 2, 64, 0) == (0, 0)
+    assert size(1, 1 << 16, 1, 4, 2, 64, 8) == (0, 0)  # a window leaves few keys
+    rc, need = size(1, 1 << 16, 1, 4, 2, 64, 0)
+    assert rc == 0 and 0 < need < 1 << 26 and need % 16 == 0
+    few = dict(q_rows=1, k_rows=1 << 16)
+    assert packed(**few, work=P, bytes=need - 1) == E_CAPACITY and packed(**few, work=P + 8, bytes=need) == E_CAPACITY and "workspace" in error()
+    assert size(-1, 8, 1, 4, 2, 64, 0)[0] == E_INVALID and size(8, 8, 1, 4, 3, 64, 0)[0] == E_INVALID and size(8, 8, 1, 4, 2, 96, 0)[0] == E_INVALID
+    assert L.after_attend_packed_workspace(3, 8, 8, 1, 4, 2, 64, 0, ctypes.byref(n)) == E_INVALID
+    assert L.after_attend_packed_workspace(1, 8, 8, 1, 4, 2, 64, 0, None) == E_INVALID
 
 
 def test_packed_without_queries_is_a_no_op():

@@ -2,6 +2,7 @@
 
 Tolerances: tests/attention_ref.py derives them from the operands: each rounding to the output's type counts half a step, 32-bit
 sums 2^-24 per term.  Everything that is a choice or a code (slots, scale bytes, nibbles, lengths) has to be equal."""
+import ctypes
 import math
 
 import pytest
@@ -72,6 +73,67 @@ def test_prompts(hip_device, kind, dim, qs, ks, heads, kv, causal, window, chunk
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("qs, ks, heads, kv, causal, window, chunk", [
+    ([5, 0, 1, 70], None, 4, 2, True, None, 1),
+    ([64, 129, 2], None, 2, 2, True, None, 1),
+    ([1, 3, 40], [77, 3, 200], 6, 2, True, None, 1),
+    ([100, 33], None, 2, 1, True, 8, 4),
+    ([66], [131], 2, 2, True, 16, 4),
+    ([9, 40], [65, 7], 2, 1, False, None, 1),
+    ([70, 3], [6, 1], 3, 3, True, 5, 1)])
+def test_prompts_that_fill_the_chip(hip_device, kind, dim, qs, ks, heads, kv, causal, window, chunk):
+    """The same sequences many times over, with other values: tiles of 128 rows instead of 32."""
+    ks, t, many = ks or qs, TYPES[kind], 600 // (len(qs) * kv) + 1
+    q, k, v = (torch.randn(n * many, h, dim, generator=gen(80 + i)).to(hip_device, t) for i, (n, h) in enumerate(((sum(qs), heads), (sum(ks), kv), (sum(ks), kv))))
+    out = attend_packed(q, k, v, starts(qs * many, hip_device), starts(ks * many, hip_device), causal=causal, window=window, chunk=chunk)
+    for i in (0, 1, many // 3, many - 1):
+        a, b = slice(i * sum(qs), (i + 1) * sum(qs)), slice(i * sum(ks), (i + 1) * sum(ks))
+        check_packed(out[a], q[a], k[b], v[b], qs, ks, dim ** -0.5, causal, window, chunk)
+    assert not torch.isnan(out).any()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("qs, ks, heads, kv, causal", [
+    ([1], [9000], 8, 2, True),                          # one new token
+    ([3, 1, 0, 2, 1], [4000, 33, 50, 2100, 6000], 4, 1, True),  # rows of very different lengths
+    ([1, 1], [5000, 0], 2, 2, False),
+    ([40], [5001], 4, 4, False),                        # two tiles, the second one ragged
+    ([2600], None, 1, 1, True),                         # a prompt: the first tiles have few keys
+    ([1], [1 << 17], 2, 1, True)])
+def test_few_queries_over_many_keys(hip_device, kind, dim, qs, ks, heads, kv, causal):
+    """The keys are shared out over the chip and joined."""
+    ks, t, n = ks or qs, TYPES[kind], ctypes.c_longlong()
+    _lib.lib().after_attend_packed_workspace(list(TYPES).index(kind), sum(qs), sum(ks), len(qs), heads, kv, dim, 0, ctypes.byref(n))
+    assert n.value > 0
+    q, k, v = (torch.randn(x, h, dim, generator=gen(90 + i)).to(hip_device, t) for i, (x, h) in enumerate(((sum(qs) + 2, heads), (sum(ks), kv), (sum(ks), kv))))
+    out = attend_packed(q, k, v, starts(qs, hip_device), starts(ks, hip_device), causal=causal)
+    assert (out[sum(qs):] == 0).all()
+    if qs == ks:  # (the whole of it would take the reference long)
+        for i in (0, 31, 32, 1000, 2599):
+            check_packed(out[i:i + 1], q[i:i + 1], k[:i + 1], v[:i + 1], [1], [i + 1], dim ** -0.5)
+    else:
+        check_packed(out[:sum(qs)], q[:sum(qs)], k, v, qs, ks, dim ** -0.5, causal)
+    kept = torch.full_like(out, 7.0)
+    attend_packed(q, k, v, starts(qs, hip_device), starts(ks, hip_device), causal=causal, out=kept)
+    assert torch.equal(kept[:sum(qs)], out[:sum(qs)]) and (kept[sum(qs):] == 7).all()
+
+
+def test_a_share_of_the_keys_with_nan(hip_device):
+    """In a piece of the keys: NaN and infinities reach the queries that see them, and no other."""
+    q, k, v = (torch.randn(n, 1, 64, generator=gen(n)).to(hip_device, torch.bfloat16) for n in (2, 8002, 8003))
+    s, ks = starts([1, 1], hip_device), starts([4001, 4001], hip_device)
+    v = v[:8002]
+    good = attend_packed(q, k, v, s, ks)
+    v2, k2 = v.clone(), k.clone()
+    v2[2000, :, 5], v2[4000, :, 6], k2[4001 + 3000, :, 9] = math.inf, math.nan, math.nan
+    out = attend_packed(q, k2, v2, s, ks)
+    assert torch.isnan(out[1]).all() and out[0, 0, 5] == math.inf and torch.isnan(out[0, 0, 6])
+    assert torch.equal(out[0, 0, 7:], good[0, 0, 7:])
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
 def test_prompt_of_a_few_thousand_tokens(hip_device, kind):
     """The last and a middle query of a long sequence, whose keys fill many tiles."""
     g, t, n = gen(1), TYPES[kind], 2500
@@ -83,10 +145,12 @@ def test_prompt_of_a_few_thousand_tokens(hip_device, kind):
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
-def test_what_a_query_does_not_see_has_no_effect(hip_device, kind):
-    """Infinities and NaN in later keys and values, in other sequences and behind the last one: the results are those without them."""
+@pytest.mark.parametrize("empty", [0, 300])
+def test_what_a_query_does_not_see_has_no_effect(hip_device, kind, empty):
+    """Infinities and NaN in later keys and values, in other sequences and behind the last one: the results are those without them.
+    (With many sequences, empty ones, the tiles have 128 rows.)"""
     g, t = gen(2), TYPES[kind]
-    lens = [70, 50]
+    lens = [70, 50] + [0] * empty
     q, k, v = (torch.randn(130, h, 64, generator=g).to(hip_device, t) for h in (4, 2, 2))
     s = starts(lens, hip_device)
     good = attend_packed(q, k, v, s)
