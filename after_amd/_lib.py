@@ -4,6 +4,7 @@ There is deliberately NO fallback: if the HIP library is missing or fails to
 load, every product entry point raises."""
 import ctypes
 import os
+import struct
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_longlong, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -51,6 +52,23 @@ class EcapaCfg(ctypes.Structure):
 class KV4(ctypes.Structure):
     _fields_ = [(n, c_void_p) for n in ("keys", "key_scales", "values", "value_scales", "weights", "lengths", "failed")] + \
                [(n, c_int) for n in ("rows", "kv_heads", "head_dim", "capacity")]
+
+
+# (struct.Struct packs these two several times faster than ctypes passes as many arguments)
+class Packed(ctypes.Structure):
+    FORMAT = struct.Struct("@7Q11q5if4i")
+    _fields_ = [(n, c_void_p) for n in ("q", "k", "v", "out", "q_starts", "k_starts", "workspace")] + \
+               [(n, ctypes.c_longlong) for n in ("workspace_bytes", "q_rows", "k_rows", "q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+                                                 "v_token_stride", "v_head_stride", "out_token_stride", "out_head_stride")] + \
+               [(n, c_int) for n in ("type", "n_seqs", "heads", "kv_heads", "head_dim")] + [("scale", c_float)] + \
+               [(n, c_int) for n in ("causal", "window", "chunk", "zero_rest")]
+
+
+class KV4Query(ctypes.Structure):
+    FORMAT = struct.Struct("@3Q4q3ifif")
+    _fields_ = [(n, c_void_p) for n in ("q", "out", "workspace")] + \
+               [(n, ctypes.c_longlong) for n in ("workspace_bytes", "q_row_stride", "q_token_stride", "q_head_stride")] + \
+               [(n, c_int) for n in ("type", "heads", "tokens")] + [("scale", c_float), ("accumulate", c_int), ("decay", c_float)]
 
 
 class AFTERHipError(RuntimeError):
@@ -154,15 +172,13 @@ SIGNATURES = {
     "after_gemm_x6_offset": (ctypes.c_longlong, [c_int, c_int, c_int, c_int]),
     "after_gemm_x6": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int,
                               c_int, c_int, c_int, c_int, c_void_p]),
-    "after_attend_packed": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_void_p, c_void_p,
-                                    c_int, c_int, c_int, c_int] + [c_longlong] * 8 + [c_float, c_int, c_int, c_int, c_int, c_void_p, c_longlong, c_void_p]),
+    "after_attend_packed": (c_int, [c_char_p, c_void_p]),  # (the struct's bytes)
     "after_attend_packed_workspace": (c_int, [c_int, c_longlong, c_longlong] + [c_int] * 5 + [POINTER(c_longlong)]),
     "after_kv4_append": (c_int, [POINTER(KV4), c_void_p, c_void_p, c_int, c_void_p, c_int] + [c_longlong] * 5 + [c_void_p]),
     "after_kv4_truncate": (c_int, [POINTER(KV4), c_void_p, c_void_p]),
     "after_kv4_read": (c_int, [POINTER(KV4), c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p]),
     "after_kv4_attend_workspace": (c_int, [POINTER(KV4), c_int, c_int, c_int, c_int, POINTER(c_longlong)]),
-    "after_kv4_attend": (c_int, [POINTER(KV4), c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong, c_float,
-                                 c_int, c_float, c_void_p, c_longlong, c_void_p]),
+    "after_kv4_attend": (c_int, [POINTER(KV4), c_char_p, c_void_p]),
     "after_kv4_evict": (c_int, [POINTER(KV4), POINTER(KV4), c_int, c_int, c_void_p, c_void_p]),
 }
 

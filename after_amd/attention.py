@@ -85,8 +85,8 @@ def _share(a, b):
 
 def _scale(scale, dim):
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, got {scale}")
+    if not abs(scale) < 3e38:
+        raise ValueError(f"scale must be finite in 32 bits, got {scale}")
     return scale
 
 
@@ -145,9 +145,10 @@ def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=True, window=None,
     size = _packed_workspace(kind, n, keys, seqs, heads, kv_heads, dim, window)
     work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None  # (as in KVCache4.attend)
     q_at, k_at, v_at = q.stride(), k.stride(), v.stride()
-    _enqueue("after_attend_packed", index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), kind, n, keys, q_starts.data_ptr(),
-             k_starts.data_ptr(), seqs, heads, kv_heads, dim, q_at[0], q_at[1], k_at[0], k_at[1], v_at[0], v_at[1], heads * dim, dim, scale,
-             1 if causal else 0, window, chunk, 1 if fresh else 0, work.data_ptr() if size else None, size)
+    _enqueue("after_attend_packed", index, _lib.Packed.FORMAT.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q_starts.data_ptr(), k_starts.data_ptr(), work.data_ptr() if size else 0, size,
+        n, keys, q_at[0], q_at[1], k_at[0], k_at[1], v_at[0], v_at[1], heads * dim, dim, kind, seqs, heads, kv_heads, dim, scale,
+        1 if causal else 0, window, chunk, 1 if fresh else 0))
     return out
 
 
@@ -215,7 +216,7 @@ class KVCache4:
         return dict(self._tensors)
 
     def _row_values(self, t, name):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != (self.rows, ) or t.device != self.device:
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != self.rows or t.get_device() != self._index:
             raise ValueError(f"{name} must be an int32 tensor ({self.rows},) on {self.device}")
         return t.contiguous()
 
@@ -226,18 +227,26 @@ class KVCache4:
         dims = 4 if starts is None else 3
         k = _operand(k, "k", dims, self._index)
         v = _operand(v, "v", dims, self._index, k.dtype)
-        if k.shape != v.shape or tuple(k.shape[-2:]) != (self.kv_heads, self.head_dim) or (starts is None and k.shape[0] != self.rows):
+        *outer, heads, dim = k.shape
+        if k.shape != v.shape or heads != self.kv_heads or dim != self.head_dim or (starts is None and outer[0] != self.rows):
             raise ValueError(f"bad shapes k{tuple(k.shape)} v{tuple(v.shape)} for {self.rows} rows of {self.kv_heads} heads of {self.head_dim}")
-        tokens = 0
+        k_at, v_at = k.stride(), v.stride()
+        tokens, total = 0, outer[0]
         if starts is None:
-            tokens = k.shape[1]
+            tokens = outer[1]
             if tokens > self.capacity:
                 raise ValueError(f"{tokens} new tokens, the cache has {self.capacity} slots per row")
-            k, v = k.flatten(0, 1), v.flatten(0, 1)
+            total *= tokens
+            # (one token of each row, as a rule: its rows are the tokens)
+            if tokens == 1:
+                k_at, v_at = (k_at[0], k_at[2]), (v_at[0], v_at[2])
+            else:
+                k, v = k.flatten(0, 1), v.flatten(0, 1)
+                k_at, v_at = k.stride(), v.stride()
         else:
             starts = _starts(starts, "starts", self.rows, self._index)
         _enqueue("after_kv4_append", self._index, self._ref, k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], None if starts is None else starts.data_ptr(),
-                 tokens, k.shape[0], *k.stride()[:2], *v.stride()[:2])
+                 tokens, total, k_at[0], k_at[1], v_at[0], v_at[1])
 
     def truncate(self, lengths=None):
         """Takes back the newest slots: row r keeps the first lengths[r] (int32 [rows] on the device); None empties the cache."""
@@ -269,8 +278,8 @@ class KVCache4:
         if rows != self.rows or dim != self.head_dim or heads == 0 or heads % self.kv_heads:
             raise ValueError(f"bad shape q{tuple(q.shape)} for {self.rows} rows of {self.kv_heads} key heads of {self.head_dim}")
         scale, decay = _scale(scale, dim), float(decay)
-        if not math.isfinite(decay):
-            raise ValueError(f"decay must be finite, got {decay}")
+        if not abs(decay) < 3e38:
+            raise ValueError(f"decay must be finite in 32 bits, got {decay}")
         out = torch.empty(rows, tokens, heads, dim, dtype=q.dtype, device=self.device)
         if tokens == 0:
             if accumulate and decay != 1.0:
@@ -285,8 +294,8 @@ class KVCache4:
         # (scratch of this call: the allocator gives it to later calls of this stream only, and to a captured graph its own)
         size = self._work[key]
         work = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
-        _enqueue("after_kv4_attend", self._index, self._ref, q.data_ptr(), out.data_ptr(), _TYPES[q.dtype], heads, tokens, *q.stride()[:3],
-                 scale, accumulate, decay, None if work is None else work.data_ptr(), size)
+        _enqueue("after_kv4_attend", self._index, self._ref, _lib.KV4Query.FORMAT.pack(
+            q.data_ptr(), out.data_ptr(), work.data_ptr() if size else 0, size, *q.stride()[:3], _TYPES[q.dtype], heads, tokens, scale, accumulate, decay))
         return out
 
     def evict(self, into, keep, recent=0):

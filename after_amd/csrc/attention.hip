@@ -791,46 +791,44 @@ extern "C" int after_attend_packed_workspace(int type, long long q_rows, long lo
     return AFTER_OK;
 }
 
-extern "C" int after_attend_packed(const void* q, const void* k, const void* v, void* out, int type, long long q_rows, long long k_rows,
-                                   const int* q_starts, const int* k_starts, int n_seqs, int heads, int kv_heads, int head_dim,
-                                   long long q_token_stride, long long q_head_stride, long long k_token_stride, long long k_head_stride,
-                                   long long v_token_stride, long long v_head_stride, long long out_token_stride, long long out_head_stride,
-                                   float scale, int causal, int window, int chunk, int zero_rest, void* workspace, long long workspace_bytes, void* stream) {
-    AFTER_TRY(check_sizes(type, q_rows, k_rows, n_seqs, heads, kv_heads, head_dim, window));
-    const int group = heads / kv_heads;
-    AFTER_REQUIRE(std::isfinite(scale), AFTER_E_INVALID, "attend_packed: scale must be finite");
-    AFTER_REQUIRE(window >= 0 && chunk >= 1 && chunk <= (1 << 24) && (causal || (window == 0 && chunk == 1)), AFTER_E_INVALID,
+extern "C" int after_attend_packed(const after_packed* call, void* stream) {
+    AFTER_REQUIRE(call, AFTER_E_INVALID, "attend_packed: no call");
+    const after_packed& c = *call;
+    AFTER_TRY(check_sizes(c.type, c.q_rows, c.k_rows, c.n_seqs, c.heads, c.kv_heads, c.head_dim, c.window));
+    const int group = c.heads / c.kv_heads;
+    AFTER_REQUIRE(std::isfinite(c.scale), AFTER_E_INVALID, "attend_packed: scale must be finite");
+    AFTER_REQUIRE(c.window >= 0 && c.chunk >= 1 && c.chunk <= (1 << 24) && (c.causal || (c.window == 0 && c.chunk == 1)), AFTER_E_INVALID,
                   "attend_packed: window >= 0 (0: none) and chunk >= 1, both for causal attention only");
-    if (q_rows == 0) return AFTER_OK;
-    const int per16 = 16 / (type == AFTER_T_F32 ? 4 : 2);
-    const long long strides = q_token_stride | q_head_stride | k_token_stride | k_head_stride | v_token_stride | v_head_stride | out_token_stride | out_head_stride;
-    AFTER_REQUIRE(q && out && q_starts && k_starts && (k_rows == 0 || (k && v)), AFTER_E_INVALID, "attend_packed: a pointer is NULL");
-    AFTER_REQUIRE((((size_t)q | (size_t)k | (size_t)v | (size_t)out) & 15) == 0 && (strides & (per16 - 1)) == 0, AFTER_E_INVALID,
+    if (c.q_rows == 0) return AFTER_OK;
+    const int per16 = 16 / (c.type == AFTER_T_F32 ? 4 : 2);
+    const long long strides = c.q_token_stride | c.q_head_stride | c.k_token_stride | c.k_head_stride | c.v_token_stride | c.v_head_stride | c.out_token_stride | c.out_head_stride;
+    AFTER_REQUIRE(c.q && c.out && c.q_starts && c.k_starts && (c.k_rows == 0 || (c.k && c.v)), AFTER_E_INVALID, "attend_packed: a pointer is NULL");
+    AFTER_REQUIRE((((size_t)c.q | (size_t)c.k | (size_t)c.v | (size_t)c.out) & 15) == 0 && (strides & (per16 - 1)) == 0, AFTER_E_INVALID,
                   "attend_packed: q, k, v, out and their token and head strides must be multiples of 16 bytes");
-    AFTER_REQUIRE(k_token_stride >= 0 && v_token_stride >= 0 && k_token_stride < (1 << 22) && v_token_stride < (1 << 22), AFTER_E_INVALID,
+    AFTER_REQUIRE(c.k_token_stride >= 0 && c.v_token_stride >= 0 && c.k_token_stride < (1 << 22) && c.v_token_stride < (1 << 22), AFTER_E_INVALID,
                   "attend_packed: the token strides of k and v must be below 2^22 elements");
     PackedArgs a;
-    a.q = q, a.k = k, a.v = v, a.out = out, a.qs = q_starts, a.ks = k_starts;
-    a.qts = q_token_stride, a.qhs = q_head_stride, a.kts = k_token_stride, a.khs = k_head_stride;
-    a.vts = v_token_stride, a.vhs = v_head_stride, a.ots = out_token_stride, a.ohs = out_head_stride;
-    a.q_rows = (int)q_rows, a.k_rows = (int)k_rows, a.n_seqs = n_seqs, a.heads = heads, a.kv_heads = kv_heads, a.group = group;
-    PackedPlan p = packed_plan(type, q_rows, k_rows, n_seqs, heads, kv_heads, head_dim, window);
-    AFTER_REQUIRE(!workspace || (((size_t)workspace & 15) == 0 && workspace_bytes >= p.bytes), AFTER_E_CAPACITY,
-                  "attend_packed: a workspace has to be 16-byte aligned, here of %lld bytes (got %lld)", p.bytes, workspace_bytes);
-    if (!workspace) p.splits = 1;
+    a.q = c.q, a.k = c.k, a.v = c.v, a.out = c.out, a.qs = c.q_starts, a.ks = c.k_starts;
+    a.qts = c.q_token_stride, a.qhs = c.q_head_stride, a.kts = c.k_token_stride, a.khs = c.k_head_stride;
+    a.vts = c.v_token_stride, a.vhs = c.v_head_stride, a.ots = c.out_token_stride, a.ohs = c.out_head_stride;
+    a.q_rows = (int)c.q_rows, a.k_rows = (int)c.k_rows, a.n_seqs = c.n_seqs, a.heads = c.heads, a.kv_heads = c.kv_heads, a.group = group;
+    PackedPlan p = packed_plan(c.type, c.q_rows, c.k_rows, c.n_seqs, c.heads, c.kv_heads, c.head_dim, c.window);
+    AFTER_REQUIRE(!c.workspace || (((size_t)c.workspace & 15) == 0 && c.workspace_bytes >= p.bytes), AFTER_E_CAPACITY,
+                  "attend_packed: a workspace has to be 16-byte aligned, here of %lld bytes (got %lld)", p.bytes, c.workspace_bytes);
+    if (!c.workspace) p.splits = 1;
     a.tiles = p.tiles, a.splits = p.splits, a.by_splits = divisor(p.splits);
-    a.part_ml = (f32x2*)workspace, a.part_o = (float*)((char*)workspace + p.ml_bytes);
-    a.scale2 = std::fmax(std::fabs(scale) * 1.44269504088896340736f, 1e-30f);
-    a.q_sign = scale < 0 ? (type == AFTER_T_F32 ? 0x80000000u : 0x80008000u) : 0u;
-    a.causal = causal != 0, a.window = window < (1 << 30) ? window : 1 << 30, a.zero_rest = zero_rest;
-    a.by_group = divisor(group), a.by_chunk = divisor(chunk), a.by_kv_heads = divisor(kv_heads);
+    a.part_ml = (f32x2*)c.workspace, a.part_o = (float*)((char*)c.workspace + p.ml_bytes);
+    a.scale2 = std::fmax(std::fabs(c.scale) * 1.44269504088896340736f, 1e-30f);
+    a.q_sign = c.scale < 0 ? (c.type == AFTER_T_F32 ? 0x80000000u : 0x80008000u) : 0u;
+    a.causal = c.causal != 0, a.window = c.window < (1 << 30) ? c.window : 1 << 30, a.zero_rest = c.zero_rest;
+    a.by_group = divisor(group), a.by_chunk = divisor(c.chunk), a.by_kv_heads = divisor(c.kv_heads);
     hipStream_t s = (hipStream_t)stream;
-    if (head_dim == 64) {
-        if (type == AFTER_T_F32) return run_packed<AFTER_T_F32, 64>(a, p.few, s);
-        if (type == AFTER_T_BF16) return run_packed<AFTER_T_BF16, 64>(a, p.few, s);
+    if (c.head_dim == 64) {
+        if (c.type == AFTER_T_F32) return run_packed<AFTER_T_F32, 64>(a, p.few, s);
+        if (c.type == AFTER_T_BF16) return run_packed<AFTER_T_BF16, 64>(a, p.few, s);
         return run_packed<AFTER_T_F16, 64>(a, p.few, s);
     }
-    if (type == AFTER_T_F32) return run_packed<AFTER_T_F32, 128>(a, p.few, s);
-    if (type == AFTER_T_BF16) return run_packed<AFTER_T_BF16, 128>(a, p.few, s);
+    if (c.type == AFTER_T_F32) return run_packed<AFTER_T_F32, 128>(a, p.few, s);
+    if (c.type == AFTER_T_BF16) return run_packed<AFTER_T_BF16, 128>(a, p.few, s);
     return run_packed<AFTER_T_F16, 128>(a, p.few, s);
 }

@@ -1530,41 +1530,41 @@ extern "C" int after_kv4_attend_workspace(const after_kv4* c, int type, int head
     return AFTER_OK;
 }
 
-extern "C" int after_kv4_attend(const after_kv4* c, const void* q, void* out, int type, int heads, int tokens, long long q_row_stride,
-                                long long q_token_stride, long long q_head_stride, float scale, int accumulate, float decay, void* workspace,
-                                long long workspace_bytes, void* stream) {
-    AFTER_TRY(check_attend(c, type, heads, tokens, "kv4_attend"));
-    const int per16 = 16 / type_bytes(type);
-    AFTER_REQUIRE(q && out && aligned16(q) && aligned16(out) && q_row_stride % per16 == 0 && q_token_stride % per16 == 0 && q_head_stride % per16 == 0,
+extern "C" int after_kv4_attend(const after_kv4* c, const after_kv4_query* query, void* stream) {
+    AFTER_REQUIRE(query, AFTER_E_INVALID, "kv4_attend: no query");
+    const after_kv4_query& x = *query;
+    AFTER_TRY(check_attend(c, x.type, x.heads, x.tokens, "kv4_attend"));
+    const int per16 = 16 / type_bytes(x.type);
+    AFTER_REQUIRE(x.q && x.out && aligned16(x.q) && aligned16(x.out) && x.q_row_stride % per16 == 0 && x.q_token_stride % per16 == 0 && x.q_head_stride % per16 == 0,
                   AFTER_E_INVALID, "kv4_attend: q, its strides and out must be 16-byte aligned");
-    AFTER_REQUIRE(std::isfinite(scale) && std::isfinite(decay), AFTER_E_INVALID, "kv4_attend: scale and decay must be finite");
-    const bool count = accumulate != 0;
-    const Plan p = attend_plan(*c, type, heads, tokens, count);
+    AFTER_REQUIRE(std::isfinite(x.scale) && std::isfinite(x.decay), AFTER_E_INVALID, "kv4_attend: scale and decay must be finite");
+    const bool count = x.accumulate != 0;
+    const Plan p = attend_plan(*c, x.type, x.heads, x.tokens, count);
     const long long need = p.total();
-    AFTER_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need), AFTER_E_CAPACITY,
-                  "kv4_attend: needs a 16-byte aligned workspace of %lld bytes (got %lld)", need, workspace_bytes);
+    AFTER_REQUIRE(need == 0 || (x.workspace && aligned16(x.workspace) && x.workspace_bytes >= need), AFTER_E_CAPACITY,
+                  "kv4_attend: needs a 16-byte aligned workspace of %lld bytes (got %lld)", need, x.workspace_bytes);
     AttendArgs a;
     a.c = *c;
-    a.q = q;
-    a.out = out;
-    a.qrs = q_row_stride;
-    a.qts = q_token_stride;
-    a.qhs = q_head_stride;
-    a.heads = heads;
-    a.tokens = tokens;
-    a.group = heads / c->kv_heads;
+    a.q = x.q;
+    a.out = x.out;
+    a.qrs = x.q_row_stride;
+    a.qts = x.q_token_stride;
+    a.qhs = x.q_head_stride;
+    a.heads = x.heads;
+    a.tokens = x.tokens;
+    a.group = x.heads / c->kv_heads;
     a.m_rows = p.m_rows;
     a.workers = 4 * p.wgs;
-    a.scale2 = std::fmax(std::fabs(scale) * 1.44269504088896340736f, 1e-30f);
-    a.q_sign = scale < 0 ? -1.f : 1.f;
-    char* w = (char*)workspace;
+    a.scale2 = std::fmax(std::fabs(x.scale) * 1.44269504088896340736f, 1e-30f);
+    a.q_sign = x.scale < 0 ? -1.f : 1.f;
+    char* w = (char*)x.workspace;
     a.scores = (float*)w;
     a.part_ml = (f32x2*)(w += p.s_bytes);
     a.final_ml = count ? (f32x2*)(w + p.ml_bytes) : nullptr;
     a.ends = (int2*)(w += p.ml_bytes + p.f_bytes);
     a.part_o = (float*)(w += p.e_bytes);
-#define CALL(T, D) return run_attend<T, D>(a, p, count, decay, (hipStream_t)stream)
-    KV4_BY_TYPE(type, c->head_dim, CALL);
+#define CALL(T, D) return run_attend<T, D>(a, p, count, x.decay, (hipStream_t)stream)
+    KV4_BY_TYPE(x.type, c->head_dim, CALL);
 #undef CALL
     return AFTER_OK;
 }

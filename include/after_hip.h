@@ -585,12 +585,24 @@ long long after_conv1_act_launches(void);
  * same time need two), with which the keys of a few queries are shared out over the chip; NULL: they are not. */
 int after_attend_packed_workspace(int type, long long q_rows, long long k_rows, int n_seqs, int heads, int kv_heads, int head_dim,
                                   int window, long long* bytes);
-int after_attend_packed(const void* q, const void* k, const void* v, void* out, int type, long long q_rows, long long k_rows,
-                        const int* q_starts, const int* k_starts, int n_seqs, int heads, int kv_heads, int head_dim,
-                        long long q_token_stride, long long q_head_stride, long long k_token_stride, long long k_head_stride,
-                        long long v_token_stride, long long v_head_stride, long long out_token_stride, long long out_head_stride,
-                        float scale, int causal, int window, int chunk, int zero_rest, void* workspace, long long workspace_bytes,
-                        void* stream);
+typedef struct after_packed {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    const int* q_starts;
+    const int* k_starts;
+    void* workspace; /* or NULL */
+    long long workspace_bytes;
+    long long q_rows, k_rows;
+    long long q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride, out_token_stride, out_head_stride;
+    int type;
+    int n_seqs, heads, kv_heads, head_dim;
+    float scale;
+    int causal, window, chunk;
+    int zero_rest;
+} after_packed;
+int after_attend_packed(const after_packed* call, void* stream);
 
 /* A cache of keys and values in four bits.  The caller owns the (device) buffers; the struct itself is passed from the host.
  * 32 neighbouring channels of a token share one scale byte b, 2^(b - 127): the smallest power of two (16 <= b <= 252) with
@@ -635,9 +647,19 @@ int after_kv4_read(const after_kv4* c, void* k, void* v, int type, const int* st
  * in use received, summed over tokens and the group's heads (decay = 0: they are replaced).  The workspace is scratch: its
  * size depends on the arguments alone, and two calls that may run at the same time need two. */
 int after_kv4_attend_workspace(const after_kv4* c, int type, int heads, int tokens, int accumulate, long long* bytes);
-int after_kv4_attend(const after_kv4* c, const void* q, void* out, int type, int heads, int tokens, long long q_row_stride,
-                     long long q_token_stride, long long q_head_stride, float scale, int accumulate, float decay, void* workspace,
-                     long long workspace_bytes, void* stream);
+typedef struct after_kv4_query {
+    const void* q;
+    void* out;
+    void* workspace;
+    long long workspace_bytes;
+    long long q_row_stride, q_token_stride, q_head_stride;
+    int type;
+    int heads, tokens;
+    float scale;
+    int accumulate;
+    float decay;
+} after_kv4_query;
+int after_kv4_attend(const after_kv4* c, const after_kv4_query* query, void* stream);
 /* Moves, per row and head, min(length, keep) slots into the cache `to` (same rows, kv_heads, head_dim; its former content is
  * replaced), in their order: the `recent` newest, and of the others those with the largest weights (NaN counts as the
  * smallest; ties go to the lower slot).  slots [rows, kv_heads, keep]: where each came from, -1 past the new length.  `c` stays as it is. */

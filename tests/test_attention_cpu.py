@@ -19,8 +19,19 @@ def packed(**k):
     a = dict(q=P, k=P, v=P, out=P, type=1, q_rows=8, k_rows=8, qs=P, ks=P, n=1, heads=4, kv=2, dim=64, strides=[256, 64, 128, 64, 128, 64, 256, 64],
              scale=0.1, causal=1, window=0, chunk=1, rest=0, work=None, bytes=0)
     a.update(k)
-    return _lib.lib().after_attend_packed(a["q"], a["k"], a["v"], a["out"], a["type"], a["q_rows"], a["k_rows"], a["qs"], a["ks"], a["n"], a["heads"],
-                                          a["kv"], a["dim"], *a["strides"], a["scale"], a["causal"], a["window"], a["chunk"], a["rest"], a["work"], a["bytes"], None)
+    call = _lib.Packed(a["q"], a["k"], a["v"], a["out"], a["qs"], a["ks"], a["work"], a["bytes"], a["q_rows"], a["k_rows"], *a["strides"], a["type"],
+                       a["n"], a["heads"], a["kv"], a["dim"], a["scale"], a["causal"], a["window"], a["chunk"], a["rest"])
+    return _lib.lib().after_attend_packed(bytes(call), None)
+
+
+@pytest.mark.parametrize("struct", [_lib.Packed, _lib.KV4Query])
+def test_the_packed_bytes_are_the_struct(struct):
+    names = [n for n, _ in struct._fields_]
+    values = list(range(1, len(names) + 1))
+    packed = struct.FORMAT.pack(*values)
+    assert len(packed) == ctypes.sizeof(struct)
+    read = struct.from_buffer_copy(packed)
+    assert [getattr(read, n) for n in names] == values
 
 
 @pytest.mark.parametrize("bad", [
@@ -70,7 +81,7 @@ def test_cache_refuses(bad):
     assert L.after_kv4_evict(ctypes.byref(cache()), c, 8, 0, P, None) == E_INVALID
     n = ctypes.c_longlong()
     assert L.after_kv4_attend_workspace(c, 1, 4, 1, 0, ctypes.byref(n)) == E_INVALID
-    assert L.after_kv4_attend(c, P, P, 1, 4, 1, 256, 256, 64, 0.1, 0, 1.0, P, 1 << 40, None) == E_INVALID
+    assert L.after_kv4_attend(c, bytes(_lib.KV4Query(P, P, P, 1 << 40, 256, 256, 64, 1, 4, 1, 0.1, 0, 1.0)), None) == E_INVALID
 
 
 def test_cache_calls_refuse():
@@ -110,11 +121,14 @@ def test_attend_refuses():
         assert L.after_kv4_attend_workspace(c, 1, heads, tokens, 0, ctypes.byref(n)) == E_INVALID
     assert L.after_kv4_attend_workspace(c, 1, 4, 1, 0, None) == E_INVALID
     assert L.after_kv4_attend_workspace(c, 1, 4, 1, 1, ctypes.byref(n)) == 0 and n.value >= 2 * 2 * 2 * 4096 * 4
-    ok = (P, P, 1, 4, 1, 256, 256, 64, 0.1, 1, 1.0, P, n.value, None)
-    for i, v, code in ((0, None, E_INVALID), (1, P + 8, E_INVALID), (2, 3, E_INVALID), (5, 4, E_INVALID), (7, 1, E_INVALID), (8, float("nan"), E_INVALID),
-                       (10, float("inf"), E_INVALID), (11, None, E_CAPACITY), (12, n.value - 1, E_CAPACITY)):
-        assert L.after_kv4_attend(c, *[v if i == j else x for j, x in enumerate(ok)]) == code, (i, v)
+    ok = dict(q=P, out=P, workspace=P, workspace_bytes=n.value, q_row_stride=256, q_token_stride=256, q_head_stride=64, type=1, heads=4, tokens=1,
+              scale=0.1, accumulate=1, decay=1.0)
+    for k, v, code in (("q", None, E_INVALID), ("out", P + 8, E_INVALID), ("type", 3, E_INVALID), ("q_row_stride", 4, E_INVALID), ("q_head_stride", 1, E_INVALID),
+                       ("scale", float("nan"), E_INVALID), ("decay", float("inf"), E_INVALID), ("workspace", None, E_CAPACITY),
+                       ("workspace_bytes", n.value - 1, E_CAPACITY)):
+        assert L.after_kv4_attend(c, bytes(_lib.KV4Query(**{**ok, k: v})), None) == code, (k, v)
         assert "kv4_attend" in error()
+    assert L.after_kv4_attend(c, None, None) == E_INVALID and L.after_attend_packed(None, None) == E_INVALID
 
 
 def test_python_refuses_without_a_gpu():

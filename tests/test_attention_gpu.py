@@ -451,7 +451,7 @@ def test_strided_queries_and_refusals(hip_device):
             c.attend(bad)
     with torch.enable_grad(), pytest.raises(NotImplementedError):
         c.attend(torch.zeros(2, 1, 2, 64, device=hip_device, requires_grad=True))
-    for k in (dict(scale=math.nan), dict(decay=math.inf)):
+    for k in (dict(scale=math.nan), dict(decay=math.inf), dict(scale=-1e39), dict(decay=1e300)):
         with pytest.raises(ValueError):
             c.attend(wide[:, :, :4], **k)
     with pytest.raises(TypeError):
