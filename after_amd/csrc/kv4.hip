@@ -300,8 +300,10 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(after_kv4 c, void* ko, vo
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16: the 16 columns are (token, head of the group) pairs that share
 // the cached head, the rows cached tokens / channels.  Everything stays in registers: which token a row of S^T stands for and
 // which channel a step of its product contracts are chosen so that a lane's S values are the P operand that it needs next.
-// A cached value is exact in bf16; queries and probabilities travel as NP bf16 pieces (1 for bf16 queries, 2 for fp16: exact,
+// A cached value is exact in bf16; queries and probabilities travel as bf16 pieces (1 for bf16 queries, 2 for fp16: exact,
 // 3 for fp32: exact), so that what is rounded is never coarser than the output's own type.
+// What bounds it: memory.  64 rows of 1 .. 8192 slots, 8 heads of 128 (296 MB): 57.6 us and 5.3 for the join, 5.1 TB/s; two rows of
+// 131071 with 8 fp16 queries a head, whose scores are written for the weights (285 + 67 MB): 77 us, 4.6 TB/s, as a copy.
 struct AttendArgs {
     after_kv4 c;
     const void* q;
@@ -359,18 +361,31 @@ struct Tile {
     unsigned char ks[2];    // the scale bytes of the keys' group
 };
 
+// 16 columns, `cols` to a piece: the sum over the pieces, in all of them
+template <int COLS>
+__device__ __forceinline__ float fold(float x) {
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xF, 0xF, true));
+    if constexpr (COLS == 4) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x124, 0xF, 0xF, true));
+    return x;
+}
+
 // JOINT: a workgroup's four waves take the tiles of one row and head in turn and add up in LDS (short rows: one launch);
 // otherwise every wave is a worker of its own.
-template <int TYPE, int D, int NM, bool COUNT, bool JOINT>
+// COLS < 16: no more queries than that, whose pieces (two of fp16, up to four of fp32) take the other columns, which a product
+// computes anyway: one product instead of one for each piece, and the columns are added up, of the scores for each tile, of the
+// output at the end.
+template <int TYPE, int D, int NM, bool COUNT, bool JOINT, int COLS>
 __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
     using T = typename Elem<TYPE>::T;
-    constexpr int NP = TYPE == AFTER_T_BF16 ? 1 : TYPE == AFTER_T_F16 ? 2 : 3;
+    constexpr int PIECES = COLS < 16 ? 16 / COLS : TYPE == AFTER_T_BF16 ? 1 : TYPE == AFTER_T_F16 ? 2 : 3;
+    constexpr int NP = COLS < 16 ? 1 : PIECES;  // operands of a lane
     constexpr int G = D / 32, S = D / 32, KW = D / 32, VW = D / 16;  // groups, steps of a score, dwords of keys / values per lane
     constexpr int RING = kRing, BYTES = kTileBytes<D>, LOADS = D / 32 + 1;
     constexpr int STRIDE = JOINT ? 128 : 32;  // tokens from one tile of a wave to its next
     extern __shared__ __align__(16) char lds[];  // [4][RING][BYTES]; JOINT: then [4][16][D + 4] floats
     const after_kv4& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, kq = lane >> 4;
+    const int col = l15 % COLS, piece_of = l15 / COLS;  // this lane's query of each 16, and which piece of it
     // the first row and head of this worker's share, and where in it the share begins
     const int worker = blockIdx.x * 4 + wave;
     int r, h, step = 0;
@@ -424,7 +439,7 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
     int vis[NM];
 #pragma unroll
     for (int nm = 0; nm < NM; ++nm) {
-        const int m = nm * 16 + l15, t = m / a.group, g = m - t * a.group;
+        const int m = nm * 16 + col, t = m / a.group, g = m - t * a.group;
         const bool in = m < a.m_rows;
         vis[nm] = in ? max(len - a.tokens + t + 1, 0) : 0;
 #pragma unroll
@@ -433,7 +448,15 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
             if (in) load_n<8, T>((const T*)a.q + r * a.qrs + t * a.qts + (long long)(h * a.group + g) * a.qhs + D / 4 * kq + 8 * s, y);
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] *= a.q_sign;
-            pieces8<NP>(y, qf[nm][s]);
+            if constexpr (COLS < 16) {
+                bf16x8 z[PIECES];
+                pieces8<PIECES>(y, z);
+                qf[nm][s][0] = z[0];
+#pragma unroll
+                for (int q = 1; q < PIECES; ++q)
+                    if (piece_of == q) qf[nm][s][0] = z[q];
+            } else
+                pieces8<NP>(y, qf[nm][s]);
         }
     }
     const int all_see = len - a.tokens + 1;  // slots below this are seen by every query
@@ -512,6 +535,12 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
                     for (int p = NP - 1; p >= 0; --p) sc[nm][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[nm][s][p], sc[nm][f], 0, 0, 0);
             }
         }
+        if constexpr (COLS < 16) {
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[0][f][i] = fold<COLS>(sc[0][f][i]);
+        }
         __builtin_amdgcn_sched_barrier(0);
         const bool masked = t0 + 32 > all_see;
         if (masked) {
@@ -528,8 +557,8 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = fmaxf(top, sc[nm][j >> 2][j & 3]);
             if constexpr (COUNT) {
-                const int m = nm * 16 + l15;
-                if (m < a.m_rows) {
+                const int m = nm * 16 + col;
+                if (m < a.m_rows && piece_of == 0) {
                     float* to = a.scores + ((size_t)rh * a.m_rows + m) * c.capacity + t0 + 8 * kq;
                     *reinterpret_cast<f32x4*>(to) = sc[nm][0] * a.scale2;
                     *reinterpret_cast<f32x4*>(to + 4) = sc[nm][1] * a.scale2;
@@ -566,9 +595,15 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
             for (int i = 0; i < 4; ++i) {
                 float x0 = p[nm][2 * i], x1 = p[nm][2 * i + 1];
 #pragma unroll
+                for (int q = 0; COLS < 16 && q < PIECES - 1; ++q) {  // what this lane's piece leaves to the ones before it
+                    const unsigned taken = piece_of > q ? 0xFFFF0000u : 0u;
+                    x0 -= __uint_as_float(__float_as_uint(x0) & taken);
+                    x1 -= __uint_as_float(__float_as_uint(x1) & taken);
+                }
+#pragma unroll
                 for (int q = 0; q < NP; ++q) {
                     unsigned u;
-                    if constexpr (NP == 1)
+                    if constexpr (PIECES == 1)
                         u = __builtin_bit_cast(unsigned, bf16x2{(__bf16)x0, (__bf16)x1});
                     else
                         u = __builtin_amdgcn_perm(__float_as_uint(x1), __float_as_uint(x0), 0x07060302u);
@@ -586,15 +621,16 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
 #pragma unroll
                 for (int nm = 0; nm < NM; ++nm) {
                     float y[8];
-                    bf16x8 z[NP];
+                    bf16x8 z[PIECES];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const int byte = j * G + g;
                         y[j] = t0 + 8 * kq + j >= vis[nm] ? 0.f : p[nm][j] * byte_scale(w.vs[byte >> 2] >> 8 * (byte & 3) & 255u);
                     }
-                    pieces8<NP>(y, z);
+                    pieces8<PIECES>(y, z);
 #pragma unroll
-                    for (int q = 0; q < NP; ++q) pf[nm][q] = __builtin_bit_cast(u32x4, z[q]);
+                    for (int q = 0; q < PIECES; ++q)
+                        if (NP > 1 || piece_of == q) pf[nm][NP > 1 ? q : 0] = __builtin_bit_cast(u32x4, z[q]);
                 }
             } else {
 #pragma unroll
@@ -628,6 +664,12 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
     for (int nm = 0; nm < NM; ++nm) {
         l[nm] += __shfl_xor(l[nm], 16);
         l[nm] += __shfl_xor(l[nm], 32);
+        if constexpr (COLS < 16) {
+#pragma unroll
+            for (int i = 0; i < 2 * G; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[nm][i][e] = fold<COLS>(o[nm][i][e]);
+        }
     }
     if constexpr (JOINT) {  // the four waves' shares -> one
         __shared__ float sm[4][NM * 16], sl[4][NM * 16];
@@ -676,8 +718,8 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
         }
 #pragma unroll
         for (int nm = 0; nm < NM; ++nm) {
-            const int m = nm * 16 + l15;
-            if (m < a.m_rows) {
+            const int m = nm * 16 + col;
+            if (m < a.m_rows && piece_of == 0) {
                 if ((!whole || COUNT) && kq == 0) a.part_ml[piece * a.m_rows + m] = f32x2{mx[nm], l[nm]};
                 const float inv = l[nm] == 0.f ? 0.f : 1.f / l[nm];
                 const int t = m / a.group, g0 = m - t * a.group;
@@ -1353,6 +1395,8 @@ struct Plan {
     long long pieces, o_bytes, ml_bytes, s_bytes, e_bytes, f_bytes;
     long long total() const { return o_bytes + ml_bytes + s_bytes + e_bytes + f_bytes; }
 };
+// How many columns of a product the queries take: with the others for their pieces, where they fit
+constexpr int attend_cols(int type, int m_rows) { return type == AFTER_T_F16 && m_rows <= 8 ? 8 : type == AFTER_T_F32 && m_rows <= 4 ? 4 : 16; }
 Plan attend_plan(const after_kv4& c, int type, int heads, int tokens, bool count) {
     Plan p;
     p.m_rows = tokens * (heads / c.kv_heads);
@@ -1365,10 +1409,12 @@ Plan attend_plan(const after_kv4& c, int type, int heads, int tokens, bool count
         const long long wanted = cdivll(512, n_rh * p.mgroups), tiles = cdivll(c.capacity, 4 * kWideTile);
         p.splits = (int)(wanted < tiles ? wanted : tiles);
     } else if (c.capacity > 512) {
-        // As many workers as the chip holds at once: three workgroups on each of 256 CUs with bf16 queries, two with the others
-        // (more registers).  64 rows of 1 .. 8192, bf16: 60 us, and 64 with two; two rows of 131071, fp16: 59 us, and 69 with
-        // three.  Rows of at most 512 slots take a workgroup each and one launch: 6.4 us against 9.
-        const int full = type == AFTER_T_BF16 ? 768 : 512;
+        // Workers for two workgroups on each of 256 CUs, for three where the queries' registers leave room and there are many rows
+        // (with few, more pieces are a longer join).  D = 128, with the join: 64 rows of 1 .. 8192 x 8 heads, bf16 75.6 us against
+        // 78.3 with two, fp16 76.3 / 82.0, fp32 81.4 / 87.2 (without pieces in columns 81.7 and 88.2); 8 rows of 1 .. 32767, bf16
+        // 45.2 / 45.7; two rows of 131071, bf16 71.6 / 68.4, fp16 72.1 / 69.0; one of 32768 26.9 / 23.6.
+        // Rows of at most 512 slots take a workgroup each and one launch: 6.2 us against 9.
+        const int full = n_rh >= 64 && (attend_cols(type, p.m_rows) < 16 || type == AFTER_T_BF16) ? 768 : 512;
         p.wgs = (int)(most < full ? most : full);
     }
     p.pieces = p.splits ? n_rh * p.splits : 4ll * p.wgs + n_rh;
@@ -1380,13 +1426,13 @@ Plan attend_plan(const after_kv4& c, int type, int heads, int tokens, bool count
     return p;
 }
 
-template <int TYPE, int D, int NM, bool COUNT>
+template <int TYPE, int D, int NM, bool COUNT, int COLS>
 void launch_attend(const AttendArgs& a, const Plan& p, hipStream_t s) {
     constexpr size_t ring = 4 * kRing * kTileBytes<D>, out = 4 * 16 * (D + 4) * 4;  // (at most 53 KB: three workgroups a CU)
     if (p.wgs)
-        hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, NM, COUNT, false>), dim3(p.wgs), dim3(256), ring, s, a);
+        hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, NM, COUNT, false, COLS>), dim3(p.wgs), dim3(256), ring, s, a);
     else
-        hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, NM, COUNT, true>), dim3(a.c.rows * a.c.kv_heads), dim3(256), ring > out ? ring : out, s, a);
+        hipLaunchKernelGGL((kv4_attend_kernel<TYPE, D, NM, COUNT, true, COLS>), dim3(a.c.rows * a.c.kv_heads), dim3(256), ring > out ? ring : out, s, a);
 }
 
 template <int TYPE, int D>
@@ -1408,16 +1454,22 @@ int run_attend(const AttendArgs& a, const Plan& p, bool count, float decay, hipS
         AFTER_HIP_CHECK(hipGetLastError());
         return AFTER_OK;
     }
-    if (p.nm == 1) {
+    constexpr int few = attend_cols(TYPE, 1);
+    if (few < 16 && attend_cols(TYPE, p.m_rows) == few) {
         if (count)
-            launch_attend<TYPE, D, 1, true>(a, p, s);
+            launch_attend<TYPE, D, 1, true, few>(a, p, s);
         else
-            launch_attend<TYPE, D, 1, false>(a, p, s);
+            launch_attend<TYPE, D, 1, false, few>(a, p, s);
+    } else if (p.nm == 1) {
+        if (count)
+            launch_attend<TYPE, D, 1, true, 16>(a, p, s);
+        else
+            launch_attend<TYPE, D, 1, false, 16>(a, p, s);
     } else {
         if (count)
-            launch_attend<TYPE, D, 2, true>(a, p, s);
+            launch_attend<TYPE, D, 2, true, 16>(a, p, s);
         else
-            launch_attend<TYPE, D, 2, false>(a, p, s);
+            launch_attend<TYPE, D, 2, false, 16>(a, p, s);
     }
     if (p.wgs)
         hipLaunchKernelGGL((kv4_join_kernel<TYPE, D>), dim3(n_rh * a.m_rows), dim3(256), 0, s, a);
