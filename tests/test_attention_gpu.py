@@ -341,6 +341,19 @@ def test_append_in_pieces_is_append_at_once(hip_device):
     assert (k2[0, :, 7:] == 0).all() and (v2[1, :, 1:] == 0).all()
 
 
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_append_takes_views(hip_device, tokens):
+    fused = torch.randn(5, tokens, 12, 64, generator=gen(64)).to(hip_device, torch.float16)
+    for k, v in ((fused[:, :, 4:6], fused[:, :, 6:8]), (fused[:1, :, 4:6].expand(5, -1, -1, -1), fused[:, :, 6:7].expand(-1, -1, 2, -1)),
+                 (fused.transpose(0, 1).contiguous().transpose(0, 1)[:, :, 4:6], fused[:, :, 6:8].contiguous())):
+        a, b = (KVCache4(5, 2, 64, 64, hip_device) for _ in range(2))
+        for _ in range(3):
+            a.append(k, v)
+            b.append(k.contiguous(), v.contiguous())
+        for n, x in a.buffers().items():
+            assert torch.equal(x, b.buffers()[n]), n
+
+
 def test_append_without_room(hip_device):
     c = KVCache4(3, 1, 64, 32, hip_device)
     k = torch.randn(3, 30, 1, 64, generator=gen(9)).to(hip_device)
@@ -634,6 +647,28 @@ def test_a_captured_step_replays(hip_device):
             for n, x in c.buffers().items():
                 assert torch.equal(x, e.buffers()[n]), n
     assert sets[0][0].lengths.tolist() == [604, 7, 1004]
+
+
+def test_captured_shares_of_the_keys(hip_device):
+    """Two graphs whose calls share their keys out over the chip, replayed in turn with eager calls between."""
+    q, k, v = (torch.zeros(n, h, 128, device=hip_device, dtype=torch.bfloat16) for n, h in ((2, 8), (9000, 2), (9000, 2)))
+    s, ks = starts([1, 1], hip_device), starts([6000, 3000], hip_device)
+    outs, graphs = [torch.zeros_like(q) for _ in range(2)], [torch.cuda.CUDAGraph() for _ in range(2)]
+    attend_packed(q, k, v, s, ks)
+    torch.cuda.synchronize()
+    for out, graph in zip(outs, graphs):
+        with torch.cuda.graph(graph):
+            attend_packed(q, k, v, s, ks, out=out)
+            out.add_(attend_packed(q, k, v, s, ks, causal=False))
+    for turn in range(4):
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=gen(100 + turn)))
+        for graph in graphs:
+            graph.replay()
+        want = attend_packed(q, k, v, s, ks)
+        want += attend_packed(q, k, v, s, ks, causal=False)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
 
 
 def test_another_stream(hip_device):
