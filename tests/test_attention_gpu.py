@@ -504,7 +504,9 @@ def test_strided_queries_and_refusals(hip_device):
     (128, [1500, 0, 700], 512, 100, 640),
     (64, [4097], 1, 0, 32),
     (128, [900], 300, 300, 320),
-    (64, [200], 199, 1, 224)])
+    (64, [200], 199, 1, 224),
+    (64, [70000, 33000], 32900, 77, 33024),
+    (64, [4096, 4100, 8193], 4095, 0, 4096)])
 @pytest.mark.parametrize("weights", ["spread", "ties", "odd"])
 def test_evict(hip_device, dim, lens, keep, recent, capacity, weights):
     H = 3
