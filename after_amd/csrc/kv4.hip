@@ -116,6 +116,17 @@ __device__ __forceinline__ unsigned quad_max(unsigned x) {
     return max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, true));  // lanes 2 3 0 1
 }
 
+// sums of the lanes up to this one (inside the vector unit: shuffles through LDS take several times as long)
+__device__ __forceinline__ int lane_sums(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // 1, 2, 4, 8 lanes on, inside each 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // lane 15 of the 16 before to the second and fourth 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // lane 31 to the upper half
+    return x;
+}
+
 struct AppendArgs {
     after_kv4 c;
     NewTokens nt;
@@ -754,6 +765,9 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
 // them per workgroup, 32 to a wave, over the same tiles of 64 tokens.  The tiles are widened to bf16 once for the four waves and
 // kept in LDS in the order in which the matrix instructions take them (a lane's operand is 16 bytes at its own number: no
 // conflicts); while one tile is multiplied the next one's codes are on their way in registers.
+// What bounds it: the vector unit (an exponential and some five more per score, and the widening) and the products in turn.  32
+// tokens of 4 rows of 9001 .. 16384, bf16, 32 / 8 heads of 128: 55 us, 0.5 PFLOP/s, the join 10 (64 KB of sums a piece), the
+// weights, for which the scores are formed again, 38; 8 rows of 1 .. 16384: 151 us in all, 177 with equal splits of each row.
 constexpr int kWideRows = 128, kWideTile = 64;
 
 template <int D>
@@ -883,8 +897,40 @@ __device__ __forceinline__ void scores32(const char* keys, const bf16x8 (&qf)[2]
     }
 }
 
-// slots per split of a row: whole tiles
-__device__ __forceinline__ int wide_chunk(int len, int splits) { return ((len + splits - 1) / splits + kWideTile - 1) / kWideTile * kWideTile; }
+// The tiles of all rows are shared out over the workgroups of a head in pieces of one length, the least with which rows x splits
+// workgroups do (each row's last piece may be shorter): with rows of different lengths all end at about the same time.
+struct WidePiece {
+    int row, at, of;  // the at-th of the row's `of` pieces
+    int first;        // its number among the head's
+    int slots;        // of a piece
+};
+__device__ __forceinline__ int wide_tiles(const after_kv4& c, int r) { return (row_length(c, r) + kWideTile - 1) / kWideTile; }
+__device__ __forceinline__ bool find_piece(const after_kv4& c, int splits, int unit, WidePiece& p) {
+    const int lane = threadIdx.x & 63, units = c.rows * splits;
+    int share = 1 << 24;  // (one piece to a row)
+    if (splits > 1) {
+        long long all = 0;
+        for (int i = lane; i < c.rows; i += 64) all += wide_tiles(c, i);
+        // (a row's last piece: at most one more for each)
+        share = (int)max(1ll, (wave_sum(all) + units - c.rows - 1) / (units - c.rows));
+    }
+    int before = 0;
+    for (int r0 = 0; r0 < c.rows; r0 += 64) {
+        const int n = r0 + lane < c.rows ? (wide_tiles(c, r0 + lane) + share - 1) / share : 0, sum = lane_sums(n);
+        const unsigned long long past = __ballot(before + sum > unit);
+        if (past) {
+            const int j = __ffsll(past) - 1;
+            p.row = __builtin_amdgcn_readfirstlane(r0 + j);
+            p.of = __builtin_amdgcn_readlane(n, j);
+            p.first = __builtin_amdgcn_readfirstlane(before) + __builtin_amdgcn_readlane(sum, j) - p.of;
+            p.at = unit - p.first;
+            p.slots = __builtin_amdgcn_readfirstlane(share) * kWideTile;
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(sum, 63);
+    }
+    return false;
+}
 
 template <int TYPE, int D>
 __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_kernel(AttendArgs a, int splits, int mgroups) {
@@ -898,13 +944,14 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_ker
     // (neighbours are dispatched to different XCDs: the workgroups that read one piece of the cache stand eight apart, on one L2)
     const int x = blockIdx.x, mg = (x >> 3) % mgroups, unit = (x >> 3) / mgroups * 8 + (x & 7), n_rh = c.rows * c.kv_heads;
     if (unit >= n_rh * splits) return;
-    const int rh = unit % n_rh, split = unit / n_rh, r = rh / c.kv_heads, h = rh % c.kv_heads;
-    const int len = row_length(c, r), chunk = wide_chunk(len, splits), used = len ? (len + chunk - 1) / chunk : 0;
-    if (split >= used) return;
-    if (mg == 0 && split == 0 && threadIdx.x == 0) a.ends[rh] = int2{rh * splits, rh * splits + used - 1};
+    const int h = unit % c.kv_heads, units = c.rows * splits;
+    WidePiece w;
+    if (!find_piece(c, splits, unit / c.kv_heads, w)) return;
+    const int r = w.row, rh = r * c.kv_heads + h, len = row_length(c, r), used = w.of, first = h * units + w.first;
+    if (mg == 0 && w.at == 0 && threadIdx.x == 0) a.ends[rh] = int2{first, first + used - 1};
     const int m0 = mg * kWideRows + wave * 32;
-    const int begin = split * chunk, last_m = min((mg + 1) * kWideRows, a.m_rows) - 1;
-    const int end = min(begin + chunk, len - a.tokens + last_m / a.group + 1);  // (what the last query here sees)
+    const int begin = w.at * w.slots, last_m = min((mg + 1) * kWideRows, a.m_rows) - 1;
+    const int end = min(min(begin + w.slots, len), len - a.tokens + last_m / a.group + 1);  // (what the last query here sees)
     const int all_see = len - a.tokens + m0 / a.group + 1;                      // every query of the wave sees the slots below
 
     bf16x8 qf[2][G][NP];
@@ -999,7 +1046,7 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_ker
         }
     }
 
-    const size_t piece = (size_t)rh * splits + split;
+    const size_t piece = (size_t)first + w.at;
 #pragma unroll
     for (int nm = 0; nm < 2; ++nm) {
         l[nm] += __shfl_xor(l[nm], 16);
@@ -1195,17 +1242,6 @@ __device__ __forceinline__ unsigned order_key(float x) {
     const unsigned u = __float_as_uint(x);
     if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 0u;
     return u == 0x80000000u ? 0x80000000u : (u >> 31) ? ~u : u | 0x80000000u;
-}
-
-// sums of the lanes up to this one (inside the vector unit: shuffles through LDS take several times as long)
-__device__ __forceinline__ int lane_sums(int x) {
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // 1, 2, 4, 8 lanes on, inside each 16
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // lane 15 of the 16 before to the second and fourth 16
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // lane 31 to the upper half
-    return x;
 }
 
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelLoads = 8, kSelSpan = 4 * kSelLoads * kSelThreads;
@@ -1473,7 +1509,7 @@ int run_attend(const AttendArgs& a, const Plan& p, bool count, float decay, hipS
         // (empty rows have no workgroup: their zeros come from the join)
         hipLaunchKernelGGL((kv4_join_kernel<TYPE, D>), dim3(n_rh * a.m_rows), dim3(256), 0, s, a);
         if (count) {
-            const long long even = cdivll((long long)n_rh * a.c.capacity, 512 * kWideTile) * kWideTile;  // two workgroups a CU
+            const long long even = cdivll((long long)n_rh * a.c.capacity, 768 * kWideTile) * kWideTile;  // three workgroups a CU
             const int slots = (int)(even < 256 ? 256 : even < kWideSlots ? even : kWideSlots), blocks = cdiv(a.c.capacity, slots);
             hipLaunchKernelGGL((kv4_wide_weights_kernel<TYPE, D>), dim3((unsigned)(n_rh * blocks)), dim3(256), 2 * Widen<D>::KEYS, s, a, blocks, slots, decay);
         }
