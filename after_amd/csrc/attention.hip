@@ -8,7 +8,7 @@
 // are its operand as they lie, and only V is read accordingly (two transposing LDS reads per 16 tokens).
 //
 // Rows.  The `group` heads that share a key head are rows of one tile, row = token * group + head: short sequences fill tiles,
-// and a key tile is read once for all of them.  A workgroup holds 128 rows, 32 to a wave; its tile number alone says which
+// and a key tile is read once for all of them.  A workgroup holds 128 rows, 32 to a wave (or 32 in all, "few rows" below); its tile number alone says which
 // sequence it serves (sequence b owns the numbers from floor(start_b * group / 128) + b on), so the grid needs no lengths.
 //
 // What bounds it.  Long prompts: the matrix pipes, with the softmax's exponentials between two products; 16384 causal tokens, bf16,
@@ -418,6 +418,8 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
 // workgroup, whose four waves share out their keys, 32 at a time.  Each wave has one buffer for keys and one for values in LDS:
 // the next keys are asked for when the scores are formed, the next values when they are added up, and no wave waits for another
 // until the four are joined.  With `splits` > 1 that many workgroups share the keys, and attend_join_kernel joins them.
+// What bounds it: short sequences, the chain of loads before the first product (3 x 256 fp32 tokens of 8 heads of 64, window 8: 8.6
+// us); one query over many keys, memory (bf16, 8 heads of 128: 32768 keys 28.4 us, 131072 102 us = 5.2 TB/s).
 constexpr int kFewRows = 32;
 // steps of 32 keys per wave, and the workgroups that have any
 __device__ __forceinline__ int few_share(const PackedArgs& a, int steps) { return max(1, (steps + 4 * a.splits - 1) / (4 * a.splits)); }
@@ -728,8 +730,10 @@ PackedPlan packed_plan(int type, long long q_rows, long long k_rows, int n_seqs,
     // 8 heads of 64, window 8 (80 workgroups) 8.9 us against 20.9, 6000 of 8 / 2 heads of 128 (378) 706 / 778, 8192 (516) 1285 /
     // 1129.  16 bits, long sequences: 2048 tokens of 8 heads of 64 (144) 17.5 / 34.3, of 8 / 2 heads of 128 6000 (378) 132 / 132 and
     // 7000 (440) 171 / 159; short ones, where the beginning of a workgroup counts: 8 x 200 of 8 heads of 128 (168) 10.0 / 12.0,
-    // 12 x 200 (248) 15.7 / 12.5.
-    p.few = wide <= (type == AFTER_T_F32 ? 512 : keys >= 1024 ? 384 : 192);
+    // 12 x 200 (248) 15.7 / 12.5.  And wherever a sequence's rows fill no more than one of 32: bf16, one token of 256 sequences of
+    // 1 .. 2048, 32 / 8 heads of 128, 204 / 222, of 400 of 1 .. 300, 8 heads of 64, 25.6 / 39.5, 16 tokens of 128 of 1 .. 1000,
+    // 8 heads of 128, 48.6 / 61.9; fp32, 128 of 1 .. 2048, 242 / 760.
+    p.few = q_rows * group <= 32ll * n_seqs || wide <= (type == AFTER_T_F32 ? 512 : keys >= 1024 ? 384 : 192);
     p.tiles = (int)(q_rows * group / (p.few ? kFewRows : BM)) + n_seqs + 1;
     p.splits = 1;
     if (p.few) {

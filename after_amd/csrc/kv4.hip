@@ -324,7 +324,8 @@ struct AttendArgs {
     int workers;      // waves that share the work (below); 0: a workgroup for each row and head
     float scale2;     // |scale| log2(e), > 0 (a masked score, -inf, stays -inf)
     float q_sign;     // the scale's sign, on the queries
-    float* part_o;    // [pieces][m_rows][D]: a piece is one worker's part of a row and head, number worker + row * H + head
+    float* part_o;    // [pieces][m_rows][D]: a piece is one worker's part of a row and head, number worker + row * H + head (many
+                      // queries: one workgroup's, number head * rows * splits + its place among the head's)
     f32x2* part_ml;   // [pieces][m_rows]: largest score, sum of exponentials to it
     f32x2* final_ml;  // [rows * H][m_rows]: the same over all pieces, if weights are wanted
     int2* ends;       // [rows * H]: the first and the last piece of a row and head, written by the workers that hold its ends
