@@ -8,14 +8,16 @@
 // are its operand as they lie, and only V is read accordingly (two transposing LDS reads per 16 tokens).
 //
 // Rows.  The `group` heads that share a key head are rows of one tile, row = token * group + head: short sequences fill tiles,
-// and a key tile is read once for all of them.  A workgroup holds 128 rows, 32 to a wave (or 32 in all, "few rows" below); its tile number alone says which
-// sequence it serves (sequence b owns the numbers from floor(start_b * group / 128) + b on), so the grid needs no lengths.
+// and a key tile is read once for all of them.  A workgroup holds 128 rows, 32 to a wave (or 32 in all: "few rows" below); its
+// tile number alone says which sequence it serves (sequence b owns the numbers from floor(start_b * group / 128) + b on), so the
+// grid needs no lengths.
 //
 // What bounds it.  Long prompts: the matrix pipes, with the softmax's exponentials between two products; 16384 causal tokens, bf16,
 // 32 / 8 heads of 128: 2120 us, 1037 TFLOP/s, where a large product of the library reaches 1155 (fp16 heads of 128 in a batch of
 // 1 .. 2047 tokens: 306 us, 710; heads of 64, 8192 tokens: 330 us, 830; fp32 heads of 128, 4096 tokens: 585 us, 118 of 153).
 // Tiles of 64 keys, two of them in LDS and two workgroups on a CU: one computes while the other waits.  Measured and left out:
-// V read by instructions that wait by themselves (2240 us), skipping the unseen half of a masked tile (2330), scheduling hints (2120).
+// V read by instructions that wait by themselves, and scheduling hints (the same time), skipping the unseen half of a masked
+// tile (2330 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
