@@ -13,8 +13,8 @@
 // grid needs no lengths.
 //
 // What bounds it.  Long prompts: the matrix pipes, with the softmax's exponentials between two products; 16384 causal tokens, bf16,
-// 32 / 8 heads of 128: 2120 us, 1037 TFLOP/s, where a large product of the library reaches 1155 (fp16 heads of 128 in a batch of
-// 1 .. 2047 tokens: 306 us, 710; heads of 64, 8192 tokens: 330 us, 830; fp32 heads of 128, 4096 tokens: 585 us, 118 of 153).
+// 32 / 8 heads of 128: 2090 us, 1053 TFLOP/s, where a large product of the library reaches 1155 (fp16 heads of 128 in a batch of
+// 1 .. 2047 tokens: 300 us, 725; heads of 64, 8192 tokens: 317 us, 868; fp32 heads of 128, 4096 tokens: 585 us, 118 of 153).
 // Tiles of 64 keys, two of them in LDS and two workgroups on a CU: one computes while the other waits.  Measured and left out:
 // V read by instructions that wait by themselves, and scheduling hints (the same time), skipping the unseen half of a masked
 // tile (2330 us).
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
     extern __shared__ __align__(16) char lds[];
     __shared__ unsigned long long odd_rows[3];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, half = lane >> 5;
     // neighbouring workgroups are dispatched to different XCDs: a key head's workgroups stay on one L2 where there are eight.
     // Tiles from the last to the first: with a causal mask the longest first.
     const int back = a.by_kv_heads(blockIdx.x), h = blockIdx.x - back * a.kv_heads, tile = a.tiles - 1 - back;
@@ -188,40 +188,20 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
     if (!find_tile<BM>(a, tile, place)) return;
     const int q0 = place.q0, nq = place.nq, k0 = place.k0, nk = place.nk, row0 = place.row0, rows = place.rows;
 
-    // this lane's query, and the keys that it and its workgroup see
+    // this lane's query, and the keys that its workgroup sees: asked for before the rest is worked out
     const int row = row0 + wave * 32 + l31, t = a.by_group(min(row, rows - 1)), g = min(row, rows - 1) - t * a.group;
-    int first, last, t_first, t_last, dummy;
-    seen(a, t + nk - nq, nk, first, last);
-    seen(a, a.by_group(row0) + nk - nq, nk, t_first, dummy);
-    seen(a, a.by_group(min(row0 + BM, rows) - 1) + nk - nq, nk, dummy, t_last);
-    // the keys that some query of the wave sees
-    int w_first = 0, w_last = 0;
-    const int w_row = __builtin_amdgcn_readfirstlane(row0 + wave * 32);
-    if (w_row < rows) {
-        seen(a, a.by_group(w_row) + nk - nq, nk, w_first, dummy);
-        seen(a, a.by_group(min(w_row + 32, rows) - 1) + nk - nq, nk, dummy, w_last);
-    }
-    // every query of the workgroup sees [all_first, all_last)
-    int all_first, all_last;
-    seen(a, a.by_group(row0) + nk - nq, nk, dummy, all_last);
-    seen(a, a.by_group(min(row0 + BM, rows) - 1) + nk - nq, nk, all_first, dummy);
-
     const T* qp = (const T*)a.q + (long long)(q0 + t) * a.qts + (long long)(h * a.group + g) * a.qhs;
-    const T* kp = (const T*)a.k + (long long)k0 * a.kts + (long long)h * a.khs;
-    const T* vp = (const T*)a.v + (long long)k0 * a.vts + (long long)h * a.vhs;
-
     // Q: 16-bit types: step s contracts channels 16 s + 8 half + 0 .. 7; fp32: step s, e channels 8 s + 4 half + e
     constexpr int QN = sizeof(T) == 4 ? D / 8 : D / 16;
     u32x4 qf[QN];
 #pragma unroll
     for (int s = 0; s < QN; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qp + (2 * s + half) * (16 / (int)sizeof(T))) ^ a.q_sign;
 
-    f32x16 o[DT];
-#pragma unroll
-    for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
-    float mx = -INFINITY, l = 0.f;
+    int t_first, t_last, dummy;
+    seen(a, a.by_group(row0) + nk - nq, nk, t_first, dummy);
+    seen(a, a.by_group(min(row0 + BM, rows) - 1) + nk - nq, nk, dummy, t_last);
+    const T* kp = (const T*)a.k + (long long)k0 * a.kts + (long long)h * a.khs;
+    const T* vp = (const T*)a.v + (long long)k0 * a.vts + (long long)h * a.vhs;
 
     // K and V tiles go from memory to LDS without passing registers, two stages: while a tile is computed the next is on its way.
     // A lane's place in LDS is its number, so the pieces are permuted by the address it reads from.  Rows behind the sequence
@@ -253,6 +233,28 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
         }
     };
     if (n_first < n_last) fetch(n_first, 0);
+    // the keys that the query sees
+    int first, last;
+    seen(a, t + nk - nq, nk, first, last);
+    // the keys that some query of the wave sees
+    int w_first = 0, w_last = 0;
+    const int w_row = __builtin_amdgcn_readfirstlane(row0 + wave * 32);
+    if (w_row < rows) {
+        seen(a, a.by_group(w_row) + nk - nq, nk, w_first, dummy);
+        seen(a, a.by_group(min(w_row + 32, rows) - 1) + nk - nq, nk, dummy, w_last);
+    }
+    // every query of the workgroup sees [all_first, all_last)
+    int all_first, all_last;
+    seen(a, a.by_group(row0) + nk - nq, nk, dummy, all_last);
+    seen(a, a.by_group(min(row0 + BM, rows) - 1) + nk - nq, nk, all_first, dummy);
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+    float mx = -INFINITY, l = 0.f;
+
     int checked = 0;
     if (tid < 3) odd_rows[tid] = 0;
     for (int n = n_first; n < n_last; ++n) {
