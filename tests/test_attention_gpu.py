@@ -120,6 +120,17 @@ def test_few_queries_over_many_keys(hip_device, kind, dim, qs, ks, heads, kv, ca
     assert torch.equal(kept[:sum(qs)], out[:sum(qs)]) and (kept[sum(qs):] == 7).all()
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_a_step_of_many_sequences(hip_device, kind):
+    """A few new tokens each, none for some, behind caches of every length."""
+    g, t, n = gen(95), TYPES[kind], 700
+    qs = torch.randint(0, 4, (n, ), generator=g).tolist()
+    ks = [max(0, a + int(x)) for a, x in zip(qs, torch.randint(-2, 150, (n, ), generator=g))]
+    q, k, v = (torch.randn(x, h, 64, generator=g).to(hip_device, t) for x, h in ((sum(qs), 4), (sum(ks), 2), (sum(ks), 2)))
+    out = attend_packed(q, k, v, starts(qs, hip_device), starts(ks, hip_device))
+    check_packed(out, q, k, v, qs, ks, 0.125)
+
+
 def test_a_share_of_the_keys_with_nan(hip_device):
     """In a piece of the keys: NaN and infinities reach the queries that see them, and no other."""
     q, k, v = (torch.randn(n, 1, 64, generator=gen(n)).to(hip_device, torch.bfloat16) for n in (2, 8002, 8003))
