@@ -819,7 +819,8 @@ struct Widen {
         for (int i = 0; i < 4; ++i) *reinterpret_cast<bf16x8*>(lds + k_to + i * 256) = widen8(w.k[i], sc);
     }
     // A NaN group is left out, its token marked in bad[g]: the queries that see it get their NaN apart from the product, in which
-    // it would reach all of them.
+    // it would reach all of them.  So is any scale beyond the format's, which slots behind the row's length may hold: nobody sees
+    // them, but their codes times 2^126 would be infinities.
     __device__ __forceinline__ void store_values(const Raw<D>& w, char* lds, unsigned long long* bad) const {
         const int g0 = D == 128 ? 2 * (quad & 1) : 0;
 #pragma unroll
@@ -830,15 +831,15 @@ struct Widen {
             for (int j = 0; j < 8; ++j) {
                 const int byte = j * G + g0 + gg;
                 const unsigned b = w.vs[G == 4 ? j : j >> 1] >> 8 * (byte & 3) & 255u;
-                any |= b == kBadByte;
+                any |= b > kMaxByte;
                 sc[j] = byte_scale(b);
             }
             if (any) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (sc[j] == INFINITY) {
+                    if (sc[j] > byte_scale(kMaxByte)) {
                         atomicOr(&bad[g0 + gg], 1ull << (8 * block + j));
-                        sc[j] = 1.f;  // (its codes are zeros)
+                        sc[j] = 1.f;  // (any that keeps its codes finite)
                     }
             }
 #pragma unroll

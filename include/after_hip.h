@@ -614,7 +614,8 @@ int after_attend_packed(const after_packed* call, void* stream);
  *          low nibble for even s
  *   key_scales, value_scales [rows][kv_heads][capacity][D / 32]
  *   weights [rows][kv_heads][capacity]: the attention each slot has received (after_kv4_attend)
- *   lengths [rows]: slots in use (values outside [0, capacity] are taken as the nearest of them)
+ *   lengths [rows]: slots in use (values outside [0, capacity] are taken as the nearest of them); what the other slots hold, bytes
+ *          that are no scale included, has no effect
  *   failed  [1]: set to 1 by an append that found no room for some of its tokens; nothing here clears it
  * One call at a time works on a cache: calls on several streams are the caller's to order. */
 typedef struct after_kv4 {
