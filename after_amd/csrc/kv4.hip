@@ -629,15 +629,16 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
         for (int g = 0; g < G; ++g) {
             u32x4 pf[NM][NP];
             if (special) {
-                // (a slot that is not seen, or a NaN group: what a masked slot holds must not reach the sum, 0 x NaN would)
+                // (a slot that is not seen, or a NaN group, whatever its codes: what a masked slot holds must not reach the sum, 0 x NaN
+                // would)
 #pragma unroll
                 for (int nm = 0; nm < NM; ++nm) {
                     float y[8];
                     bf16x8 z[PIECES];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const int byte = j * G + g;
-                        y[j] = t0 + 8 * kq + j >= vis[nm] ? 0.f : p[nm][j] * byte_scale(w.vs[byte >> 2] >> 8 * (byte & 3) & 255u);
+                        const unsigned b = w.vs[(j * G + g) >> 2] >> 8 * ((j * G + g) & 3) & 255u;
+                        y[j] = t0 + 8 * kq + j >= vis[nm] ? 0.f : b == kBadByte ? NAN : p[nm][j] * byte_scale(b);
                     }
                     pieces8<PIECES>(y, z);
 #pragma unroll

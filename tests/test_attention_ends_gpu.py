@@ -50,3 +50,18 @@ def test_bytes_behind_the_length_have_no_effect(hip_device, kind, dim, T, capaci
         c.weights.zero_()
         assert torch.equal(c.attend(q), good)
         assert torch.equal(c.attend(q, accumulate=True), good) and torch.equal(c.weights, w)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("T, capacity", [(3, 128), (3, 640), (24, 640)])
+def test_a_group_of_nan_has_any_codes(hip_device, kind, dim, T, capacity):
+    """Byte 255 reads as NaN whatever the group's codes are."""
+    lens = [70, 41]
+    c = filled(hip_device, 2, 2, dim, capacity, lens, 14)
+    c.value_scales[0, 1, 20, 1] = c.value_scales[1, 0, 40, 0] = 255  # (the second one is the newest slot)
+    q = torch.randn(2, T, 4, dim, generator=gen(3)).to(hip_device, TYPES[kind])
+    out = c.attend(q)
+    assert torch.isnan(c.read()[1][0, 1, 20, 32:64]).all()
+    assert torch.isnan(out[0, :, 2:, 32:64]).all() and torch.isnan(out[1, -1, :2, :32]).all() and torch.isnan(out).sum() == (T * 2 + 2) * 32
+    check_attend(c, q, lens, out, dim ** -0.5)
