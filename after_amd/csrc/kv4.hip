@@ -360,6 +360,7 @@ __device__ __forceinline__ void pieces8(const float (&x)[8], bf16x8 (&p)[N]) {
 }
 
 constexpr int kRing = 3;  // tiles of 32 tokens that each wave has in LDS
+constexpr float kLift = 66.f, kDrop = 0x1p-66f;  // probabilities are held 2^kLift times as large until they are weighed
 template <int D>
 constexpr int kTileBytes = 32 * D + 2 * D;  // keys, values, key scales, value scales
 
@@ -577,18 +578,19 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
                 }
             }
             // The maximum moves only when a score outgrows it by 2^2, so that most tiles need no exchange between lanes: a
-            // probability of up to 4 is as exact (and still has an exponent to spare for every scale byte, below).
+            // probability of up to 4 is as exact.  It is a whole number, so that probabilities can be held 2^kLift times as large
+            // (below) without another rounding.
             top *= a.scale2;
             if (__any(top > mx[nm] + 2.f)) {
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
-                const float now = fmaxf(mx[nm], top), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[nm] - now);
+                const float now = rintf(fmaxf(mx[nm], top)), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[nm] - now);
                 mx[nm] = now;
                 l[nm] *= f;
 #pragma unroll
                 for (int i = 0; i < 2 * G; ++i) o[nm][i] = o[nm][i] * f;
             }
-            const float off = mx[nm] == -INFINITY ? 0.f : mx[nm];
+            const float off = (mx[nm] == -INFINITY ? 0.f : mx[nm]) - kLift;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 p[nm][j] = __builtin_amdgcn_exp2f(fmaf(sc[nm][j >> 2][j & 3], a.scale2, -off));
@@ -597,9 +599,10 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
         }
         // P times the scale of its token and group, as bf16 pieces.  The scale is a power of two: its exponent is added to the
         // probability's as an integer, two tokens at a time -- one v_perm_b32 for both bytes, one v_pk_mad_u16, and a maximum
-        // with 0 for what falls below bf16's exponents (products below 2^-126 vanish; p = 0 counts as 2^-127): a third of the
-        // instructions of extracting eight scales per group and multiplying.  Pieces are cut off, not rounded, so that none is
-        // negative; a single one is rounded.
+        // with 0 for what falls below bf16's exponents (products below 2^-126 vanish): a third of the instructions of extracting
+        // eight scales per group and multiplying.  With p held 2^kLift times as large, a p of 0 stays below them under every
+        // scale less than 2^65; larger ones are multiplied.  Pieces are cut off, not rounded, so that none is negative; a single
+        // one is rounded.
         u16x2 bits[NM][NP][4];
 #pragma unroll
         for (int nm = 0; nm < NM; ++nm)
@@ -621,16 +624,16 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
                         u = __builtin_amdgcn_perm(__float_as_uint(x1), __float_as_uint(x0), 0x07060302u);
                     x0 -= __uint_as_float(u << 16);
                     x1 -= __uint_as_float(u & 0xFFFF0000u);
-                    bits[nm][q][i] = __builtin_bit_cast(u16x2, u) - (unsigned short)(127 << 7);
+                    bits[nm][q][i] = __builtin_bit_cast(u16x2, u) - (unsigned short)((127 + (int)kLift) << 7);
                 }
             }
-        const bool special = masked || __any((w.look & 0x7F7F7F7Fu) + 0x01010101u & w.look & 0x80808080u);
+        const bool special = masked || __any(w.look & w.look << 1 & 0x80808080u);  // (bytes from 192 on: the two highest bits)
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             u32x4 pf[NM][NP];
             if (special) {
-                // (a slot that is not seen, or a NaN group, whatever its codes: what a masked slot holds must not reach the sum, 0 x NaN
-                // would)
+                // (a slot that is not seen, a large scale, or a NaN group, whatever its codes: what a masked slot holds must not reach
+                // the sum, 0 x NaN would)
 #pragma unroll
                 for (int nm = 0; nm < NM; ++nm) {
                     float y[8];
@@ -638,7 +641,7 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const unsigned b = w.vs[(j * G + g) >> 2] >> 8 * ((j * G + g) & 3) & 255u;
-                        y[j] = t0 + 8 * kq + j >= vis[nm] ? 0.f : b == kBadByte ? NAN : p[nm][j] * byte_scale(b);
+                        y[j] = t0 + 8 * kq + j >= vis[nm] ? 0.f : b == kBadByte ? NAN : p[nm][j] * kDrop * byte_scale(b);
                     }
                     pieces8<PIECES>(y, z);
 #pragma unroll
@@ -677,6 +680,7 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
     for (int nm = 0; nm < NM; ++nm) {
         l[nm] += __shfl_xor(l[nm], 16);
         l[nm] += __shfl_xor(l[nm], 32);
+        l[nm] *= kDrop;
         if constexpr (COLS < 16) {
 #pragma unroll
             for (int i = 0; i < 2 * G; ++i)

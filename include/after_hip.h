@@ -581,6 +581,7 @@ long long after_conv1_act_launches(void);
  * mask does (transformerv2.py:62-96).  causal = 0: all keys.  A query that sees no key gets zeros; what a query does not see
  * has no effect on it, NaN and infinities included.  Rows of out behind the last sequence stay as they are, or are set to
  * zero with zero_rest.  D = 64 or 128.  fp32: fp32 products; bf16 / fp16: products of that type, sums and softmax in fp32.
+ * Sums are divided at the end: they stay finite while the largest value times the keys that a query sees is below 2^120.
  * workspace: scratch of the size that _workspace names (its answer depends on the arguments alone; two calls that may run at the
  * same time need two), with which the keys of a few queries are shared out over the chip; NULL: they are not. */
 int after_attend_packed_workspace(int type, long long q_rows, long long k_rows, int n_seqs, int heads, int kv_heads, int head_dim,
@@ -645,7 +646,8 @@ int after_kv4_read(const after_kv4* c, void* k, void* v, int type, const int* st
 /* out [rows, tokens, heads, D] (contiguous, of q's type): attention of the newest `tokens` tokens of each row, whose keys are
  * in the cache already: query t sees the slots below lengths[r] - tokens + t + 1, none of them: zeros.  (A row with fewer new
  * tokens than others has its queries at the end.)  accumulate: weights = decay * weights + the probabilities that each slot
- * in use received, summed over tokens and the group's heads (decay = 0: they are replaced).  The workspace is scratch: its
+ * in use received, summed over tokens and the group's heads (decay = 0: they are replaced).  Sums are divided at the end: they
+ * stay finite while the largest value times the slots that a query sees is below 2^120.  The workspace is scratch: its
  * size depends on the arguments alone, and two calls that may run at the same time need two. */
 int after_kv4_attend_workspace(const after_kv4* c, int type, int heads, int tokens, int accumulate, long long* bytes);
 typedef struct after_kv4_query {

@@ -65,3 +65,37 @@ def test_a_group_of_nan_has_any_codes(hip_device, kind, dim, T, capacity):
     assert torch.isnan(c.read()[1][0, 1, 20, 32:64]).all()
     assert torch.isnan(out[0, :, 2:, 32:64]).all() and torch.isnan(out[1, -1, :2, :32]).all() and torch.isnan(out).sum() == (T * 2 + 2) * 32
     check_attend(c, q, lens, out, dim ** -0.5)
+
+
+# ---------------------------------------------------------------------------------------------------------------- values
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("heads, T, capacity", [(2, 1, 64), (2, 1, 640), (20, 1, 640), (2, 20, 640), (24, 2, 64)])
+@pytest.mark.parametrize("small, large", [(0, 124), (0, 60), (-60, 63), (-60, 10), (-100, 64)])
+def test_a_slot_without_weight(hip_device, kind, heads, T, capacity, small, large):
+    """Values of 2^large in slots whose probability is 0 in 32 bits, next to values of 2^small."""
+    g = gen(4)
+    k, v = (torch.randn(1, 60, 1, 64, generator=g) for _ in range(2))
+    v *= 2.0 ** small
+    for s in (5, 17, 40):  # (slot 17's second group only)
+        v[0, s, 0, 32 if s == 17 else 0:] = torch.randn(32 if s == 17 else 64, generator=g).clamp(-5, 5) * 2.0 ** large
+        k[0, s] = -4.0
+    k, q = k.clamp(-4, 1), 2 + 0.25 * torch.rand(1, T, heads, 64, generator=g)  # (those slots' scores are some 195 octaves below)
+    c = KVCache4(1, 1, 64, capacity, hip_device)
+    c.append(k.to(hip_device), v.to(hip_device))
+    q = q.to(hip_device, TYPES[kind])
+    check_attend(c, q, [60], c.attend(q, scale=0.25), 0.25)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("T, capacity", [(1, 64), (2, 640), (40, 640)])
+def test_values_over_the_whole_range(hip_device, kind, T, capacity):
+    """Scale bytes from 2^-90 to 2^110 side by side, all with a part in the sum."""
+    g = gen(5)
+    v = torch.randn(1, 60, 1, 64, generator=g) * 2.0 ** torch.randint(-90, 110, (1, 60, 1, 2), generator=g).repeat_interleave(32, -1)
+    c = KVCache4(1, 1, 64, capacity, hip_device)
+    c.append(torch.randn(1, 60, 1, 64, generator=g).to(hip_device), v.to(hip_device))
+    q = torch.randn(1, T, 2, 64, generator=g).to(hip_device, torch.float32 if kind == "fp16" else TYPES[kind])
+    if kind == "fp16":  # (fp16 holds no value beyond 65504: the same without the upper half)
+        c.value_scales.clamp_(max=120)
+        q = q.half()
+    check_attend(c, q, [60], c.attend(q), 0.125)
