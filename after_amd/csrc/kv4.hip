@@ -74,6 +74,7 @@ __device__ __forceinline__ int scale_byte(unsigned top) {
     return min(max(b, kMinByte), kMaxByte);
 }
 __device__ __forceinline__ float byte_scale(int b) { return __uint_as_float((unsigned)b << 23); }
+__device__ __forceinline__ float scale_or_nan(unsigned b) { return __uint_as_float(b << 23 | (b + 1) >> 8); }  // (255: NaN)
 
 // two floats -> the low byte: two codes
 __device__ __forceinline__ unsigned round4(float a, float b, float scale) {
@@ -628,12 +629,18 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
                 }
             }
         const bool special = masked || __any(w.look & w.look << 1 & 0x80808080u);  // (bytes from 192 on: the two highest bits)
+        if (special) {
+#pragma unroll
+            for (int nm = 0; nm < NM; ++nm)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) p[nm][j] *= kDrop;
+        }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             u32x4 pf[NM][NP];
             if (special) {
                 // (a slot that is not seen, a large scale, or a NaN group, whatever its codes: what a masked slot holds must not reach
-                // the sum, 0 x NaN would)
+                // the sum, 0 x NaN would; all ones or none by a shift, since the compiler branches around a choice)
 #pragma unroll
                 for (int nm = 0; nm < NM; ++nm) {
                     float y[8];
@@ -641,7 +648,7 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const unsigned b = w.vs[(j * G + g) >> 2] >> 8 * ((j * G + g) & 3) & 255u;
-                        y[j] = t0 + 8 * kq + j >= vis[nm] ? 0.f : b == kBadByte ? NAN : p[nm][j] * kDrop * byte_scale(b);
+                        y[j] = __uint_as_float(__float_as_uint(p[nm][j] * scale_or_nan(b)) & (unsigned)(t0 + 8 * kq + j - vis[nm] >> 31));
                     }
                     pieces8<PIECES>(y, z);
 #pragma unroll
