@@ -1,0 +1,17 @@
+// What the attention kernels of attention.hip and kv4.hip share.
+#pragma once
+#include <hip/hip_runtime.h>
+
+namespace after {
+
+// A softmax's running maximum is a product rounded to 32 bits, round(top * scale2), and fmaf(score, scale2, -maximum) rounds no
+// product: at the largest score the two are up to 2^-24 of the maximum apart, more than an exponential's range holds from 2^32 on.
+// Beyond this maximum, where that is 1/4, products are rounded before the difference.
+constexpr float kFarTop = 0x1p22f;
+__device__ __forceinline__ float scaled_below(float s, float scale2, float maximum) {
+#pragma clang fp contract(off)
+    const float x = s * scale2;
+    return x - maximum;
+}
+
+}  // namespace after

@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "attention.h"
 #include "common.h"
 #include "gemm_pipe.h"
 
@@ -254,6 +255,8 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
     float mx = -INFINITY, l = 0.f;
+    bool far = false;                                      // some query's maximum is beyond kFarTop
+    float off = 0.f, times = a.scale2, limit = -INFINITY;  // p = 2^(score times - off); the maximum moves beyond the limit
 
     int checked = 0;
     if (tid < 3) odd_rows[tid] = 0;
@@ -317,19 +320,27 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
             for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[f][e]);
         top = fmaxf(top, __shfl_xor(top, 32)) * a.scale2;
         // the maximum moves only when scores outgrow it by 2^8: probabilities up to 256 are as exact, and a rescale is rare
-        if (__any(top > mx + 8.f)) {
+        // (where the maximum is beyond kFarTop, scores are brought down here in every tile: the usual one has no branch for it)
+        if (__any(top > limit)) {
             const float now = fmaxf(mx, top), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - now);
             mx = now;
+            far = __any(fabsf(now) > kFarTop && now != -INFINITY);
+            off = far || now == -INFINITY ? 0.f : now, times = far ? 1.f : a.scale2, limit = far ? -INFINITY : now + 8.f;
             l *= f;
 #pragma unroll
             for (int i = 0; i < DT; ++i) o[i] = o[i] * f;
+            if (far) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) sc[g][e] = scaled_below(sc[g][e], a.scale2, mx == -INFINITY ? 0.f : mx);
+            }
         }
-        const float off = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
         for (int f = 0; f < 2; ++f)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                sc[f][e] = __builtin_amdgcn_exp2f(fmaf(sc[f][e], a.scale2, -off));
+                sc[f][e] = __builtin_amdgcn_exp2f(fmaf(sc[f][e], times, -off));
                 l += sc[f][e];
             }
         // O^T += V^T P^T
@@ -474,6 +485,8 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
     float mx = -INFINITY, l = 0.f;
+    bool far = false;
+    float off = 0.f, times = a.scale2, limit = -INFINITY;  // p = 2^(score times - off); the maximum moves beyond the limit
 
     const unsigned k_lds = (unsigned)(unsigned long)(__attribute__((address_space(3))) char*)lds + wave * (2 * HALF), v_lds = k_lds + HALF;
     u32x4* lk = reinterpret_cast<u32x4*>(lds + wave * (2 * HALF));
@@ -527,17 +540,22 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
 #pragma unroll
         for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[e]);
         top = fmaxf(top, __shfl_xor(top, 32)) * a.scale2;
-        if (__any(top > mx + 8.f)) {  // (as above)
+        if (__any(top > limit)) {  // (as above)
             const float now = fmaxf(mx, top), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - now);
             mx = now;
+            far = __any(fabsf(now) > kFarTop && now != -INFINITY);
+            off = far || now == -INFINITY ? 0.f : now, times = far ? 1.f : a.scale2, limit = far ? -INFINITY : now + 8.f;
             l *= f;
 #pragma unroll
             for (int i = 0; i < DT; ++i) o[i] = o[i] * f;
+            if (far) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sc[e] = scaled_below(sc[e], a.scale2, mx == -INFINITY ? 0.f : mx);
+            }
         }
-        const float off = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale2, -off));
+            sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], times, -off));
             l += sc[e];
         }
         if (more)

@@ -99,3 +99,27 @@ def test_values_over_the_whole_range(hip_device, kind, T, capacity):
         c.value_scales.clamp_(max=120)
         q = q.half()
     check_attend(c, q, [60], c.attend(q), 0.125)
+
+
+# ---------------------------------------------------------------------------------------------------------------- scores
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("scale", [0.125, 0.3, -0.7])
+def test_prompts_with_scores_of_any_size(hip_device, kind, dim, form, scale):
+    """Scores far beyond 2^32, so that even their roundings are far apart: the largest takes all."""
+    t, g = TYPES[kind], gen(6)
+    big = 250.0 if kind == "fp16" else 1e15
+    size = torch.randperm(150, generator=g) + 100.0
+    for x in (1.0, 1.37, 1.91):
+        q = torch.full((150, 2, dim), x * (3e4 if kind == "fp16" else big), device=hip_device).to(t)
+        k = (size.view(150, 1, 1) * big).expand(150, 1, dim).contiguous().to(hip_device, t)
+        v = torch.randn(150, 1, dim, generator=g).to(hip_device, t)
+        out = packed(form, q, k, v, [150], scale=scale)
+        sign = 1 if scale > 0 else -1
+        # (a bf16 key keeps eight bits of its size: of equal ones, all)
+        s = k[:, 0, 0].double() * sign
+        for i in (0, 1, 31, 64, 99, 149):
+            best = (s[:i + 1] == s[:i + 1].max()).nonzero()[:, 0]
+            want = v[best].double().mean(0)
+            assert ((out[i].double() - want).abs() <= 2 * ref.HALF[t] * v[best].double().abs().amax(0)).all(), (x, i)
