@@ -16,6 +16,7 @@
 
 #include <cmath>
 
+#include "attention.h"
 #include "common.h"
 #include "gemm_pipe.h"
 
@@ -330,7 +331,7 @@ struct AttendArgs {
     f32x2* part_ml;   // [pieces][m_rows]: largest score, sum of exponentials to it
     f32x2* final_ml;  // [rows * H][m_rows]: the same over all pieces, if weights are wanted
     int2* ends;       // [rows * H]: the first and the last piece of a row and head, written by the workers that hold its ends
-    float* scores;    // [rows * H][m_rows][C] or nullptr
+    float* scores;    // [rows * H][m_rows][C], not scaled, or nullptr
 };
 
 // How the slots in use are shared out: the steps of 32 slots of all rows and heads, one behind the other, are cut into equal
@@ -477,10 +478,12 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
 
     f32x4 o[NM][2 * G];
     float mx[NM], l[NM];
+    float off[NM], times[NM], limit[NM];  // p = 2^(score times - off); the maximum moves beyond the limit
 #pragma unroll
     for (int nm = 0; nm < NM; ++nm) {
-        mx[nm] = -INFINITY;
+        mx[nm] = limit[nm] = -INFINITY;
         l[nm] = 0.f;
+        off[nm] = -kLift, times[nm] = a.scale2;
 #pragma unroll
         for (int i = 0; i < 2 * G; ++i) o[nm][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -574,27 +577,34 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
                 const int m = nm * 16 + col;
                 if (m < a.m_rows && piece_of == 0) {
                     float* to = a.scores + ((size_t)rh * a.m_rows + m) * c.capacity + t0 + 8 * kq;
-                    *reinterpret_cast<f32x4*>(to) = sc[nm][0] * a.scale2;
-                    *reinterpret_cast<f32x4*>(to + 4) = sc[nm][1] * a.scale2;
+                    *reinterpret_cast<f32x4*>(to) = sc[nm][0];
+                    *reinterpret_cast<f32x4*>(to + 4) = sc[nm][1];
                 }
             }
             // The maximum moves only when a score outgrows it by 2^2, so that most tiles need no exchange between lanes: a
             // probability of up to 4 is as exact.  It is a whole number, so that probabilities can be held 2^kLift times as large
-            // (below) without another rounding.
+            // (below) without another rounding.  Where it is beyond kFarTop, scores are brought down here in every tile: the usual
+            // one has no branch for it.
             top *= a.scale2;
-            if (__any(top > mx[nm] + 2.f)) {
+            if (__any(top > limit[nm])) {
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
                 const float now = rintf(fmaxf(mx[nm], top)), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[nm] - now);
+                const float below = now == -INFINITY ? 0.f : now;
+                const bool far = __any(fabsf(below) > kFarTop);
                 mx[nm] = now;
+                off[nm] = (far ? 0.f : below) - kLift, times[nm] = far ? 1.f : a.scale2, limit[nm] = far ? -INFINITY : now + 2.f;
                 l[nm] *= f;
 #pragma unroll
                 for (int i = 0; i < 2 * G; ++i) o[nm][i] = o[nm][i] * f;
+                if (far) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sc[nm][j >> 2][j & 3] = scaled_below(sc[nm][j >> 2][j & 3], a.scale2, below);
+                }
             }
-            const float off = (mx[nm] == -INFINITY ? 0.f : mx[nm]) - kLift;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                p[nm][j] = __builtin_amdgcn_exp2f(fmaf(sc[nm][j >> 2][j & 3], a.scale2, -off));
+                p[nm][j] = __builtin_amdgcn_exp2f(fmaf(sc[nm][j >> 2][j & 3], times[nm], -off[nm]));
                 l[nm] += p[nm][j];
             }
         }
@@ -973,6 +983,7 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_ker
     load_queries<TYPE, D, NP>(a, r, h, m0, len, qf, vis);
     f32x4 o[2][2 * G];
     float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float off[2] = {0.f, 0.f}, times[2] = {a.scale2, a.scale2}, limit[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int nm = 0; nm < 2; ++nm)
 #pragma unroll
@@ -1020,20 +1031,26 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_ker
 #pragma unroll
                 for (int j = 0; j < 8; ++j) top = fmaxf(top, sc[nm][j >> 2][j & 3]);
                 top *= a.scale2;
-                if (__any(top > mx[nm] + 8.f)) {  // (as in attend_packed: the maximum moves when scores outgrow it by 2^8)
+                if (__any(top > limit[nm])) {  // (as in attend_packed: the maximum moves when scores outgrow it by 2^8)
                     top = fmaxf(top, __shfl_xor(top, 16));
                     top = fmaxf(top, __shfl_xor(top, 32));
                     const float now = fmaxf(mx[nm], top), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[nm] - now);
+                    const float below = now == -INFINITY ? 0.f : now;
+                    const bool far = __any(fabsf(below) > kFarTop);
                     mx[nm] = now;
+                    off[nm] = far ? 0.f : below, times[nm] = far ? 1.f : a.scale2, limit[nm] = far ? -INFINITY : now + 8.f;
                     l[nm] *= f;
 #pragma unroll
                     for (int i = 0; i < 2 * G; ++i) o[nm][i] = o[nm][i] * f;
+                    if (far) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) sc[nm][j >> 2][j & 3] = scaled_below(sc[nm][j >> 2][j & 3], a.scale2, below);
+                    }
                 }
-                const float off = mx[nm] == -INFINITY ? 0.f : mx[nm];
                 float p[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    p[j] = __builtin_amdgcn_exp2f(fmaf(sc[nm][j >> 2][j & 3], a.scale2, -off));
+                    p[j] = __builtin_amdgcn_exp2f(fmaf(sc[nm][j >> 2][j & 3], times[nm], -off[nm]));
                     l[nm] += p[j];
                 }
                 pieces8<NP>(p, pf[nm]);
@@ -1157,8 +1174,12 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(AttendArgs a, int slot
     for (int m = 0; m < a.m_rows; ++m) {
         const f32x4 x = *reinterpret_cast<const f32x4*>(scores + (size_t)m * c.capacity);
         const float top = ml[m][0], off = top == -INFINITY ? 0.f : top, inv = ml[m][1] == 0.f ? 0.f : 1.f / ml[m][1];
+        const bool far = fabsf(off) > kFarTop;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[i] += x[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[i] - off) * inv;
+        for (int i = 0; i < 4; ++i) {  // (rounded as where they were summed up: the probabilities add up to 1)
+            const float y = far ? scaled_below(x[i], a.scale2, off) : fmaf(x[i], a.scale2, -off);
+            sum[i] += y == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(y) * inv;
+        }
     }
     float* w = c.weights + (size_t)rh * c.capacity + s;
     // (the four slots are inside the capacity; those past the length keep what they hold)
@@ -1202,6 +1223,7 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_wei
         if (m0 + (lane & 31) < a.m_rows) ml = a.final_ml[(size_t)rh * a.m_rows + m0 + (lane & 31)];
         float off[2][4], inv[2][4];  // of query 16 nm + 4 kq + i
         int sees[2][4];
+        bool far = false;
 #pragma unroll
         for (int nm = 0; nm < 2; ++nm)
 #pragma unroll
@@ -1209,9 +1231,11 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_wei
                 const int m = nm * 16 + 4 * kq + i;
                 const float top = __shfl(ml[0], m), sum = __shfl(ml[1], m);
                 off[nm][i] = top == -INFINITY ? 0.f : top;
+                far |= fabsf(off[nm][i]) > kFarTop;
                 inv[nm][i] = sum == 0.f ? 0.f : 1.f / sum;
                 sees[nm][i] = __shfl(vis[nm], 4 * kq + i);
             }
+        far = __any(far);
         const int all_see = m0 + 32 <= a.m_rows ? len - a.tokens + m0 / a.group + 1 : 0;
         if (widen.mine()) widen.load_keys(raw, begin);
         for (int t0 = begin; t0 < end; t0 += kWideTile, ++n) {
@@ -1223,6 +1247,12 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_wei
             for (int part = 0; part < 2; ++part) {
                 f32x4 sc[2][2];
                 scores32<D, NP, false>(stage + part * (Widen<D>::KEYS / 2), qf, sc);
+                if (far) {  // (as where they were summed up)
+#pragma unroll
+                    for (int nm = 0; nm < 2; ++nm)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) sc[nm][j >> 2][j & 3] = scaled_below(sc[nm][j >> 2][j & 3], a.scale2, off[nm][j & 3]);
+                }
 #pragma unroll
                 for (int f = 0; f < 2; ++f) {
                     const int tok = 32 * part + 8 * (l15 >> 2) + 4 * f + (l15 & 3), s = t0 + tok;
@@ -1231,7 +1261,7 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_wei
                     for (int nm = 0; nm < 2; ++nm)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const float x = __builtin_amdgcn_exp2f(fmaf(sc[nm][f][i], a.scale2, -off[nm][i]));
+                            const float x = __builtin_amdgcn_exp2f(far ? sc[nm][f][i] : fmaf(sc[nm][f][i], a.scale2, -off[nm][i]));
                             w = t0 + kWideTile <= all_see || s < sees[nm][i] ? fmaf(x, inv[nm][i], w) : w;
                         }
                     w += __shfl_xor(w, 16);

@@ -123,3 +123,30 @@ def test_prompts_with_scores_of_any_size(hip_device, kind, dim, form, scale):
             best = (s[:i + 1] == s[:i + 1].max()).nonzero()[:, 0]
             want = v[best].double().mean(0)
             assert ((out[i].double() - want).abs() <= 2 * ref.HALF[t] * v[best].double().abs().amax(0)).all(), (x, i)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("heads, T, capacity", [(1, 1, 64), (1, 1, 640), (12, 1, 640), (20, 1, 64), (40, 1, 640), (2, 40, 640)])
+@pytest.mark.parametrize("scale", [0.125, 0.3, -0.7])
+def test_cached_scores_of_any_size(hip_device, kind, heads, T, capacity, scale):
+    """... over the cache: the output is the best slot's values, and that slot receives all of the attention."""
+    t, g, n = TYPES[kind], gen(7), 50
+    size = torch.randperm(n, generator=g)
+    k = (2.0 ** (size - 12 if kind == "fp16" else size + 20)).view(1, n, 1, 1).expand(1, n, 1, 64)
+    v = torch.randn(1, n, 1, 64, generator=g)
+    c = KVCache4(1, 1, 64, capacity, hip_device)
+    c.append(k.contiguous().to(hip_device), v.to(hip_device))
+    K, V = ref.cache_values(c)
+    for x in (1.0, 1.37, 1.91):
+        q = torch.full((1, T, heads, 64), x * (3e4 if kind == "fp16" else 1e15), device=hip_device).to(t)
+        c.weights.zero_()
+        out, weights = c.attend(q, scale=scale, accumulate=True), torch.zeros(n)
+        for i in range(T):
+            seen = size[:max(0, n - T + i + 1)]
+            best = int(seen.argmax() if scale > 0 else seen.argmin())
+            weights[best] += heads
+            want = V[0, 0, best].expand(heads, 64)
+            close(out[0, i], want, 2 * ref.HALF[t] * want.abs(), f"query {i}")
+        # (at a negative scale the smallest key is the best: its score is 2^-12 x 3e4 x 64 x 0.7 from the next all the same)
+        # (an exponential and the sum that holds it alone: from arguments rounded at up to 8 and 8 octaves, 16 x 2^-24)
+        close(c.weights[0, 0, :n], weights.double(), 2.0 ** -19 * weights, "weights")
