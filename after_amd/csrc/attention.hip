@@ -38,6 +38,11 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int BM = 128, BN = 64;
+// In fp16 products probabilities, and the sum that divides them, are held 2^7 times as large: up to 2^15 with a maximum that moves at
+// 2^8, and what is rounded to nothing is below 2^-32 of the largest, where without it keys 25.2 octaves below vanished from the
+// output but not from the sum (2^17 of them and a key of value 0: 0 instead of 0.0034).
+template <int TYPE>
+constexpr float kLift = TYPE == AFTER_T_F16 ? 7.f : 0.f;
 
 template <int TYPE>
 struct Elem;
@@ -256,7 +261,7 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
         for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
     float mx = -INFINITY, l = 0.f;
     bool far = false;                                      // some query's maximum is beyond kFarTop
-    float off = 0.f, times = a.scale2, limit = -INFINITY;  // p = 2^(score times - off); the maximum moves beyond the limit
+    float off = -kLift<TYPE>, times = a.scale2, limit = -INFINITY;  // p = 2^(score times - off); the maximum moves beyond the limit
 
     int checked = 0;
     if (tid < 3) odd_rows[tid] = 0;
@@ -325,7 +330,7 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
             const float now = fmaxf(mx, top), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - now);
             mx = now;
             far = __any(fabsf(now) > kFarTop && now != -INFINITY);
-            off = far || now == -INFINITY ? 0.f : now, times = far ? 1.f : a.scale2, limit = far ? -INFINITY : now + 8.f;
+            off = (far || now == -INFINITY ? 0.f : now) - kLift<TYPE>, times = far ? 1.f : a.scale2, limit = far ? -INFINITY : now + 8.f;
             l *= f;
 #pragma unroll
             for (int i = 0; i < DT; ++i) o[i] = o[i] * f;
@@ -360,7 +365,7 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
                 for (int s = 0; s < 2; ++s) {
                     typename E::V8 pf;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) pf[e] = (T)sc[f][8 * s + e];  // (the products' own type: half a step of 2^-9 / 2^-12 each)
+                    for (int e = 0; e < 8; ++e) pf[e] = (T)sc[f][8 * s + e];  // (the products' own type: half a step, 2^-9 / 2^-12, each)
 #pragma unroll
                     for (int i = 0; i < DT; ++i) {
                         // lane l of 16 reads 8 bytes of row l / 4: it gets column l of the four rows
@@ -486,7 +491,7 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
         for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
     float mx = -INFINITY, l = 0.f;
     bool far = false;
-    float off = 0.f, times = a.scale2, limit = -INFINITY;  // p = 2^(score times - off); the maximum moves beyond the limit
+    float off = -kLift<TYPE>, times = a.scale2, limit = -INFINITY;  // p = 2^(score times - off); the maximum moves beyond the limit
 
     const unsigned k_lds = (unsigned)(unsigned long)(__attribute__((address_space(3))) char*)lds + wave * (2 * HALF), v_lds = k_lds + HALF;
     u32x4* lk = reinterpret_cast<u32x4*>(lds + wave * (2 * HALF));
@@ -544,7 +549,7 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
             const float now = fmaxf(mx, top), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - now);
             mx = now;
             far = __any(fabsf(now) > kFarTop && now != -INFINITY);
-            off = far || now == -INFINITY ? 0.f : now, times = far ? 1.f : a.scale2, limit = far ? -INFINITY : now + 8.f;
+            off = (far || now == -INFINITY ? 0.f : now) - kLift<TYPE>, times = far ? 1.f : a.scale2, limit = far ? -INFINITY : now + 8.f;
             l *= f;
 #pragma unroll
             for (int i = 0; i < DT; ++i) o[i] = o[i] * f;

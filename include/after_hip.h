@@ -580,7 +580,8 @@ long long after_conv1_act_launches(void);
  * before (chunk = 1: the keys up to its own), and with window > 0 of the earlier chunks only keys > p - window, as DenoiserV2's
  * mask does (transformerv2.py:62-96).  causal = 0: all keys.  A query that sees no key gets zeros; what a query does not see
  * has no effect on it, NaN and infinities included.  Rows of out behind the last sequence stay as they are, or are set to
- * zero with zero_rest.  D = 64 or 128.  fp32: fp32 products; bf16 / fp16: products of that type, sums and softmax in fp32.
+ * zero with zero_rest.  D = 64 or 128.  fp32: fp32 products; bf16 / fp16: products of that type, sums and softmax in fp32: a
+ * probability is rounded to the type before it is multiplied (fp16: what is below 2^-32 of a query's largest counts as 0).
  * Sums are divided at the end: they stay finite while the largest value times the keys that a query sees is below 2^120.
  * workspace: scratch of the size that _workspace names (its answer depends on the arguments alone; two calls that may run at the
  * same time need two), with which the keys of a few queries are shared out over the chip; NULL: they are not. */

@@ -150,3 +150,30 @@ def test_cached_scores_of_any_size(hip_device, kind, heads, T, capacity, scale):
         # (at a negative scale the smallest key is the best: its score is 2^-12 x 3e4 x 64 x 0.7 from the next all the same)
         # (an exponential and the sum that holds it alone: from arguments rounded at up to 8 and 8 octaves, 16 x 2^-24)
         close(c.weights[0, 0, :n], weights.double(), 2.0 ** -19 * weights, "weights")
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_many_probabilities_below_the_smallest_of_fp16(hip_device, kind):
+    """Every 512th key's score is 25.2 octaves above the others', its value 0: the others weigh 1.3e-5 together."""
+    n, t = 1 << 17, TYPES[kind]
+    q, k, v = torch.zeros(1, 1, 64), torch.zeros(n, 1, 64), torch.full((n, 1, 64), 1000.0)
+    q[..., 0], k[::512, 0, 0], v[::512] = 1.0, 25.2 * math.log(2), 0.0
+    q, k, v = (x.to(hip_device, t) for x in (q, k, v))
+    out = attend_packed(q, k, v, starts([1], hip_device), starts([n], hip_device), scale=1.0)
+    rest = 511 * math.exp(-float(k[0, 0, 0]))
+    want = torch.full((1, 1, 64), 1000 * rest / (1 + rest), dtype=torch.float64)
+    # (in fp16 products a probability is kept to 2^-32 of the largest, absolutely; sums in 32 bits, above and below the line, of chains of
+    # at most n / 256 = 512 terms: 6.2e-5)
+    tol = want * ({torch.bfloat16: 2.0 ** -8}.get(t, 0) + 7e-5 + ref.HALF[t]) + (511000 * 2.0 ** -32 + 2.0 ** -25 if kind == "fp16" else 0)
+    close(out, want, tol)
+
+
+def test_small_probabilities_in_wide_tiles(hip_device):
+    n, seqs, m, down = 3000, 60, 40, 24.5 * math.log(2)
+    q, k, v = torch.zeros(seqs * m, 8, 64), torch.zeros(seqs, n, 8, 64), torch.ones(seqs, n, 8, 64)
+    q[..., 0], k[:, 0, :, 0], v[:, 0] = 1.0, down, 0.0
+    q, k, v = (x.to(hip_device, torch.float16) for x in (q, k.flatten(0, 1), v.flatten(0, 1) * 100))
+    out = attend_packed(q, k, v, starts([m] * seqs, hip_device), starts([n] * seqs, hip_device), causal=False, scale=1.0)
+    rest = (n - 1) * math.exp(-float(k[0, 0, 0]))
+    want = torch.full(out.shape, 100 * rest / (1 + rest), dtype=torch.float64)
+    close(out, want, 100 * n * 2.0 ** -32 + want * (2 * n * 2.0 ** -24 + 2.0 ** -11) + 2.0 ** -25)  # (sums of n terms, above and below the line)
