@@ -14,4 +14,7 @@ __device__ __forceinline__ float scaled_below(float s, float scale2, float maxim
     return x - maximum;
 }
 
+// What a query's sum of exponentials divides by: nothing seen gives zeros, but where every score is -inf, 0 / 0 is NaN
+__device__ __forceinline__ float inverse_sum(float sum, bool sees) { return sum == 0.f ? (sees ? NAN : 0.f) : 1.f / sum; }
+
 }  // namespace after

@@ -408,7 +408,7 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
 
     // to memory by way of LDS: a lane holds one row's every eighth group of four channels, a store of whole rows takes half the time
     l += __shfl_xor(l, 32);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = inverse_sum(l, first < last);
     constexpr int PITCH = D * (int)sizeof(T) + 16;
     char* mine = lds + wave * (32 * PITCH);
     lds_barrier();  // (the tiles are no longer read)
@@ -671,8 +671,9 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
     }
     if (row0 + r >= rows) return;
     if (used <= 1) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const int tr = a.by_group(row0 + r), gr = row0 + r - tr * a.group;
+        seen(a, tr + nk - nq, nk, first, last);
+        const float inv = inverse_sum(sum, first < last);
         T* out = (T*)a.out + (long long)(q0 + tr) * a.ots + (long long)(h * a.group + gr) * a.ohs + c;
 #pragma unroll
         for (int i = 0; i < DT; ++i) {
@@ -717,7 +718,10 @@ __global__ __launch_bounds__(256) void attend_join_kernel(PackedArgs a) {
     float sum = ml[1] * f;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) sum += __shfl_xor(sum, o);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int tr = a.by_group(place.row0 + r), gr = place.row0 + r - tr * a.group;
+    int first, last;
+    seen(a, tr + place.nk - place.nq, place.nk, first, last);
+    const float inv = inverse_sum(sum, first < last);
     fw acc;
 #pragma unroll
     for (int i = 0; i < W; ++i) acc[i] = 0.f;
@@ -737,7 +741,6 @@ __global__ __launch_bounds__(256) void attend_join_kernel(PackedArgs a) {
         float y = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) y += part[i][threadIdx.x];
-        const int tr = a.by_group(place.row0 + r), gr = place.row0 + r - tr * a.group;
         ((T*)a.out)[(long long)(place.q0 + tr) * a.ots + (long long)(h * a.group + gr) * a.ohs + threadIdx.x] = (T)y;
     }
 }

@@ -735,10 +735,10 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
 #pragma unroll
                     for (int i = 0; i < W; ++i) acc[i] += so[w][row][d + i] * f;
                 }
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                const int t = m / a.group, g = m - t * a.group;
+                const float inv = inverse_sum(sum, len - a.tokens + t + 1 > 0);
 #pragma unroll
                 for (int i = 0; i < W; ++i) acc[i] *= inv;
-                const int t = m / a.group, g = m - t * a.group;
                 store_n<W, T>((T*)a.out + (((size_t)r * a.tokens + t) * a.heads + h * a.group + g) * D + d, acc);
                 if (COUNT && (threadIdx.x & 15) == 0) a.final_ml[(size_t)rh * a.m_rows + m] = f32x2{top, sum};
             }
@@ -755,7 +755,7 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
             const int m = nm * 16 + col;
             if (m < a.m_rows && piece_of == 0) {
                 if ((!whole || COUNT) && kq == 0) a.part_ml[piece * a.m_rows + m] = f32x2{mx[nm], l[nm]};
-                const float inv = l[nm] == 0.f ? 0.f : 1.f / l[nm];
+                const float inv = inverse_sum(l[nm], vis[nm] > 0);
                 const int t = m / a.group, g0 = m - t * a.group;
                 T* out = (T*)a.out + (((size_t)r * a.tokens + t) * a.heads + h * a.group + g0) * D + 8 * kq;
                 float* part = a.part_o + (piece * a.m_rows + m) * D + 8 * kq;
@@ -1086,7 +1086,7 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_ker
         if (m >= a.m_rows) continue;
         if (kq == 0) a.part_ml[piece * a.m_rows + m] = f32x2{mx[nm], l[nm]};
         const bool whole = used == 1;
-        const float inv = whole ? (l[nm] == 0.f ? 0.f : 1.f / l[nm]) : 1.f;
+        const float inv = whole ? inverse_sum(l[nm], vis[nm] > 0) : 1.f;
         const int t = m / a.group, g0 = m - t * a.group;
         T* out = (T*)a.out + (((size_t)r * a.tokens + t) * a.heads + h * a.group + g0) * D + 8 * kq;
         float* part = a.part_o + (piece * a.m_rows + m) * D + 8 * kq;
@@ -1139,7 +1139,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttendArgs a) {
         const f32x2 all = join_ml(a, p, m);
         if (a.final_ml && threadIdx.x == 0) a.final_ml[blockIdx.x] = all;
         if (p.x == p.y) return;
-        const float inv = all[1] == 0.f ? 0.f : 1.f / all[1];
+        const float inv = inverse_sum(all[1], row_length(c, r) - a.tokens + m / a.group + 1 > 0);
 #pragma unroll 4
         for (int s = p.x + group; s <= p.y; s += 16) {
             const size_t at = (size_t)s * a.m_rows + m;
@@ -1170,15 +1170,20 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(AttendArgs a, int slot
     const f32x2* ml = a.final_ml + (size_t)rh * a.m_rows;
     const float* scores = a.scores + (size_t)rh * a.m_rows * c.capacity + s;
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    int sees = len - a.tokens + 1, g = 0;  // slots that query m sees
 #pragma unroll 8
     for (int m = 0; m < a.m_rows; ++m) {
         const f32x4 x = *reinterpret_cast<const f32x4*>(scores + (size_t)m * c.capacity);
-        const float top = ml[m][0], off = top == -INFINITY ? 0.f : top, inv = ml[m][1] == 0.f ? 0.f : 1.f / ml[m][1];
+        const float top = ml[m][0], off = top == -INFINITY ? 0.f : top, inv = inverse_sum(ml[m][1], sees > 0);
         const bool far = fabsf(off) > kFarTop;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {  // (rounded as where they were summed up: the probabilities add up to 1)
             const float y = far ? scaled_below(x[i], a.scale2, off) : fmaf(x[i], a.scale2, -off);
-            sum[i] += y == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(y) * inv;
+            sum[i] += s + i < sees ? __builtin_amdgcn_exp2f(y) * inv : 0.f;
+        }
+        if (++g == a.group) {
+            g = 0;
+            ++sees;
         }
     }
     float* w = c.weights + (size_t)rh * c.capacity + s;
@@ -1232,8 +1237,8 @@ __global__ __launch_bounds__(256, TYPE == AFTER_T_F32 ? 1 : 2) void kv4_wide_wei
                 const float top = __shfl(ml[0], m), sum = __shfl(ml[1], m);
                 off[nm][i] = top == -INFINITY ? 0.f : top;
                 far |= fabsf(off[nm][i]) > kFarTop;
-                inv[nm][i] = sum == 0.f ? 0.f : 1.f / sum;
                 sees[nm][i] = __shfl(vis[nm], 4 * kq + i);
+                inv[nm][i] = inverse_sum(sum, sees[nm][i] > 0);
             }
         far = __any(far);
         const int all_see = m0 + 32 <= a.m_rows ? len - a.tokens + m0 / a.group + 1 : 0;

@@ -578,7 +578,8 @@ long long after_conv1_act_launches(void);
  * ascending; entries outside [0, rows] are taken as the nearest of them).  The queries are the newest of their sequence's
  * keys: query i of n stands at p = i + (keys - n).  causal: it sees the keys of its own chunk of `chunk` tokens and all chunks
  * before (chunk = 1: the keys up to its own), and with window > 0 of the earlier chunks only keys > p - window, as DenoiserV2's
- * mask does (transformerv2.py:62-96).  causal = 0: all keys.  A query that sees no key gets zeros; what a query does not see
+ * mask does (transformerv2.py:62-96).  causal = 0: all keys.  A query that sees no key gets zeros, one that sees only scores of
+ * -infinity NaN; what a query does not see
  * has no effect on it, NaN and infinities included.  Rows of out behind the last sequence stay as they are, or are set to
  * zero with zero_rest.  D = 64 or 128.  fp32: fp32 products; bf16 / fp16: products of that type, sums and softmax in fp32: a
  * probability is rounded to the type before it is multiplied (fp16: what is below 2^-32 of a query's largest counts as 0).
@@ -645,7 +646,8 @@ int after_kv4_truncate(const after_kv4* c, const int* lengths, void* stream);
  * zeros past a row's length. */
 int after_kv4_read(const after_kv4* c, void* k, void* v, int type, const int* start, int count, void* stream);
 /* out [rows, tokens, heads, D] (contiguous, of q's type): attention of the newest `tokens` tokens of each row, whose keys are
- * in the cache already: query t sees the slots below lengths[r] - tokens + t + 1, none of them: zeros.  (A row with fewer new
+ * in the cache already: query t sees the slots below lengths[r] - tokens + t + 1, none of them: zeros; all scores -infinity: NaN,
+ * in the output and in the weights of the slots that it sees.  (A row with fewer new
  * tokens than others has its queries at the end.)  accumulate: weights = decay * weights + the probabilities that each slot
  * in use received, summed over tokens and the group's heads (decay = 0: they are replaced).  Sums are divided at the end: they
  * stay finite while the largest value times the slots that a query sees is below 2^120.  The workspace is scratch: its

@@ -177,3 +177,51 @@ def test_small_probabilities_in_wide_tiles(hip_device):
     rest = (n - 1) * math.exp(-float(k[0, 0, 0]))
     want = torch.full(out.shape, 100 * rest / (1 + rest), dtype=torch.float64)
     close(out, want, 100 * n * 2.0 ** -32 + want * (2 * n * 2.0 ** -24 + 2.0 ** -11) + 2.0 ** -25)  # (sums of n terms, above and below the line)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompts_whose_scores_are_all_minus_infinity(hip_device, kind, form, dim):
+    """A softmax of nothing but -inf is NaN; one of -inf and a number is the number's; a query without keys gets zeros."""
+    t, g = TYPES[kind], gen(8)
+    q, k, v = (torch.randn(n, 2, dim, generator=g).to(hip_device, t) for n in (130, 128, 128))
+    q[:, 0, 3], k[:100, 0, 3], k[100:, 0, 3] = q[:, 0, 3].abs() + 1, -math.inf, -1.0
+    out = packed(form, q, k, v, [130], [128])
+    assert (out[:2] == 0).all() and torch.isnan(out[2:102, 0]).all() and not torch.isnan(out[102:, 0]).any() and not torch.isnan(out[:, 1]).any()
+    at = [102, 115, 129]
+    for i in at:
+        check_packed(out[i:i + 1, :1], q[i:i + 1, :1], k[100:i - 1, :1], v[100:i - 1, :1], [1], [i - 101], dim ** -0.5)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_shares_of_the_keys_with_scores_of_minus_infinity(hip_device, kind):
+    g = gen(9)
+    q, k, v = (torch.randn(n, 2, 64, generator=g).to(hip_device, TYPES[kind]) for n in (1, 9000, 9000))
+    q[:, :, 3], k[:, 0, 3] = 1.0, -math.inf
+    k[:8000, 1, 3] = -math.inf
+    out = attend_packed(q, k, v, starts([1], hip_device), starts([9000], hip_device))
+    assert torch.isnan(out[:, 0]).all()
+    check_packed(out[:, 1:], q[:, 1:], k[8000:, 1:], v[8000:, 1:], [1], [1000], 0.125)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("T, capacity", [(3, 128), (3, 640), (24, 640)])
+def test_cached_scores_that_are_all_minus_infinity(hip_device, kind, dim, T, capacity):
+    lens, g = [70, 2, 0, 600 if capacity > 600 else 100], gen(10)
+    c = KVCache4(4, 2, dim, capacity, hip_device)
+    k, v = (torch.randn(sum(lens), 2, dim, generator=g).to(hip_device) for _ in range(2))
+    k[:, 0, 3] = 4.0
+    c.append(k, v, starts(lens, hip_device))
+    q = torch.randn(4, T, 4, dim, generator=g).to(hip_device, TYPES[kind])
+    q[:, -1, 1, 3] = -math.inf  # the last token of the second head of key head 0
+    good = c.attend(torch.where(torch.isinf(q), 0, q))
+    before = c.weights.clone()
+    out = c.attend(q, accumulate=True)
+    for r, n in enumerate(lens):
+        assert torch.isnan(out[r, -1, 1]).all() if n else (out[r, -1, 1] == 0).all()
+        keep = torch.ones(T, 4, dtype=torch.bool)
+        keep[-1, 1] = False
+        assert torch.equal(out[r][keep], good[r][keep])
+        assert torch.isnan(c.weights[r, 0, :n]).all() and not torch.isnan(c.weights[r, 1]).any() and torch.equal(c.weights[r, :, n:], before[r, :, n:])
