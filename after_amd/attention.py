@@ -85,8 +85,8 @@ def _share(a, b):
 
 def _scale(scale, dim):
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    if not abs(scale) < 3e38:
-        raise ValueError(f"scale must be finite in 32 bits, got {scale}")
+    if not abs(scale) < 2.35e38:  # (log2 e times as much is the kernels' factor)
+        raise ValueError(f"scale must be within 2.35e38, got {scale}")
     return scale
 
 

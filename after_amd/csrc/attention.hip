@@ -830,7 +830,7 @@ extern "C" int after_attend_packed(const after_packed* call, void* stream) {
     const after_packed& c = *call;
     AFTER_TRY(check_sizes(c.type, c.q_rows, c.k_rows, c.n_seqs, c.heads, c.kv_heads, c.head_dim, c.window));
     const int group = c.heads / c.kv_heads;
-    AFTER_REQUIRE(std::isfinite(c.scale), AFTER_E_INVALID, "attend_packed: scale must be finite");
+    AFTER_REQUIRE(std::isfinite(scale_log2(c.scale)) && !std::isnan(c.scale), AFTER_E_INVALID, "attend_packed: scale must be finite, times log2 e too");
     AFTER_REQUIRE(c.window >= 0 && c.chunk >= 1 && c.chunk <= (1 << 24) && (c.causal || (c.window == 0 && c.chunk == 1)), AFTER_E_INVALID,
                   "attend_packed: window >= 0 (0: none) and chunk >= 1, both for causal attention only");
     if (c.q_rows == 0) return AFTER_OK;
@@ -852,7 +852,7 @@ extern "C" int after_attend_packed(const after_packed* call, void* stream) {
     if (!c.workspace) p.splits = 1;
     a.tiles = p.tiles, a.splits = p.splits, a.by_splits = divisor(p.splits);
     a.part_ml = (f32x2*)c.workspace, a.part_o = (float*)((char*)c.workspace + p.ml_bytes);
-    a.scale2 = std::fmax(std::fabs(c.scale) * 1.44269504088896340736f, 1e-30f);
+    a.scale2 = scale_log2(c.scale);
     a.q_sign = c.scale < 0 ? (c.type == AFTER_T_F32 ? 0x80000000u : 0x80008000u) : 0u;
     a.causal = c.causal != 0, a.window = c.window < (1 << 30) ? c.window : 1 << 30, a.zero_rest = c.zero_rest;
     a.by_group = divisor(group), a.by_chunk = divisor(c.chunk), a.by_kv_heads = divisor(c.kv_heads);

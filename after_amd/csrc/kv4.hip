@@ -1700,7 +1700,8 @@ extern "C" int after_kv4_attend(const after_kv4* c, const after_kv4_query* query
     const int per16 = 16 / type_bytes(x.type);
     AFTER_REQUIRE(x.q && x.out && aligned16(x.q) && aligned16(x.out) && x.q_row_stride % per16 == 0 && x.q_token_stride % per16 == 0 && x.q_head_stride % per16 == 0,
                   AFTER_E_INVALID, "kv4_attend: q, its strides and out must be 16-byte aligned");
-    AFTER_REQUIRE(std::isfinite(x.scale) && std::isfinite(x.decay), AFTER_E_INVALID, "kv4_attend: scale and decay must be finite");
+    AFTER_REQUIRE(std::isfinite(scale_log2(x.scale)) && !std::isnan(x.scale) && std::isfinite(x.decay), AFTER_E_INVALID,
+                  "kv4_attend: scale (times log2 e too) and decay must be finite");
     const bool count = x.accumulate != 0;
     const Plan p = attend_plan(*c, x.type, x.heads, x.tokens, count);
     const long long need = p.total();
@@ -1718,7 +1719,7 @@ extern "C" int after_kv4_attend(const after_kv4* c, const after_kv4_query* query
     a.group = x.heads / c->kv_heads;
     a.m_rows = p.m_rows;
     a.workers = 4 * p.wgs;
-    a.scale2 = std::fmax(std::fabs(x.scale) * 1.44269504088896340736f, 1e-30f);
+    a.scale2 = scale_log2(x.scale);
     a.q_sign = x.scale < 0 ? -1.f : 1.f;
     char* w = (char*)x.workspace;
     a.scores = (float*)w;

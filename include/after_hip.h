@@ -584,6 +584,7 @@ long long after_conv1_act_launches(void);
  * zero with zero_rest.  D = 64 or 128.  fp32: fp32 products; bf16 / fp16: products of that type, sums and softmax in fp32: a
  * probability is rounded to the type before it is multiplied (fp16: what is below 2^-32 of a query's largest counts as 0).
  * Sums are divided at the end: they stay finite while the largest value times the keys that a query sees is below 2^120.
+ * scale: any sign, 0 too, up to 2.35e38 (here and in after_kv4_attend).
  * workspace: scratch of the size that _workspace names (its answer depends on the arguments alone; two calls that may run at the
  * same time need two), with which the keys of a few queries are shared out over the chip; NULL: they are not. */
 int after_attend_packed_workspace(int type, long long q_rows, long long k_rows, int n_seqs, int heads, int kv_heads, int head_dim,

@@ -225,3 +225,58 @@ def test_cached_scores_that_are_all_minus_infinity(hip_device, kind, dim, T, cap
         keep[-1, 1] = False
         assert torch.equal(out[r][keep], good[r][keep])
         assert torch.isnan(c.weights[r, 0, :n]).all() and not torch.isnan(c.weights[r, 1]).any() and torch.equal(c.weights[r, :, n:], before[r, :, n:])
+
+
+# ---------------------------------------------------------------------------------------------------------------- scales
+SCALES = [0.0, -0.2, 1e-42, 2e-38, -3e-36, 2.3e38]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("scale", SCALES)
+def test_prompts_with_any_scale(hip_device, kind, form, scale):
+    t, g = TYPES[kind], gen(11)
+    q, k, v = (torch.randn(n, h, 64, generator=g).to(hip_device, t) for n, h in ((70, 4), (90, 2), (90, 2)))
+    if 1e-40 < abs(scale) < 1e-30 and kind != "fp16":  # scores of some size all the same
+        up = min(0.1 / abs(scale), 2e35) ** 0.5
+        q, k = q * up, k * up
+    if scale > 1e30:
+        q, k = q * 0 + 2.0 ** -14, k * 2.0 ** (-10 if kind == "fp16" else -105)
+        q = q if kind == "fp16" else q * 2.0 ** -4
+    if kind == "fp16" and scale > 1e30:
+        k = torch.where(torch.arange(90, device=hip_device).view(90, 1, 1) % 7 == 3, 0, -k.abs())  # (scores 0 and far below)
+    out = packed(form, q, k, v, [70], [90], scale=scale)
+    check_packed(out, -q if scale < 0 else q, k, v, [70], [90], abs(scale))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("T, capacity", [(2, 64), (2, 640), (24, 640)])
+@pytest.mark.parametrize("scale", SCALES)
+def test_cached_keys_with_any_scale(hip_device, kind, T, capacity, scale):
+    t, g = TYPES[kind], gen(12)
+    k, v = (torch.randn(2, 60, 2, 64, generator=g).to(hip_device) for _ in range(2))
+    up = 1.0
+    if 1e-40 < abs(scale) < 1e-30:
+        up = min(0.1 / abs(scale), 2e35)
+    if scale > 1e30:
+        up = 2.0 ** -100
+    k *= up if kind == "fp16" else up ** 0.5
+    c = KVCache4(2, 2, 64, capacity, hip_device)
+    c.append(k, v)
+    q = torch.randn(2, T, 4, 64, generator=g).to(hip_device) * (1.0 if kind == "fp16" else up ** 0.5)
+    if scale > 1e30:
+        q = q * 2.0 ** (-13 if kind == "fp16" else -27)
+    q = q.to(t)
+    before = c.weights.clone()
+    out = c.attend(q, scale=scale, accumulate=True)
+    check_attend(c, -q if scale < 0 else q, [60, 60], out, abs(scale), c.weights, before)
+
+
+def test_scales_that_32_bits_do_not_hold_are_refused(hip_device):
+    c = filled(hip_device, 1, 1, 64, 64, [40], 16)
+    q = torch.zeros(1, 1, 1, 64, device=hip_device)
+    for scale in (2.4e38, -2.4e38, math.inf, math.nan, 1e300):
+        with pytest.raises(ValueError, match="scale"):
+            c.attend(q, scale=scale)
+        with pytest.raises(ValueError, match="scale"):
+            attend_packed(q[0], q[0], q[0], starts([1], hip_device), scale=scale)
