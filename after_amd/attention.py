@@ -1,6 +1,7 @@
 """Attention over sequences of different lengths: of whole prompts (`attend_packed`), and over a key / value cache that is held
 in four bits (`KVCache4`), next to the attention and the streaming K/V caches inside `DenoiserV2`
-(after/diffusion/networks/transformerv2.py:62-235).  fp32, bf16 and fp16 tensors; inference only, like the rest of the package;
+(after/diffusion/networks/transformerv2.py:62-235).  fp32, bf16 and fp16 tensors; inference only, like the rest of the package
+(a tensor that requires a gradient or carries a tangent is refused);
 hand-written HIP kernels behind the C ABI of include/after_hip.h, no fallback.
 
     cache = KVCache4(rows=4, kv_heads=8, head_dim=128, capacity=16384)
@@ -19,10 +20,18 @@ import math
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _refuse_gradients(t, name):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(f"{name} requires a gradient: after_amd is inference only (use torch.no_grad())")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:  # (outside of any level a look costs nothing)
+        raise NotImplementedError(f"{name} carries a tangent: after_amd is inference only")
 
 
 def _operand(t, name, dims, index=None, dtype=None):
@@ -41,8 +50,7 @@ def _operand(t, name, dims, index=None, dtype=None):
         raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
     if dtype is not None and kind is not dtype:
         raise TypeError(f"{name} is {kind}, expected {dtype}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise NotImplementedError(f"{name} requires a gradient: after_amd is inference only (use torch.no_grad())")
+    _refuse_gradients(t, name)
     odd = strides[0] | strides[1] | (strides[2] if dims == 4 else 0) | t.data_ptr() // t.element_size()
     # (a token's place in a tile is addressed with 32 bits; what the strides of an empty tensor are does not matter)
     if odd & (3 if kind is torch.float32 else 7) or strides[-1] != 1 or strides[-3] >= 1 << 22:
@@ -137,10 +145,10 @@ def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=True, window=None,
     elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != dtype or out.device != q.device \
             or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f"out must be a contiguous, 16-byte aligned {dtype} tensor {tuple(q.shape)} on {q.device}")
-    elif out.requires_grad and torch.is_grad_enabled():
-        raise NotImplementedError("out requires a gradient: after_amd is inference only (use torch.no_grad())")
-    elif _share([out], [k, v] if out.data_ptr() == q.data_ptr() and q.is_contiguous() else [q, k, v]):
-        raise ValueError("out shares memory with q, k or v (it may be q itself, if that is contiguous)")
+    else:
+        _refuse_gradients(out, "out")
+        if _share([out], [k, v] if out.data_ptr() == q.data_ptr() and q.is_contiguous() else [q, k, v]):
+            raise ValueError("out shares memory with q, k or v (it may be q itself, if that is contiguous)")
     window, kind = min(window or 0, 1 << 30), _TYPES[dtype]
     size = _packed_workspace(kind, n, keys, seqs, heads, kv_heads, dim, window)
     work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None  # (as in KVCache4.attend)

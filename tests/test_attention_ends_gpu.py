@@ -280,3 +280,22 @@ def test_scales_that_32_bits_do_not_hold_are_refused(hip_device):
             c.attend(q, scale=scale)
         with pytest.raises(ValueError, match="scale"):
             attend_packed(q[0], q[0], q[0], starts([1], hip_device), scale=scale)
+
+
+# ---------------------------------------------------------------------------------------------------------------- tangents
+def test_forward_mode_tangents_are_refused(hip_device):
+    import torch.autograd.forward_ad as fwd
+    x = torch.randn(4, 2, 64, generator=gen(19)).to(hip_device)
+    s, c = starts([4], hip_device), filled(hip_device, 1, 2, 64, 32, [10], 20)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for a in ((dual, x, x), (x, dual, x), (x, x, dual)):
+            with pytest.raises(NotImplementedError, match="tangent"):
+                attend_packed(*a, s)
+        with pytest.raises(NotImplementedError, match="tangent"):
+            attend_packed(x, x, x, s, out=dual)
+        with pytest.raises(NotImplementedError, match="tangent"):
+            c.attend(dual[None])
+        with pytest.raises(NotImplementedError, match="tangent"):
+            c.append(x, dual, s)
+        assert torch.equal(attend_packed(x, x, x, s), attend_packed(fwd.unpack_dual(dual).primal, x, x, s))
