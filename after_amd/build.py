@@ -75,9 +75,9 @@ def build_library(force=False, verbose=False):
     os.makedirs(LIBDIR, exist_ok=True)
     hipcc = _hipcc()
     ver = check_hipcc_version(hipcc)
-    # objects of another compiler must not survive an mtime check: the version that built them is recorded
-    stamp = os.path.join(LIBDIR, "hipcc_version.txt")
-    if os.path.exists(stamp) and open(stamp).read().strip() != ver:
+    # objects of another compiler or of other flags must not survive an mtime check: what built them is recorded
+    stamp, made_by = os.path.join(LIBDIR, "hipcc_version.txt"), ver + "\n" + " ".join(FLAGS) + "\n"
+    if not os.path.exists(stamp) or open(stamp).read() != made_by:
         force = True
     srcs = sources()
     hmt = _deps_mtime()
@@ -97,9 +97,7 @@ def build_library(force=False, verbose=False):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
-        open(stamp, "w").write(ver + "\n")
-    elif not os.path.exists(stamp):
-        open(stamp, "w").write(ver + "\n")
+        open(stamp, "w").write(made_by)
     return LIB
 
 
