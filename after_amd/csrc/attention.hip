@@ -809,7 +809,7 @@ static int check_sizes(int type, long long q_rows, long long k_rows, int n_seqs,
     AFTER_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, AFTER_E_INVALID, "attend_packed: heads must be a multiple of kv_heads (got %d, %d)", heads,
                   kv_heads);
     AFTER_REQUIRE(head_dim == 64 || head_dim == 128, AFTER_E_INVALID, "attend_packed: head_dim 64 or 128 (got %d)", head_dim);
-    AFTER_REQUIRE(n_seqs >= 0 && n_seqs <= (1 << 24) && q_rows >= 0 && k_rows >= 0 && k_rows < (1ll << 30), AFTER_E_INVALID,
+    AFTER_REQUIRE(n_seqs >= 0 && n_seqs <= (1 << 24) && q_rows >= 0 && q_rows < (1ll << 30) && k_rows >= 0 && k_rows < (1ll << 30), AFTER_E_INVALID,
                   "attend_packed: 0 <= n_seqs <= 2^24, 0 <= rows < 2^30");
     AFTER_REQUIRE(q_rows * (heads / kv_heads) < (1ll << 30), AFTER_E_INVALID, "attend_packed: q_rows x heads / kv_heads must stay below 2^30");
     const PackedPlan p = packed_plan(type, q_rows, k_rows, n_seqs, heads, kv_heads, head_dim, window);
