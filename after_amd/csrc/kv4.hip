@@ -1521,11 +1521,17 @@ Plan attend_plan(const after_kv4& c, int type, int heads, int tokens, bool count
         p.splits = (int)(wanted < tiles ? wanted : tiles);
     } else if (c.capacity > 512) {
         // Workers for two workgroups on each of 256 CUs, for three where the queries' registers leave room and there are many rows
-        // (with few, more pieces are a longer join).  D = 128, with the join: 64 rows of 1 .. 8192 x 8 heads, bf16 75.6 us against
-        // 78.3 with two, fp16 76.3 / 82.0, fp32 81.4 / 87.2 (without pieces in columns 81.7 and 88.2); 8 rows of 1 .. 32767, bf16
-        // 45.2 / 45.7; two rows of 131071, bf16 71.6 / 68.4, fp16 72.1 / 69.0; one of 32768 26.9 / 23.6.
+        // (with few, more pieces are a longer join), for one where two do not fit a CU.  Up to 16 queries of a row and head, D = 128,
+        // with the join: 64 rows of 1 .. 8192 x 8 heads, bf16 75.6 us against 78.3 with two, fp16 76.3 / 82.0, fp32 81.4 / 87.2
+        // (without pieces in columns 81.7 and 88.2); 8 rows of 1 .. 32767, bf16 45.2 / 45.7; two rows of 131071, bf16 71.6 / 68.4,
+        // fp16 72.1 / 69.0; one of 32768 26.9 / 23.6.  24 queries, D = 128, calls one behind the other on the same cache: bf16 (two
+        // fit) 8 rows of 1 .. 32767 59.3 us against 67.7 with three, 32 of 1 .. 8192 56.6 / 65.4, 64 of 4096 86.6 / 106.8, but 64 of
+        // 1 .. 8192 126.4 / 110.3; fp16 and fp32 (one fits) 8 rows 87.6 and 110.2 against 99.1 and 121.5 with two, 64 rows of
+        // 1 .. 8192 181.8 and 209.3 / 185.3 and 214.9.
         // Rows of at most 512 slots take a workgroup each and one launch: 6.2 us against 9.
-        const int full = n_rh >= 64 && (attend_cols(type, p.m_rows) < 16 || type == AFTER_T_BF16) ? 768 : 512;
+        const int full = p.nm == 2 ? (type != AFTER_T_BF16 && c.head_dim == 128 ? 256 : 512)
+                         : n_rh >= 64 && (attend_cols(type, p.m_rows) < 16 || type == AFTER_T_BF16) ? 768
+                                                                                                    : 512;
         p.wgs = (int)(most < full ? most : full);
     }
     p.pieces = p.splits ? n_rh * p.splits : 4ll * p.wgs + n_rh;
