@@ -79,7 +79,7 @@ struct PackedArgs {
     void* out;
     const int *qs, *ks;
     long long qts, qhs, kts, khs, vts, vhs, ots, ohs;
-    int q_rows, k_rows, n_seqs, heads, kv_heads, group, tiles, splits;
+    int q_rows, k_rows, n_seqs, kv_heads, group, tiles, splits;
     Divisor by_group, by_chunk, by_kv_heads, by_splits;
     float scale2;     // |scale| log2 e, > 0 (a masked score, -inf, stays -inf)
     unsigned q_sign;  // the sign bits of a word of q, if scale is negative
@@ -845,7 +845,7 @@ extern "C" int after_attend_packed(const after_packed* call, void* stream) {
     a.q = c.q, a.k = c.k, a.v = c.v, a.out = c.out, a.qs = c.q_starts, a.ks = c.k_starts;
     a.qts = c.q_token_stride, a.qhs = c.q_head_stride, a.kts = c.k_token_stride, a.khs = c.k_head_stride;
     a.vts = c.v_token_stride, a.vhs = c.v_head_stride, a.ots = c.out_token_stride, a.ohs = c.out_head_stride;
-    a.q_rows = (int)c.q_rows, a.k_rows = (int)c.k_rows, a.n_seqs = c.n_seqs, a.heads = c.heads, a.kv_heads = c.kv_heads, a.group = group;
+    a.q_rows = (int)c.q_rows, a.k_rows = (int)c.k_rows, a.n_seqs = c.n_seqs, a.kv_heads = c.kv_heads, a.group = group;
     PackedPlan p = packed_plan(c.type, c.q_rows, c.k_rows, c.n_seqs, c.heads, c.kv_heads, c.head_dim, c.window);
     AFTER_REQUIRE(!c.workspace || (((size_t)c.workspace & 15) == 0 && c.workspace_bytes >= p.bytes), AFTER_E_CAPACITY,
                   "attend_packed: a workspace has to be 16-byte aligned, here of %lld bytes (got %lld)", p.bytes, c.workspace_bytes);
