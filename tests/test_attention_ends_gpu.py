@@ -282,6 +282,73 @@ def test_scales_that_32_bits_do_not_hold_are_refused(hip_device):
             attend_packed(q[0], q[0], q[0], starts([1], hip_device), scale=scale)
 
 
+# ---------------------------------------------------------------------------------------------------------------- many
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("heads, kv, tokens, lens, capacity", [
+    (3, 1, 43, [200, 40, 3], 256),           # 129 queries of a row and head: one more than a workgroup serves
+    (2, 1, 150, [149, 0, 700, 20], 704),     # 300
+    (4, 2, 150, [151, 64], 1024),
+    (3, 1, 86, [85], 128)])                  # 258: a last workgroup of two
+def test_more_queries_than_a_workgroup_serves(hip_device, kind, heads, kv, tokens, lens, capacity):
+    c = filled(hip_device, len(lens), kv, 64, capacity, lens, seed=tokens)
+    q = torch.randn(len(lens), tokens, heads, 64, generator=gen(17)).to(hip_device, TYPES[kind])
+    before = torch.rand(c.weights.shape, generator=gen(18)).to(hip_device)
+    c.weights.copy_(before)
+    out = c.attend(q, accumulate=True, decay=0.5)
+    check_attend(c, q, lens, out, 0.125, c.weights, before, 0.5)
+    assert torch.equal(c.attend(q), out)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rows", [70, 150])
+@pytest.mark.parametrize("capacity", [96, 544])
+def test_more_rows_than_lanes(hip_device, kind, rows, capacity):
+    """Rows are searched 64 at a time, in the append of many tokens and in both forms of attention; some rows are empty."""
+    g, t = gen(rows), TYPES[kind]
+    lens = torch.randint(0, 70, (rows, ), generator=g)
+    lens[torch.rand(rows, generator=g) < 0.2] = 0
+    lens[64:67] = torch.tensor([0, 69, 0])
+    lens = lens.tolist()
+    c = KVCache4(rows, 2, 64, capacity, hip_device)
+    k, v = (torch.randn(sum(lens), 2, 64, generator=g).to(hip_device, t) for _ in range(2))
+    c.append(k, v, starts(lens, hip_device))
+    assert c.lengths.tolist() == lens
+    codes, at = [ref.round4(x.transpose(0, 1)) for x in (k, v)], 0
+    for r, n in enumerate(lens):
+        for (code, byte), got, scales in zip(codes, (ref.key_codes(c.keys[r:r + 1]), ref.value_codes(c.values[r:r + 1])), (c.key_scales, c.value_scales)):
+            assert torch.equal(got[0, :, :n], code[:, at:at + n]) and torch.equal(scales[r, :, :n].cpu(), byte[:, at:at + n])
+        at += n
+    for tokens in (1, 20):
+        q = torch.randn(rows, tokens, 4, 64, generator=g).to(hip_device, t)
+        before = c.weights.clone()
+        out = c.attend(q, accumulate=True)
+        check_attend(c, q, lens, out, 0.125, c.weights, before)
+    small = KVCache4(rows, 2, 64, 32, hip_device)
+    slots, w = c.evict(small, 20, 3), c.weights.cpu()
+    for r, n in enumerate(lens):
+        for h in range(2):
+            want = ref.evict(w[r, h], n, 20, 3)
+            assert slots[r, h].tolist() == want + [-1] * (20 - len(want))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_repeats_are_equal(hip_device, kind):
+    """Every form of the two operators, three times: the same bits."""
+    t = TYPES[kind]
+    c = filled(hip_device, 5, 2, 128, 4096, [4000, 17, 2500, 1, 0], 62)
+    for T in (1, 4, 24):
+        q = torch.randn(5, T, 8, 128, generator=gen(T)).to(hip_device, t)
+        want, w = c.attend(q, accumulate=True, decay=0.0), c.weights.clone()
+        for _ in range(2):
+            assert torch.equal(c.attend(q, accumulate=True, decay=0.0), want) and torch.equal(c.weights, w)
+    for qs, ks in (([1], [9000]), ([300, 7], None), ([40] * 300, None)):
+        ks = ks or qs
+        q, k, v = (torch.randn(n, h, 128, generator=gen(h)).to(hip_device, t) for n, h in ((sum(qs), 4), (sum(ks), 2), (sum(ks), 2)))
+        want = attend_packed(q, k, v, starts(qs, hip_device), starts(ks, hip_device))
+        for _ in range(2):
+            assert torch.equal(attend_packed(q, k, v, starts(qs, hip_device), starts(ks, hip_device)), want)
+
+
 # ---------------------------------------------------------------------------------------------------------------- tangents
 def test_forward_mode_tangents_are_refused(hip_device):
     import torch.autograd.forward_ad as fwd
