@@ -360,6 +360,22 @@ __device__ __forceinline__ void pieces8(const float (&x)[8], bf16x8 (&p)[N]) {
     }
 }
 
+// ... of queries, exactly: all pieces but the last are cut off, not rounded, since fp32's largest numbers would become infinities
+template <int N>
+__device__ __forceinline__ void query_pieces8(const float (&x)[8], bf16x8 (&p)[N]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float rest = x[i];
+#pragma unroll
+        for (int n = 0; n < N - 1; ++n) {
+            const unsigned u = __float_as_uint(rest) & 0xFFFF0000u;
+            p[n][i] = __builtin_bit_cast(__bf16, (unsigned short)(u >> 16));
+            rest -= __uint_as_float(u);
+        }
+        p[N - 1][i] = (__bf16)rest;
+    }
+}
+
 constexpr int kRing = 3;  // tiles of 32 tokens that each wave has in LDS
 constexpr float kLift = 66.f, kDrop = 0x1p-66f;  // probabilities are held 2^kLift times as large until they are weighed
 template <int D>
@@ -464,13 +480,13 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
             for (int i = 0; i < 8; ++i) y[i] *= a.q_sign;
             if constexpr (COLS < 16) {
                 bf16x8 z[PIECES];
-                pieces8<PIECES>(y, z);
+                query_pieces8<PIECES>(y, z);
                 qf[nm][s][0] = z[0];
 #pragma unroll
                 for (int q = 1; q < PIECES; ++q)
                     if (piece_of == q) qf[nm][s][0] = z[q];
             } else
-                pieces8<NP>(y, qf[nm][s]);
+                query_pieces8<NP>(y, qf[nm][s]);
         }
     }
     const int all_see = len - a.tokens + 1;  // slots below this are seen by every query
@@ -894,7 +910,7 @@ __device__ __forceinline__ void load_queries(const AttendArgs& a, int r, int h, 
             if (in) load_n<8, T>((const T*)a.q + r * a.qrs + t * a.qts + (long long)(h * a.group + g) * a.qhs + 32 * s + 8 * kq, y);
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] *= a.q_sign;
-            pieces8<NP>(y, qf[nm][s]);
+            query_pieces8<NP>(y, qf[nm][s]);
         }
     }
 }

@@ -272,6 +272,17 @@ def test_cached_keys_with_any_scale(hip_device, kind, T, capacity, scale):
     check_attend(c, -q if scale < 0 else q, [60, 60], out, abs(scale), c.weights, before)
 
 
+@pytest.mark.parametrize("T, capacity", [(1, 64), (1, 640), (9, 640), (20, 640), (40, 640)])
+def test_queries_next_to_the_largest_number(hip_device, T, capacity):
+    """fp32 queries beyond bf16's largest number, whose pieces they are cut into."""
+    g = gen(21)
+    c = KVCache4(1, 1, 64, capacity, hip_device)
+    c.append((torch.randn(1, 60, 1, 64, generator=g) * 2.0 ** -70).to(hip_device), torch.randn(1, 60, 1, 64, generator=g).to(hip_device))
+    q = torch.randn(1, T, 1, 64, generator=g).sign() * torch.finfo(torch.float32).max * (1 - 2.0 ** -10 * torch.rand(1, T, 1, 64, generator=g))
+    q = q.to(hip_device)
+    check_attend(c, q, [60], c.attend(q, scale=2.0 ** -59), 2.0 ** -59)
+
+
 def test_scales_that_32_bits_do_not_hold_are_refused(hip_device):
     c = filled(hip_device, 1, 1, 64, 64, [40], 16)
     q = torch.zeros(1, 1, 1, 64, device=hip_device)
