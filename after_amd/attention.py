@@ -116,7 +116,7 @@ def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=True, window=None,
 
     causal: a query sees the keys up to its own position; with `chunk` > 1 also the rest of its chunk, and with `window` only the
     newest `window` keys outside its chunk: the mask of DenoiserV2's local attention (transformerv2.py:62-96).  A query that
-    sees nothing gets zeros.  Rows behind the last sequence are zeros in a new tensor and left alone in `out`, which must be
+    sees nothing gets zeros.  Sums and softmax are fp32; bf16 and fp16 products take probabilities rounded to that type.  Rows behind the last sequence are zeros in a new tensor and left alone in `out`, which must be
     contiguous and must not overlap q, k or v; it may be q itself."""
     chunk, window = int(chunk), None if window is None else int(window)
     if not 1 <= chunk <= 1 << 24 or (window is not None and window < 1):
@@ -277,10 +277,12 @@ class KVCache4:
     def attend(self, q, scale=None, accumulate=False, decay=1.0):
         """Attention of the newest tokens of every row, q [rows, tokens, heads, head_dim], over the cached keys and values (their
         own have been appended): token t of T sees the slots below lengths - T + t + 1; one that sees none gets zeros.  A row
-        with fewer new tokens than T has its own at the end.  Returns [rows, tokens, heads, head_dim].
+        with fewer new tokens than T has its own at the end.  Returns [rows, tokens, heads, head_dim].  Sums and softmax are fp32;
+        a probability is multiplied in as many bf16 pieces as hold a number of q's type: for bf16 queries it is rounded to bf16.
 
         accumulate: `weights` = decay * weights + the probability that each slot received, summed over the tokens and the heads
-        of its group (decay = 0 replaces them)."""
+        of its group (decay = 0 replaces them).  Up to 32 queries of a row and key head keep their scores for that, in scratch of
+        4 bytes x queries x rows x kv_heads x capacity."""
         q = _operand(q, "q", 4, self._index)
         rows, tokens, heads, dim = q.shape
         if rows != self.rows or dim != self.head_dim or heads == 0 or heads % self.kv_heads:

@@ -650,9 +650,12 @@ int after_kv4_read(const after_kv4* c, void* k, void* v, int type, const int* st
  * in the cache already: query t sees the slots below lengths[r] - tokens + t + 1, none of them: zeros; all scores -infinity: NaN,
  * in the output and in the weights of the slots that it sees.  (A row with fewer new
  * tokens than others has its queries at the end.)  accumulate: weights = decay * weights + the probabilities that each slot
- * in use received, summed over tokens and the group's heads (decay = 0: they are replaced).  Sums are divided at the end: they
- * stay finite while the largest value times the slots that a query sees is below 2^120.  The workspace is scratch: its
- * size depends on the arguments alone, and two calls that may run at the same time need two. */
+ * in use received, summed over tokens and the group's heads (decay = 0: they are replaced).  Products are of bf16 numbers: cached
+ * keys and values are such; a query is cut into one (bf16), two (fp16) or three (fp32) of them, exactly, and a probability into as
+ * many, to within 2^-9, 2^-15 or 2^-23 of itself.  The softmax, its sums, the weights and the output before it is rounded are
+ * fp32.  Sums are divided at the end: they stay finite while the largest value times the slots that a query sees is below 2^120.
+ * The workspace is scratch: its size depends on the arguments alone (the cache's capacity, not its lengths: with accumulate and up
+ * to 32 queries of a row and head, 4 bytes for each of them and every slot), and two calls that may run at the same time need two. */
 int after_kv4_attend_workspace(const after_kv4* c, int type, int heads, int tokens, int accumulate, long long* bytes);
 typedef struct after_kv4_query {
     const void* q;
