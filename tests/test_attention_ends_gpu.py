@@ -360,6 +360,85 @@ def test_repeats_are_equal(hip_device, kind):
             assert torch.equal(attend_packed(q, k, v, starts(qs, hip_device), starts(ks, hip_device)), want)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("capacity", [32, 96, 544, 1056])
+def test_full_rows(hip_device, kind, dim, capacity):
+    """Every slot in use: the last tile ends with the buffers."""
+    g, t, lens = gen(22), TYPES[kind], [capacity, capacity - 1]
+    c = filled(hip_device, 2, 1, dim, capacity, lens, 23)
+    for T in (1, 12, 40):
+        q = torch.randn(2, T, 2, dim, generator=g).to(hip_device, t)
+        before = c.weights.clone()
+        check_attend(c, q, lens, c.attend(q, accumulate=True), dim ** -0.5, c.weights, before)
+
+
+def test_no_sequences(hip_device):
+    q, none = torch.randn(5, 2, 64, generator=gen(24)).to(hip_device), torch.zeros(1, dtype=torch.int32, device=hip_device)
+    assert torch.equal(attend_packed(q, q, q, none), torch.zeros_like(q))
+    kept = torch.full_like(q, 3.0)
+    assert (attend_packed(q, q, q, none, out=kept) == 3).all()
+
+
+# ---------------------------------------------------------------------------------------------------------------- graphs and streams
+@pytest.mark.parametrize("tokens", [3, 40])
+def test_a_captured_pass_replays(hip_device, tokens):
+    """Append, observe, evict and read in one graph, replayed with other tokens, counts and lengths: every replay as the eager run."""
+    R, H, KV, D, C, g = 3, 4, 2, 128, 1024, gen(25)
+    k, v, q = (torch.zeros(n, h, D, device=hip_device, dtype=torch.float16) for n, h in ((900, KV), (900, KV), (R * tokens, H)))
+    s, held = torch.zeros(R + 1, dtype=torch.int32, device=hip_device), torch.zeros(R, dtype=torch.int32, device=hip_device)
+
+    def run(big, small):
+        big.truncate(held)
+        big.append(k, v, s)
+        out = big.attend(q.view(R, tokens, H, D), accumulate=True, decay=0.5)
+        return [out, big.evict(small, 200, 8), *small.read(), *big.buffers().values(), *small.buffers().values()]
+
+    sets = [(KVCache4(R, KV, D, C, hip_device), KVCache4(R, KV, D, 256, hip_device)) for _ in range(2)]
+    run(*sets[0])  # (the first call of each kernel)
+    for x in (*sets[0][0].buffers().values(), *sets[0][1].buffers().values()):
+        x.zero_()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = run(*sets[0])
+    for turn, (lens, old) in enumerate((([300, 0, 500], [0, 0, 0]), ([1, 450, 30], [200, 0, 500]), ([0, 0, 700], [201, 7, 3]), ([250, 250, 250], [9, 9, 9]))):
+        for x in (k, v, q):
+            x.copy_(torch.randn(x.shape, generator=g))
+        s.copy_(starts(lens, hip_device))
+        held.copy_(torch.tensor(old, dtype=torch.int32))
+        graph.replay()
+        want = run(*sets[1])
+        torch.cuda.synchronize()
+        for i, (a, b) in enumerate(zip(got, want)):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), (turn, i)
+
+
+def test_two_streams_at_once(hip_device):
+    """Calls of both operators on two streams, each with a cache of its own: as one behind the other."""
+    g = gen(26)
+    k, v = (torch.randn(9000, 2, 128, generator=g).to(hip_device, torch.bfloat16) for _ in range(2))
+    q = torch.randn(2, 1, 8, 128, generator=g).to(hip_device, torch.bfloat16)
+    one, ks = starts([1, 1], hip_device), starts([6000, 3000], hip_device)
+    caches = [filled(hip_device, 2, 2, 128, 8192, [8000, 5000], 27 + i) for i in range(2)]
+
+    def run(c):
+        y = [attend_packed(q[:, 0], k, v, one, ks), c.attend(q, accumulate=True, decay=0.0), c.attend(q.expand(2, 9, 8, 128), accumulate=True)]
+        return y + [c.weights.clone()]
+
+    want = [run(c) for c in caches]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(3):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(run(caches[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for y in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(y, want[i]))
+
+
 # ---------------------------------------------------------------------------------------------------------------- tangents
 def test_forward_mode_tangents_are_refused(hip_device):
     import torch.autograd.forward_ad as fwd
