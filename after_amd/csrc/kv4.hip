@@ -377,7 +377,8 @@ __device__ __forceinline__ void query_pieces8(const float (&x)[8], bf16x8 (&p)[N
 }
 
 constexpr int kRing = 3;  // tiles of 32 tokens that each wave has in LDS
-constexpr float kLift = 66.f, kDrop = 0x1p-66f;  // probabilities are held 2^kLift times as large until they are weighed
+constexpr int kLift = 66;  // probabilities are taken 2^kLift times as large to be weighed
+constexpr float kLifted = 0x1p66f;
 template <int D>
 constexpr int kTileBytes = 32 * D + 2 * D;  // keys, values, key scales, value scales
 
@@ -498,7 +499,7 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
     for (int nm = 0; nm < NM; ++nm) {
         mx[nm] = limit[nm] = -INFINITY;
         l[nm] = 0.f;
-        off[nm] = -kLift, times[nm] = a.scale2;
+        off[nm] = 0.f, times[nm] = a.scale2;
 #pragma unroll
         for (int i = 0; i < 2 * G; ++i) o[nm][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -597,18 +598,17 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
                 }
             }
             // The maximum moves only when a score outgrows it by 2^2, so that most tiles need no exchange between lanes: a
-            // probability of up to 4 is as exact.  It is a whole number, so that probabilities can be held 2^kLift times as large
-            // (below) without another rounding.  Where it is beyond kFarTop, scores are brought down here in every tile: the usual
+            // probability of up to 4 is as exact.  Where it is beyond kFarTop, scores are brought down here in every tile: the usual
             // one has no branch for it.
             top *= a.scale2;
             if (__any(top > limit[nm])) {
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
-                const float now = rintf(fmaxf(mx[nm], top)), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[nm] - now);
+                const float now = fmaxf(mx[nm], top), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[nm] - now);
                 const float below = now == -INFINITY ? 0.f : now;
                 const bool far = __any(fabsf(below) > kFarTop);
                 mx[nm] = now;
-                off[nm] = (far ? 0.f : below) - kLift, times[nm] = far ? 1.f : a.scale2, limit[nm] = far ? -INFINITY : now + 2.f;
+                off[nm] = far ? 0.f : below, times[nm] = far ? 1.f : a.scale2, limit[nm] = far ? -INFINITY : now + 2.f;
                 l[nm] *= f;
 #pragma unroll
                 for (int i = 0; i < 2 * G; ++i) o[nm][i] = o[nm][i] * f;
@@ -626,7 +626,7 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
         // P times the scale of its token and group, as bf16 pieces.  The scale is a power of two: its exponent is added to the
         // probability's as an integer, two tokens at a time -- one v_perm_b32 for both bytes, one v_pk_mad_u16, and a maximum
         // with 0 for what falls below bf16's exponents (products below 2^-126 vanish): a third of the instructions of extracting
-        // eight scales per group and multiplying.  With p held 2^kLift times as large, a p of 0 stays below them under every
+        // eight scales per group and multiplying.  With p taken 2^kLift times as large, a p of 0 stays below them under every
         // scale less than 2^65; larger ones are multiplied.  Pieces are cut off, not rounded, so that none is negative; a single
         // one is rounded.
         u16x2 bits[NM][NP][4];
@@ -634,7 +634,7 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
         for (int nm = 0; nm < NM; ++nm)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float x0 = p[nm][2 * i], x1 = p[nm][2 * i + 1];
+                float x0 = p[nm][2 * i] * kLifted, x1 = p[nm][2 * i + 1] * kLifted;
 #pragma unroll
                 for (int q = 0; COLS < 16 && q < PIECES - 1; ++q) {  // what this lane's piece leaves to the ones before it
                     const unsigned taken = piece_of > q ? 0xFFFF0000u : 0u;
@@ -650,16 +650,10 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
                         u = __builtin_amdgcn_perm(__float_as_uint(x1), __float_as_uint(x0), 0x07060302u);
                     x0 -= __uint_as_float(u << 16);
                     x1 -= __uint_as_float(u & 0xFFFF0000u);
-                    bits[nm][q][i] = __builtin_bit_cast(u16x2, u) - (unsigned short)((127 + (int)kLift) << 7);
+                    bits[nm][q][i] = __builtin_bit_cast(u16x2, u) - (unsigned short)((127 + kLift) << 7);
                 }
             }
         const bool special = masked || __any(w.look & w.look << 1 & 0x80808080u);  // (bytes from 192 on: the two highest bits)
-        if (special) {
-#pragma unroll
-            for (int nm = 0; nm < NM; ++nm)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) p[nm][j] *= kDrop;
-        }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             u32x4 pf[NM][NP];
@@ -712,7 +706,6 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
     for (int nm = 0; nm < NM; ++nm) {
         l[nm] += __shfl_xor(l[nm], 16);
         l[nm] += __shfl_xor(l[nm], 32);
-        l[nm] *= kDrop;
         if constexpr (COLS < 16) {
 #pragma unroll
             for (int i = 0; i < 2 * G; ++i)

@@ -583,7 +583,8 @@ long long after_conv1_act_launches(void);
  * has no effect on it, NaN and infinities included.  Rows of out behind the last sequence stay as they are, or are set to
  * zero with zero_rest.  D = 64 or 128.  fp32: fp32 products; bf16 / fp16: products of that type, sums and softmax in fp32: a
  * probability is rounded to the type before it is multiplied (fp16: what is below 2^-32 of a query's largest counts as 0).
- * Sums are divided at the end: they stay finite while the largest value times the keys that a query sees is below 2^120.
+ * Sums are divided at the end: they stay finite while the largest value times the keys that a query sees is below 2^120.  What is
+ * below 2^-126 of the largest probability counts as 0 in any type.
  * scale: any sign, 0 too, up to 2.35e38 (here and in after_kv4_attend).
  * workspace: scratch of the size that _workspace names (its answer depends on the arguments alone; two calls that may run at the
  * same time need two), with which the keys of a few queries are shared out over the chip; NULL: they are not. */
@@ -653,7 +654,8 @@ int after_kv4_read(const after_kv4* c, void* k, void* v, int type, const int* st
  * in use received, summed over tokens and the group's heads (decay = 0: they are replaced).  Products are of bf16 numbers: cached
  * keys and values are such; a query is cut into one (bf16), two (fp16) or three (fp32) of them, exactly, and a probability into as
  * many, to within 2^-9, 2^-15 or 2^-23 of itself.  The softmax, its sums, the weights and the output before it is rounded are
- * fp32.  Sums are divided at the end: they stay finite while the largest value times the slots that a query sees is below 2^120.
+ * fp32; what is below 2^-126 of the largest probability counts as 0.  Sums are divided at the end: they stay finite while the
+ * largest value times the slots that a query sees is below 2^120.
  * The workspace is scratch: its size depends on the arguments alone (the cache's capacity, not its lengths: with accumulate and up
  * to 32 queries of a row and head, 4 bytes for each of them and every slot), and two calls that may run at the same time need two. */
 int after_kv4_attend_workspace(const after_kv4* c, int type, int heads, int tokens, int accumulate, long long* bytes);

@@ -152,6 +152,26 @@ def test_cached_scores_of_any_size(hip_device, kind, heads, T, capacity, scale):
         close(c.weights[0, 0, :n], weights.double(), 2.0 ** -19 * weights, "weights")
 
 
+@pytest.mark.parametrize("T, heads, capacity", [(1, 4, 64), (1, 4, 640), (1, 12, 640), (1, 24, 640), (20, 2, 640)])
+def test_exponentials_keep_their_32_bits(hip_device, T, heads, capacity):
+    """Scores of one product each, up to 4 in size, over a few slots.  A score is off by 2^-24 of itself, its distance from the maximum
+    by another rounding, at most 3 x 2^-24 x 8 log2 e together, an exponential by two steps, and as much again in the sum."""
+    g = gen(28)
+    k, v = torch.zeros(32, 5, 1, 64), torch.randn(32, 5, 1, 64, generator=g)
+    k[..., 0] = torch.randn(32, 5, 1, generator=g)
+    c = KVCache4(32, 1, 64, capacity, hip_device)
+    c.append(k.to(hip_device), v.to(hip_device))
+    q = torch.zeros(32, T, heads, 64)
+    q[..., 0] = torch.rand(32, T, heads, generator=g) - 0.5
+    out = c.attend(q.to(hip_device), scale=1.5)
+    K, V = ref.cache_values(c)
+    for r in range(32):
+        seen = torch.arange(5) < (5 - T + 1 + torch.arange(T)).view(T, 1)
+        want, _, probs = ref.attention(q[r], K[r, :, :5].transpose(0, 1), V[r, :, :5].transpose(0, 1), seen, 1.5)
+        spread = torch.einsum("nhm,md->nhd", probs, V[r, 0, :5].abs())
+        close(out[r], want, 2 * (24 * math.log(2) + 2) * 2.0 ** -24 * spread + 1e-38, f"row {r}")
+
+
 @pytest.mark.parametrize("kind", list(TYPES))
 def test_many_probabilities_below_the_smallest_of_fp16(hip_device, kind):
     """Every 512th key's score is 25.2 octaves above the others', its value 0: the others weigh 1.3e-5 together."""
