@@ -323,6 +323,7 @@ struct AttendArgs {
     long long qrs, qts, qhs;
     int heads, tokens, group, m_rows;  // m_rows = tokens * group
     int workers;      // waves that share the work (below); 0: a workgroup for each row and head
+    int pieces;       // that part_o and part_ml hold
     float scale2;     // |scale| log2(e), > 0 (a masked score, -inf, stays -inf)
     float q_sign;     // the scale's sign, on the queries
     float* part_o;    // [pieces][m_rows][D]: a piece is one worker's part of a row and head, number worker + row * H + head (many
@@ -432,10 +433,14 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
         const long long mine = min(share, all * c.kv_heads - at);
         if (mine <= 0) return;
         left = (long long)__builtin_amdgcn_readfirstlane((int)(mine >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)mine);
+        // (at < all * H, which the last row's sum reaches, unless another call changes the lengths meanwhile: that is the caller's
+        // mistake, but here, in the join and in eviction every index stays in its range all the same, and every search ends)
         long long before = 0;
-        int r0 = 0;
-        for (;; r0 += 64) {  // (ends: at < all * H, which the last row's sum reaches)
-            long long sum = r0 + lane < c.rows ? row_steps(c, r0 + lane) : 0;
+        int n = 0;
+        r = -1;
+        for (int r0 = 0; r0 < c.rows; r0 += 64) {
+            const int own = r0 + lane < c.rows ? row_steps(c, r0 + lane) : 0;
+            long long sum = own;
 #pragma unroll
             for (int o = 1; o < 64; o *= 2) {
                 const long long y = __shfl_up(sum, o);
@@ -445,13 +450,14 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
             if (past) {
                 const int first = __ffsll(past) - 1;
                 r = r0 + first;
+                n = __shfl(own, first);
                 before += first ? __shfl(sum, first - 1) : 0;
                 break;
             }
             before += __shfl(sum, 63);
         }
+        if (r < 0) return;
         const long long in = at - before * c.kv_heads;
-        const int n = row_steps(c, r);
         h = (int)(in / n);
         step = (int)(in - (long long)h * n);
         // (the same in every lane: kept in scalar registers)
@@ -784,8 +790,9 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
         step = 0;
         if (++h == c.kv_heads) {
             h = 0;
-            do ++r;  // (ends: work is left, so a later row holds it)
-            while (row_length(c, r) == 0);
+            do {
+                if (++r == c.rows) return;  // (work is left, so a later row holds it: as above)
+            } while (row_length(c, r) == 0);
         }
     }
     }
@@ -1140,7 +1147,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttendArgs a) {
     const after_kv4& c = a.c;
     const int rh = blockIdx.x / a.m_rows, m = blockIdx.x % a.m_rows, r = rh / c.kv_heads, h = rh % c.kv_heads;
     const int group = threadIdx.x >> 4, d = (threadIdx.x & 15) * W;
-    const int2 p = a.ends[rh];  // (an empty row has none: not looked at)
+    const int2 ends = a.ends[rh], p = {max(ends.x, 0), min(ends.y, a.pieces - 1)};  // (an empty row has none: not looked at)
     float acc[W] = {};
     if (row_length(c, r) > 0) {
         if (p.x == p.y && !a.final_ml) return;  // (whole: written already)
@@ -1453,7 +1460,7 @@ __global__ __launch_bounds__(256) void kv4_move_kernel(after_kv4 c, after_kv4 to
     if (sb == 0 && lane == 0 && rh % c.kv_heads == 0) to.lengths[r] = n;
     if (m <= 0) return;
     const size_t src = (size_t)rh * c.capacity, dst = (size_t)rh * to.capacity + 8 * sb;
-    const int pick = lane < m ? slots[(size_t)rh * keep + 8 * sb + lane] : 0;  // (slot 0 for what is not there: read, not used)
+    const int pick = lane < m ? max(slots[(size_t)rh * keep + 8 * sb + lane], 0) : 0;  // (slot 0 for what is not there: read, not used)
     u32x2 x[8];
     if (2 * lane < D) {
 #pragma unroll
@@ -1733,6 +1740,7 @@ extern "C" int after_kv4_attend(const after_kv4* c, const after_kv4_query* query
     a.group = x.heads / c->kv_heads;
     a.m_rows = p.m_rows;
     a.workers = 4 * p.wgs;
+    a.pieces = (int)p.pieces;
     a.scale2 = scale_log2(x.scale);
     a.q_sign = x.scale < 0 ? -1.f : 1.f;
     char* w = (char*)x.workspace;
