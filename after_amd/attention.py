@@ -30,7 +30,7 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 def _refuse_gradients(t, name):
     if t.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError(f"{name} requires a gradient: after_amd is inference only (use torch.no_grad())")
-    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:  # (outside of any level a look costs nothing)
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
         raise NotImplementedError(f"{name} carries a tangent: after_amd is inference only")
 
 
@@ -50,7 +50,8 @@ def _operand(t, name, dims, index=None, dtype=None):
         raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
     if dtype is not None and kind is not dtype:
         raise TypeError(f"{name} is {kind}, expected {dtype}")
-    _refuse_gradients(t, name)
+    if t.requires_grad or forward_ad._current_level >= 0:
+        _refuse_gradients(t, name)
     odd = strides[0] | strides[1] | (strides[2] if dims == 4 else 0) | t.data_ptr() // t.element_size()
     # (a token's place in a tile is addressed with 32 bits; what the strides of an empty tensor are does not matter)
     if odd & (3 if kind is torch.float32 else 7) or strides[-1] != 1 or strides[-3] >= 1 << 22:
