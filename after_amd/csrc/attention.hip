@@ -13,8 +13,9 @@
 // grid needs no lengths.
 //
 // What bounds it.  Long prompts: the matrix pipes, with the softmax's exponentials between two products; 16384 causal tokens, bf16,
-// 32 / 8 heads of 128: 2090 us, 1053 TFLOP/s, where a large product of the library reaches 1155 (fp16 heads of 128 in a batch of
-// 1 .. 2047 tokens: 300 us, 725; heads of 64, 8192 tokens: 317 us, 868; fp32 heads of 128, 4096 tokens: 585 us, 118 of 153).
+// 32 / 8 heads of 128: 2070 .. 2200 us from card to card, 1000 .. 1060 TFLOP/s, where a large product of the library reaches 1155
+// (fp16 heads of 128 in a batch of 1 .. 2047 tokens: 297 .. 312 us, 700 .. 735, its workgroups' beginnings and ends stand alone; heads
+// of 64, 8192 tokens: 313 us, 880; fp32 heads of 128, 4096 tokens: 580 us, 118 of 153).
 // Tiles of 64 keys, two of them in LDS and two workgroups on a CU: one computes while the other waits.  Measured and left out:
 // V read by instructions that wait by themselves, and scheduling hints (the same time), skipping the unseen half of a masked
 // tile (2330 us).

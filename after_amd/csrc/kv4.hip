@@ -314,8 +314,10 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(after_kv4 c, void* ko, vo
 // which channel a step of its product contracts are chosen so that a lane's S values are the P operand that it needs next.
 // A cached value is exact in bf16; queries and probabilities travel as bf16 pieces (1 for bf16 queries, 2 for fp16: exact,
 // 3 for fp32: exact), so that what is rounded is never coarser than the output's own type.
-// What bounds it: memory.  64 rows of 1 .. 8192 slots, 8 heads of 128 (296 MB): 57.6 us and 5.3 for the join, 5.1 TB/s; two rows of
-// 131071 with 8 fp16 queries a head, whose scores are written for the weights (285 + 67 MB): 77 us, 4.6 TB/s, as a copy.
+// What bounds it: memory.  64 rows of 1 .. 8192 slots, 8 heads of 128 (296 MB): 57 us and 5.6 for the join, 5.2 TB/s (fp16 61, fp32
+// 66); two rows of 131071 with 8 fp16 queries a head, whose scores are written for the weights (285 + 67 MB): 80 us, 4.4 TB/s: the
+// stores of scores count in the counter that the ring waits on, so that its third tile is asked for late.  24 queries a head, 8 rows
+// of 1 .. 32767: 57 us in bf16, 86 in fp16, 110 in fp32.
 struct AttendArgs {
     after_kv4 c;
     const void* q;
@@ -803,9 +805,11 @@ __global__ __launch_bounds__(256) void kv4_attend_kernel(AttendArgs a) {
 // them per workgroup, 32 to a wave, over the same tiles of 64 tokens.  The tiles are widened to bf16 once for the four waves and
 // kept in LDS in the order in which the matrix instructions take them (a lane's operand is 16 bytes at its own number: no
 // conflicts); while one tile is multiplied the next one's codes are on their way in registers.
-// What bounds it: the vector unit (an exponential and some five more per score, and the widening) and the products in turn.  32
-// tokens of 4 rows of 9001 .. 16384, bf16, 32 / 8 heads of 128: 55 us, 0.5 PFLOP/s, the join 10 (64 KB of sums a piece), the
-// weights, for which the scores are formed again, 38; 8 rows of 1 .. 16384: 151 us in all, 177 with equal splits of each row.
+// What bounds it: waits between phases that depend on each other (one barrier a tile, codes asked for one tile ahead, scores, softmax
+// and product one behind the other inside a wave): the matrix pipes are busy a quarter of the time, the vector unit less than half,
+// and a wave waits 0.4 of its own.  32 tokens of 4 rows of 9001 .. 16384, bf16, 32 / 8 heads of 128: 52 us, 0.5 PFLOP/s, the join 10
+// (64 KB of sums a piece), the weights, for which the scores are formed again, 38.5; 64 tokens of 64 / 8 heads over the same rows
+// 207 and 23, 512 tokens 1163 and 60; 8 rows of 1 .. 16384: 151 us in all, 177 with equal splits of each row.
 constexpr int kWideRows = 128, kWideTile = 64;
 
 template <int D>
