@@ -117,8 +117,10 @@ def attend_packed(q, k, v, q_starts, k_starts=None, *, causal=True, window=None,
 
     causal: a query sees the keys up to its own position; with `chunk` > 1 also the rest of its chunk, and with `window` only the
     newest `window` keys outside its chunk: the mask of DenoiserV2's local attention (transformerv2.py:62-96).  A query that
-    sees nothing gets zeros.  Sums and softmax are fp32; bf16 and fp16 products take probabilities rounded to that type.  Rows behind the last sequence are zeros in a new tensor and left alone in `out`, which must be
-    contiguous and must not overlap q, k or v; it may be q itself."""
+    sees nothing gets zeros.  Sums and softmax are fp32; bf16 and fp16 products take probabilities rounded to that type.
+
+    Rows behind the last sequence are zeros in a new tensor and left alone in `out`, which must be contiguous and must not
+    overlap q, k or v; it may be q itself."""
     chunk, window = int(chunk), None if window is None else int(window)
     if not 1 <= chunk <= 1 << 24 or (window is not None and window < 1):
         raise ValueError(f"chunk must be 1 .. 2^24 and window at least 1, got {chunk} and {window}")

@@ -366,7 +366,7 @@ __global__ __launch_bounds__(256, sizeof(typename Elem<TYPE>::T) * D > 256 ? 1 :
                 for (int s = 0; s < 2; ++s) {
                     typename E::V8 pf;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) pf[e] = (T)sc[f][8 * s + e];  // (the products' own type: half a step, 2^-9 / 2^-12, each)
+                    for (int e = 0; e < 8; ++e) pf[e] = (T)sc[f][8 * s + e];  // (the products' own type: half a step, 2^-8 / 2^-11, each)
 #pragma unroll
                     for (int i = 0; i < DT; ++i) {
                         // lane l of 16 reads 8 bytes of row l / 4: it gets column l of the four rows

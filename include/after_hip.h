@@ -579,13 +579,13 @@ long long after_conv1_act_launches(void);
  * keys: query i of n stands at p = i + (keys - n).  causal: it sees the keys of its own chunk of `chunk` tokens and all chunks
  * before (chunk = 1: the keys up to its own), and with window > 0 of the earlier chunks only keys > p - window, as DenoiserV2's
  * mask does (transformerv2.py:62-96).  causal = 0: all keys.  A query that sees no key gets zeros, one that sees only scores of
- * -infinity NaN; what a query does not see
- * has no effect on it, NaN and infinities included.  Rows of out behind the last sequence stay as they are, or are set to
+ * -infinity NaN; what a query does not see has no effect on it, NaN and infinities included.  Rows of out behind the last sequence stay as they are, or are set to
  * zero with zero_rest.  D = 64 or 128.  fp32: fp32 products; bf16 / fp16: products of that type, sums and softmax in fp32: a
- * probability is rounded to the type before it is multiplied (fp16: what is below 2^-32 of a query's largest counts as 0).
+ * probability is rounded to the type before it is multiplied, by 2^-8 or 2^-11 of itself at most (fp16: what is below 2^-32 of a
+ * query's largest counts as 0).
  * Sums are divided at the end: they stay finite while the largest value times the keys that a query sees is below 2^120.  What is
  * below 2^-126 of the largest probability counts as 0 in any type.
- * scale: any sign, 0 too, up to 2.35e38 (here and in after_kv4_attend).
+ * scale: any sign, 0 too, up to 2.35e38 (here and in after_kv4_attend).  out overlaps neither k nor v, and q only where it is q.
  * workspace: scratch of the size that _workspace names (its answer depends on the arguments alone; two calls that may run at the
  * same time need two), with which the keys of a few queries are shared out over the chip; NULL: they are not. */
 int after_attend_packed_workspace(int type, long long q_rows, long long k_rows, int n_seqs, int heads, int kv_heads, int head_dim,
@@ -649,11 +649,10 @@ int after_kv4_truncate(const after_kv4* c, const int* lengths, void* stream);
 int after_kv4_read(const after_kv4* c, void* k, void* v, int type, const int* start, int count, void* stream);
 /* out [rows, tokens, heads, D] (contiguous, of q's type): attention of the newest `tokens` tokens of each row, whose keys are
  * in the cache already: query t sees the slots below lengths[r] - tokens + t + 1, none of them: zeros; all scores -infinity: NaN,
- * in the output and in the weights of the slots that it sees.  (A row with fewer new
- * tokens than others has its queries at the end.)  accumulate: weights = decay * weights + the probabilities that each slot
- * in use received, summed over tokens and the group's heads (decay = 0: they are replaced).  Products are of bf16 numbers: cached
+ * in the output and in the weights of the slots that it sees.  (A row with fewer new tokens than others has its queries at the
+ * end.)  accumulate: weights = decay * weights + the probabilities that each slot in use received, summed over tokens and the group's heads (decay = 0: they are replaced).  Products are of bf16 numbers: cached
  * keys and values are such; a query is cut into one (bf16), two (fp16) or three (fp32) of them, exactly, and a probability into as
- * many, to within 2^-9, 2^-15 or 2^-23 of itself.  The softmax, its sums, the weights and the output before it is rounded are
+ * many, to within 2^-8, 2^-15 or 2^-23 of itself.  The softmax, its sums, the weights and the output before it is rounded are
  * fp32; what is below 2^-126 of the largest probability counts as 0.  Sums are divided at the end: they stay finite while the
  * largest value times the slots that a query sees is below 2^120.
  * The workspace is scratch: its size depends on the arguments alone (the cache's capacity, not its lengths: with accumulate and up
